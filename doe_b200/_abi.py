@@ -33,6 +33,9 @@ DOE_DEVICE_ERR_TIMEOUT = 0x8
 
 DOE_KV_F16 = 0
 DOE_KV_INT8 = 1
+DOE_KV_INT4 = 2
+KV_INT4_BLOCK_BYTES = 1152
+LOGPROBS_MAX_TOP = 32
 
 # set_upload_behavior usage modes
 DOE_UPLOAD_COPY_DST_COPY_SRC = 0
@@ -170,6 +173,9 @@ SIGNATURES = {
     "doe_paged_decode_ex": (_I, [C.POINTER(PagedKV), _U32, _U32, _P, _P, _P, _P, _F, _P, _U32,
                                  C.POINTER(DecodeOptions), _LP]),
     "doe_paged_gather": (_I, [C.POINTER(PagedKV), _U32, _U32, _U32, _P, _P, _P, _P, _LP]),
+    "doe_paged_read": (_I, [C.POINTER(PagedKV), _U32, _U32, _P, _P, _P, _U32, _LP]),
+    "doe_paged_copy_pages": (_I, [C.POINTER(PagedKV), _P, _U32, _LP]),
+    "doe_token_logprobs": (_I, [_P, _U32, _U64, _U32, _U64, _P, _U32, _P, _P, _P, _P, _LP]),
     "doe_kv_write_dense": (_I, [_P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _LP]),
     "doe_kv_read_dense": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _LP]),
     "doe_rope_f32": (_I, [_P, _P, _U32, _U32, _U32, _U32, _LP]),
@@ -202,6 +208,11 @@ SIGNATURES = {
     "doe_kv_pool_destroy": (_I, [_P]),
     "doe_kv_pool_reserve": (_I, [_P, _U32, _U32]),
     "doe_kv_pool_release": (_I, [_P, _U32]),
+    "doe_kv_pool_truncate": (_I, [_P, _U32, _U32]),
+    "doe_kv_pool_fork": (_I, [_P, _U32, _U32, _U32]),
+    "doe_kv_pool_make_writable": (_I, [_P, _U32, _U32, _U32, _P, _U32, C.POINTER(_U32)]),
+    "doe_kv_pool_compact": (_I, [_P, _P, _U32, C.POINTER(_U32)]),
+    "doe_kv_pool_page_refs": (_I, [_P, _U32, C.POINTER(_U32)]),
     "doe_kv_pool_free_pages": (_I, [_P, C.POINTER(_U32)]),
     "doe_kv_pool_seq_pages": (_I, [_P, _U32, C.POINTER(_U32)]),
     "doe_kv_pool_block_table": (_I, [_P, _P, _U64]),

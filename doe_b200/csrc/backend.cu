@@ -520,6 +520,12 @@ int run_rope(const DispatchCtx& d) {
   return op_result(d.ctx, doe_rope_f32((float*)qk.ptr, (const float*)fc.ptr, u[0], u[2], u[1], u[3], &l));
 }
 
+// Bytes of a K or V pool of the paged cache types.
+uint64_t pool_bytes(uint32_t kv_dtype, uint64_t pages, uint64_t page_size, uint64_t kv_heads, uint64_t head_dim) {
+  if (kv_dtype == DOE_KV_INT4) return pages * kv_heads * (page_size / 16) * DOE_KV_INT4_BLOCK_BYTES;
+  return pages * page_size * kv_heads * head_dim * (kv_dtype == DOE_KV_INT8 ? 1 : 2);
+}
+
 // attention_paged_decode: {num_seqs, num_heads, num_kv_heads, head_dim,
 // page_size, num_pages, max_pages_per_seq, kv_dtype, scale, split_pages};
 // q, k_pool, v_pool, block_table, seq_lens, out, [new_k, new_v], [k_scale, v_scale].
@@ -540,10 +546,10 @@ int run_paged_decode(const DispatchCtx& d) {
   DOE_TRY(resolve(d, 9, u[7] == DOE_KV_INT8, &ks));
   DOE_TRY(resolve(d, 10, u[7] == DOE_KV_INT8, &vs));
   const uint64_t B = u[0], H = u[1], Hkv = u[2], D = u[3], page = u[4], np = u[5], mp = u[6];
-  const uint64_t eb = u[7] == DOE_KV_INT8 ? 1 : 2;
+  const uint64_t pool = pool_bytes(u[7], np, page, Hkv, D);
   DOE_TRY(need(d, q, B * H * D * 2, "q"));
-  DOE_TRY(need(d, kp, np * page * Hkv * D * eb, "k_pool"));
-  DOE_TRY(need(d, vp, np * page * Hkv * D * eb, "v_pool"));
+  DOE_TRY(need(d, kp, pool, "k_pool"));
+  DOE_TRY(need(d, vp, pool, "v_pool"));
   DOE_TRY(need(d, bt, B * mp * 4, "block_table"));
   DOE_TRY(need(d, sl, B * 4, "seq_lens"));
   DOE_TRY(need(d, o, B * H * D * 4, "out"));
@@ -585,11 +591,11 @@ int run_paged_append(const DispatchCtx& d) {
   DOE_TRY(resolve(d, 7, u[7] == DOE_KV_INT8, &ks));
   DOE_TRY(resolve(d, 8, u[7] == DOE_KV_INT8, &vs));
   const uint64_t B = u[0], T = u[1], Hkv = u[2], D = u[3], page = u[4], np = u[5], mp = u[6];
-  const uint64_t eb = u[7] == DOE_KV_INT8 ? 1 : 2;
+  const uint64_t pool = pool_bytes(u[7], np, page, Hkv, D);
   DOE_TRY(need(d, nk, B * T * Hkv * D * 2, "new_k"));
   DOE_TRY(need(d, nv, B * T * Hkv * D * 2, "new_v"));
-  DOE_TRY(need(d, kp, np * page * Hkv * D * eb, "k_pool"));
-  DOE_TRY(need(d, vp, np * page * Hkv * D * eb, "v_pool"));
+  DOE_TRY(need(d, kp, pool, "k_pool"));
+  DOE_TRY(need(d, vp, pool, "v_pool"));
   DOE_TRY(need(d, bt, B * mp * 4, "block_table"));
   DOE_TRY(need(d, pos, B * 4, "positions"));
   doe_paged_kv kv;

@@ -83,6 +83,19 @@ int launch_paged_decode(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t num_
 int launch_paged_append(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tokens,
                         const void* new_k, const void* new_v, const int32_t* positions,
                         const float* freq_cis, uint32_t rope_positions, const doe_launch* launch);
+int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t num_heads, const void* q,
+                             const int32_t* seq_lens, const void* new_k, const void* new_v, float scale, float* out,
+                             uint32_t split_pages, const doe_decode_options* opts, const doe_launch* launch,
+                             uint64_t* ws_needed_out);
+int launch_int4_append(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tokens, const void* new_k,
+                       const void* new_v, const int32_t* positions, const float* freq_cis, uint32_t rope_positions,
+                       const doe_launch* launch);
+int launch_paged_read(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tokens, const int32_t* positions,
+                      void* k_out, void* v_out, uint32_t dtype, const doe_launch* launch);
+int launch_copy_pages(const doe_paged_kv* kv, const int32_t* pairs, uint32_t n, const doe_launch* launch);
+int launch_token_logprobs(const void* logits, uint32_t dtype, uint64_t rows, uint32_t vocab, uint64_t row_stride,
+                          const int32_t* tokens, uint32_t top_k, float* logprob, float* entropy, int32_t* top_ids,
+                          float* top_logprobs, const doe_launch* launch);
 int launch_paged_gather(const doe_paged_kv* kv, uint32_t seq, uint32_t start, uint32_t len,
                         void* k_out, void* v_out, void* ks_out, void* vs_out,
                         const doe_launch* launch);

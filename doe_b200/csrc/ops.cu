@@ -4,6 +4,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <vector>
 
 #include "common.cuh"
 
@@ -49,7 +50,7 @@ int check_paged_kv(const doe_paged_kv* kv, const char* fn) {
   if (!kv) return invalid("%s: kv is null", fn);
   if (!kv->k_pool || !kv->v_pool || !kv->block_table)
     return invalid("%s: k_pool, v_pool and block_table are required", fn);
-  if (kv->kv_dtype > DOE_KV_INT8) return invalid("%s: unknown kv_dtype %u", fn, kv->kv_dtype);
+  if (kv->kv_dtype > DOE_KV_INT4) return invalid("%s: unknown kv_dtype %u", fn, kv->kv_dtype);
   if (kv->kv_dtype == DOE_KV_INT8 && (!kv->k_scale || !kv->v_scale))
     return invalid("%s: int8 pools need k_scale and v_scale", fn);
   if (kv->page_size == 0 || kv->page_size % 16 != 0)
@@ -57,6 +58,23 @@ int check_paged_kv(const doe_paged_kv* kv, const char* fn) {
   if (kv->num_kv_heads == 0 || kv->head_dim == 0 || kv->num_pages == 0)
     return invalid("%s: num_kv_heads, head_dim and num_pages must be positive", fn);
   if (kv->max_pages_per_seq == 0) return invalid("%s: max_pages_per_seq must be positive", fn);
+  if (kv->kv_dtype == DOE_KV_INT4 && kv->head_dim != 128) {
+    set_op_error("%s: int4 pools are built for head_dim 128 (got %u)", fn, kv->head_dim);
+    return DOE_UNSUPPORTED;
+  }
+  return DOE_OK;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// The int4 chunk kernels' own limits.
+int check_int4_chunk(const doe_paged_kv* kv, const char* fn, uint32_t n_tokens, const void* a, const void* b) {
+  if (n_tokens > 0x40000000u || ((uint64_t)n_tokens / 16 + 2) * kv->num_kv_heads > 0x7fffffffull)
+    return invalid("%s: too many tokens (%u) for one launch", fn, n_tokens);
+  if ((uint64_t)kv->page_size > 0x40000000u || kv->max_pages_per_seq > 0x7fffffffu || kv->num_pages > 0x7fffffffu)
+    return invalid("%s: page_size, num_pages and max_pages_per_seq are limited to 31 bits", fn);
+  if (!aligned16(kv->k_pool) || !aligned16(kv->v_pool) || !aligned16(a) || !aligned16(b))
+    return invalid("%s: pools and rows must be 16-byte aligned", fn);
   return DOE_OK;
 }
 
@@ -287,6 +305,12 @@ int doe_paged_append(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_token
   if (!new_k || !new_v || !positions)
     return invalid("doe_paged_append: new_k, new_v and positions are required");
   if (num_seqs > 65535) return invalid("doe_paged_append: at most 65535 sequences per launch");
+  if (kv->kv_dtype == DOE_KV_INT4) {
+    rc = check_int4_chunk(kv, "doe_paged_append", n_tokens, new_k, new_v);
+    if (rc != DOE_OK) return rc;
+    return launch_int4_append(kv, num_seqs, n_tokens, new_k, new_v, positions, nullptr, 0,
+                              launch_or_default(launch));
+  }
   return launch_paged_append(kv, num_seqs, n_tokens, new_k, new_v, positions, nullptr, 0,
                              launch_or_default(launch));
 }
@@ -301,6 +325,12 @@ int doe_paged_append_rope(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_
   if (!new_k || !new_v || !positions)
     return invalid("doe_paged_append_rope: new_k, new_v and positions are required");
   if (num_seqs > 65535) return invalid("doe_paged_append_rope: at most 65535 sequences per launch");
+  if (kv->kv_dtype == DOE_KV_INT4) {
+    rc = check_int4_chunk(kv, "doe_paged_append_rope", n_tokens, new_k, new_v);
+    if (rc != DOE_OK) return rc;
+    return launch_int4_append(kv, num_seqs, n_tokens, new_k, new_v, positions, freq_cis, rope_positions,
+                              launch_or_default(launch));
+  }
   return launch_paged_append(kv, num_seqs, n_tokens, new_k, new_v, positions, freq_cis, rope_positions,
                              launch_or_default(launch));
 }
@@ -310,11 +340,86 @@ int doe_paged_gather(const doe_paged_kv* kv, uint32_t seq, uint32_t start, uint3
                      const doe_launch* launch) {
   int rc = check_paged_kv(kv, "doe_paged_gather");
   if (rc != DOE_OK) return rc;
+  if (kv->kv_dtype == DOE_KV_INT4) {
+    set_op_error("doe_paged_gather: int4 pools are read as values (doe_paged_read)");
+    return DOE_UNSUPPORTED;
+  }
   if (!k_out || !v_out) return invalid("doe_paged_gather: k_out and v_out are required");
   if ((k_scale_out == nullptr) != (v_scale_out == nullptr))
     return invalid("doe_paged_gather: scale outputs go together");
   return launch_paged_gather(kv, seq, start, len, k_out, v_out, k_scale_out, v_scale_out,
                              launch_or_default(launch));
+}
+
+int doe_paged_read(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tokens, const int32_t* positions,
+                   void* k_out, void* v_out, uint32_t dtype, const doe_launch* launch) {
+  int rc = check_paged_kv(kv, "doe_paged_read");
+  if (rc != DOE_OK) return rc;
+  if (!positions || !k_out || !v_out) return invalid("doe_paged_read: positions, k_out and v_out are required");
+  if (dtype > DOE_DTYPE_F32) return invalid("doe_paged_read: unknown dtype %u", dtype);
+  if (num_seqs > 65535) return invalid("doe_paged_read: at most 65535 sequences per launch");
+  if (kv->head_dim % 8 != 0 || (uint64_t)kv->num_kv_heads * kv->head_dim > 0x40000000ull) {
+    set_op_error("doe_paged_read: head_dim must be a multiple of 8 (got %u)", kv->head_dim);
+    return DOE_UNSUPPORTED;
+  }
+  rc = check_int4_chunk(kv, "doe_paged_read", n_tokens, k_out, v_out);
+  if (rc != DOE_OK) return rc;
+  return launch_paged_read(kv, num_seqs, n_tokens, positions, k_out, v_out, dtype, launch_or_default(launch));
+}
+
+int doe_paged_copy_pages(const doe_paged_kv* kv, const int32_t* pairs, uint32_t num_pairs,
+                         const doe_launch* launch) {
+  int rc = check_paged_kv(kv, "doe_paged_copy_pages");
+  if (rc != DOE_OK) return rc;
+  if (num_pairs == 0) return DOE_OK;
+  if (!pairs) return invalid("doe_paged_copy_pages: pairs is null");
+  if (!aligned16(kv->k_pool) || !aligned16(kv->v_pool) ||
+      (kv->kv_dtype == DOE_KV_INT8 && (!aligned16(kv->k_scale) || !aligned16(kv->v_scale))))
+    return invalid("doe_paged_copy_pages: pools and scales must be 16-byte aligned");
+  if (num_pairs > kv->num_pages)
+    return invalid("doe_paged_copy_pages: %u pairs for %u pages", num_pairs, kv->num_pages);
+  try {
+    // copies run at once, so no page may be written twice or written and read
+    std::vector<uint8_t> use(kv->num_pages, 0);  // 1: source, 2: target
+    for (uint32_t i = 0; i < 2 * num_pairs; ++i)
+      if ((uint32_t)pairs[i] >= kv->num_pages) {
+        set_op_error("doe_paged_copy_pages: page %d outside [0, %u)", pairs[i], kv->num_pages);
+        return DOE_OUT_OF_RANGE;
+      }
+    for (uint32_t i = 0; i < num_pairs; ++i) {
+      uint8_t &from = use[(uint32_t)pairs[2 * i]], &to = use[(uint32_t)pairs[2 * i + 1]];
+      if ((from & 2) || to != 0 || pairs[2 * i] == pairs[2 * i + 1])
+        return invalid("doe_paged_copy_pages: page %d or %d is the target of one pair and in another (or itself)",
+                       pairs[2 * i], pairs[2 * i + 1]);
+      from = 1;
+      to = 2;
+    }
+  } catch (...) {
+    set_op_error("doe_paged_copy_pages: out of host memory");
+    return DOE_ERROR;
+  }
+  return launch_copy_pages(kv, pairs, num_pairs, launch_or_default(launch));
+}
+
+int doe_token_logprobs(const void* logits, uint32_t dtype, uint64_t rows, uint32_t vocab, uint64_t row_stride,
+                       const int32_t* tokens, uint32_t top_k, float* logprob, float* entropy, int32_t* top_ids,
+                       float* top_logprobs, const doe_launch* launch) {
+  if (dtype > DOE_DTYPE_F32) return invalid("doe_token_logprobs: unknown dtype %u", dtype);
+  if (vocab == 0 || vocab > 0x7fffffffu) return invalid("doe_token_logprobs: vocab must be 1 .. 2^31 - 1");
+  if (row_stride < vocab) return invalid("doe_token_logprobs: row_stride is below vocab");
+  if (top_k > DOE_LOGPROBS_MAX_TOP)
+    return invalid("doe_token_logprobs: top_k must be at most %u (got %u)", DOE_LOGPROBS_MAX_TOP, top_k);
+  if (rows == 0) return DOE_OK;
+  if (!logits) return invalid("doe_token_logprobs: logits is null");
+  if ((tokens == nullptr) != (logprob == nullptr))
+    return invalid("doe_token_logprobs: tokens and logprob go together");
+  if ((top_k != 0) != (top_ids != nullptr) || (top_k != 0) != (top_logprobs != nullptr))
+    return invalid("doe_token_logprobs: top_ids and top_logprobs go with top_k > 0");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == DOE_DTYPE_F32 ? 4 : 2) != 0)
+    return invalid("doe_token_logprobs: logits must be aligned to their type");
+  if (rows > (1ull << 40) / row_stride + 1) return invalid("doe_token_logprobs: too many elements");
+  return launch_token_logprobs(logits, dtype, rows, vocab, row_stride, tokens, top_k, logprob, entropy, top_ids,
+                               top_logprobs, launch_or_default(launch));
 }
 
 int doe_kv_write_dense(const void* k_proj, const void* v_proj, void* k_cache, void* v_cache,

@@ -768,6 +768,9 @@ int launch_paged_decode(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t num_
                         const void* new_v, float scale, float* out, uint32_t split_pages,
                         const doe_decode_options* opts, const doe_launch* launch,
                         uint64_t* ws_needed_out) {
+  if (kv->kv_dtype == DOE_KV_INT4)
+    return launch_paged_decode_int4(kv, num_seqs, num_heads, q, seq_lens, new_k, new_v, scale, out, split_pages, opts,
+                                    launch, ws_needed_out);
   const uint32_t Hkv = kv->num_kv_heads;
   const uint32_t group = num_heads / Hkv;
   const uint32_t tiles_per_page = kv->page_size / 16;

@@ -7,7 +7,9 @@ status.  Nothing here computes on the host.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
+import numpy as np
 import torch
 
 from . import _abi as abi
@@ -206,6 +208,83 @@ def paged_gather(cache: PagedKVCache, seq: int, start: int, length: int, status=
         ks.data_ptr() if ks is not None else None, vs.data_ptr() if vs is not None else None,
         C.byref(l)))
     return (k, v) if ks is None else (k, v, ks, vs)
+
+
+def paged_read(cache: PagedKVCache, positions, n_tokens: int, dtype=torch.float16, out=None, status=None, stream=None):
+    """kv_read as values: tokens positions[b] .. + n_tokens of every sequence b (block-table
+    row b) -> (k, v) [B, n_tokens, Hkv, D] of dtype (f16, bf16 or f32), for any cache type.
+
+    Rows on unmapped pages are left as they were (zeros without `out`)."""
+    _need(positions, torch.int32, "positions")
+    if dtype not in _DTYPES:
+        raise ValueError("dtype must be float16, bfloat16 or float32")
+    B = _rows_of(cache, positions.numel())
+    shape = (B, int(n_tokens), cache.num_kv_heads, cache.head_dim)
+    if out is None:
+        k, v = torch.zeros((2,) + shape, dtype=dtype, device=positions.device)
+    else:
+        k, v = out
+        for t, n in ((k, "out k"), (v, "out v")):
+            _need(t, dtype, n)
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{n} must be {shape}")
+    kv = cache.struct()
+    l = _launch(0, status, stream, positions.device)
+    abi.check("doe_paged_read", abi.lib().doe_paged_read(
+        C.byref(kv), B, shape[1], positions.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], C.byref(l)))
+    return k, v
+
+
+def _rows_of(cache: PagedKVCache, n: int) -> int:
+    if n > cache.block_table.shape[0]:
+        raise ValueError(f"{n} sequences, the block table has {cache.block_table.shape[0]} rows")
+    return n
+
+
+def paged_copy_pages(cache: PagedKVCache, pairs, stream=None) -> None:
+    """Copies pages pairs[i][0] -> pairs[i][1] (K, V and scales) inside the cache.
+
+    `pairs` [n, 2] is on the host (KvPool.make_writable, KvPool.compact); no
+    page may be a target twice, or a target and a source."""
+    p = np.ascontiguousarray(pairs, dtype=np.int32)
+    if p.size and (p.ndim != 2 or p.shape[1] != 2):
+        raise ValueError("pairs must be [n, 2]")
+    kv = cache.struct()
+    l = _launch(0, None, stream, cache.k_pool.device)
+    abi.check("doe_paged_copy_pages", abi.lib().doe_paged_copy_pages(C.byref(kv), p.ctypes.data, p.size // 2, C.byref(l)))
+
+
+class TokenLogprobs(NamedTuple):
+    """token_logprobs' results; logprob is None without tokens, top_* are [rows, 0] for top_k 0."""
+
+    logprob: torch.Tensor | None   # [rows] f32
+    entropy: torch.Tensor          # [rows] f32
+    top_ids: torch.Tensor          # [rows, top_k] int32
+    top_logprobs: torch.Tensor     # [rows, top_k] f32
+
+
+def token_logprobs(logits, tokens=None, top_k: int = 0, status=None, stream=None) -> TokenLogprobs:
+    """Log probabilities of tokens [rows] int32 under logits [rows, vocab] (f32, f16 or bf16; rows
+    may be strided), each row's entropy (natural logarithm) and its top_k <= 32 alternatives, ties
+    to the lowest index (doe_token_logprobs)."""
+    if not logits.is_cuda or logits.dtype not in _DTYPES or logits.ndim != 2 or logits.stride(1) != 1 \
+            or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        raise ValueError("logits must be a CUDA f32, f16 or bf16 [rows, vocab] tensor with contiguous rows")
+    rows, vocab = logits.shape
+    if tokens is not None:
+        _need(tokens, torch.int32, "tokens")
+        if tokens.numel() != rows:
+            raise ValueError(f"{rows} rows of logits, {tokens.numel()} tokens")
+    dev = logits.device
+    f = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
+    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    l = _launch(0, status, stream, dev)
+    abi.check("doe_token_logprobs", abi.lib().doe_token_logprobs(
+        logits.data_ptr(), _DTYPES[logits.dtype], rows, vocab, max(logits.stride(0), vocab),
+        tokens.data_ptr() if tokens is not None else None, top_k, f[0].data_ptr() if tokens is not None else None,
+        f[1].data_ptr(), ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None, C.byref(l)))
+    return TokenLogprobs(f[0] if tokens is not None else None, f[1], ids, top)
 
 
 def kv_write_dense(k_proj, v_proj, k_cache, v_cache, positions, status=None, stream=None):

@@ -51,6 +51,20 @@ typedef enum doe_status {
 /* KV element types of a paged cache.                                       */
 #define DOE_KV_F16 0u
 #define DOE_KV_INT8 1u /* int8 symmetric + f16 scale per (token, kv head)   */
+/* 4-bit symmetric + f16 scale per (token, kv head, 32 dims); head_dim 128.
+ * s = f16(max|x| / 7), value = (n - 8) * s with n = clamp(rint(x / s), -7, 7)
+ * + 8.  16 tokens of one kv head are one block of 1152 bytes, codes then
+ * scales, so the pools are [num_pages, num_kv_heads, page_size / 16, 1152]
+ * bytes, 16-byte aligned; k_scale and v_scale are not used.
+ *   K codes: 32-bit word [token][t][group] (t < 4) holds dims 32 group + 8 t
+ *     + {0, 2, 4, 6} in the nibbles of its low half (lowest first) and
+ *     + {1, 3, 5, 7} in those of its high half;
+ *   V codes: 16-bit half [token >> 3][g][(token >> 1) & 3][group][token & 1]
+ *     (g < 8) holds dims 32 group + 4 g + {0, 1, 2, 3};
+ *   scales (from byte 1024): K [token][group], V [token >> 1][group][token & 1].
+ * Only finite rows are meaningful.                                          */
+#define DOE_KV_INT4 2u
+#define DOE_KV_INT4_BLOCK_BYTES 1152u
 
 /* Launch context of the operator surface.  `workspace` is device scratch
  * of at least the op's *_workspace_bytes(); `status` is an optional device
@@ -275,7 +289,7 @@ int doe_attention_stitch_f32(const float* partials, uint32_t rows,
                              uint32_t num_shards, uint32_t head_dim, float* out,
                              const doe_launch* launch);
 
-/* A paged KV cache: pools [num_pages * page_size, num_kv_heads, head_dim]
+/* A paged KV cache: f16 / int8 pools [num_pages * page_size, num_kv_heads, head_dim]
  * (attention_head256_f16kv.wgsl:51-63 kv_layout 2, row = page_table[p /
  * page] * page + p % page), one block-table row per sequence.  int8 pools
  * carry f16 scales laid out [num_pages, num_kv_heads, page_size].          */
@@ -284,7 +298,7 @@ typedef struct doe_paged_kv {
   void* v_pool;
   void* k_scale;
   void* v_scale;
-  uint32_t kv_dtype; /* DOE_KV_F16 or DOE_KV_INT8 */
+  uint32_t kv_dtype; /* DOE_KV_F16, DOE_KV_INT8 or DOE_KV_INT4 */
   uint32_t num_pages;
   uint32_t page_size; /* a multiple of 16 */
   uint32_t num_kv_heads;
@@ -390,6 +404,28 @@ int doe_paged_decode_ex(const doe_paged_kv* kv, uint32_t num_seqs,
 int doe_paged_gather(const doe_paged_kv* kv, uint32_t seq, uint32_t start,
                      uint32_t len, void* k_out, void* v_out, void* k_scale_out,
                      void* v_scale_out, const doe_launch* launch);
+
+/* The batched kv_read as values: tokens [positions[b], + n_tokens) of every
+ * sequence b < num_seqs (block-table row b) into k_out / v_out [num_seqs,
+ * n_tokens, Hkv, D] of `dtype` (DOE_DTYPE_*, one rounding of code * scale; f16
+ * pools are converted).  The rows a prefill over a cached prefix reads, or an
+ * export; any pool type (doe_paged_gather copies codes and does not take int4
+ * pools).  Rows on unmapped pages set DOE_DEVICE_ERR_PAGE and are left as they
+ * were.  head_dim a multiple of 8; pools and outputs 16-byte aligned.       */
+int doe_paged_read(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tokens,
+                   const int32_t* positions, void* k_out, void* v_out, uint32_t dtype,
+                   const doe_launch* launch);
+
+/* Copies whole pages (K, V and their scales) inside a cache: page pairs[2 i] to
+ * page pairs[2 i + 1], i < num_pairs, all as if at once.  `pairs` is HOST
+ * memory, read before the call returns: the lists that doe_kv_pool_make_writable
+ * and doe_kv_pool_compact give.  Pages out of range return DOE_OUT_OF_RANGE; a
+ * page that is the target of two pairs, or a target and a source, returns
+ * DOE_INVALID_ARGUMENT; nothing is copied then.  Ordered on the launch's stream
+ * like any kernel: enqueue it after the last write to the sources and before
+ * the first write to the targets.  Pools 16-byte aligned.                   */
+int doe_paged_copy_pages(const doe_paged_kv* kv, const int32_t* pairs, uint32_t num_pairs,
+                         const doe_launch* launch);
 
 /* Dense per-head kv_write / kv_read, the reference's own form
  * (emit_kernel_body.zig:620-760; CPU semantics
@@ -659,6 +695,24 @@ int doe_gelu_tanh_f32(const float* x, float* y, uint64_t n, const doe_launch* la
  * the smallest index mod 256, then the smallest index, wins (the kernel's
  * 256-thread strided scan and left-leaning tree); with none, 0.             */
 int doe_argmax_f32(const float* logits, uint32_t n, uint32_t* token, const doe_launch* launch);
+/* Log probabilities of given tokens with the row's entropy and its top
+ * alternatives, over `rows` rows of `vocab` logits of `dtype` (DOE_DTYPE_*),
+ * rows row_stride >= vocab elements apart (any alignment of the element type):
+ *   logprob[r] = x[r, tokens[r]] - lse_r, entropy[r] = -sum_v p log p (natural
+ *   logarithms), lse_r = log sum_v exp(x[r, v]);
+ *   top_ids / top_logprobs [rows, top_k]: the top_k <= 32 largest logits, in
+ *   descending order, ties to the lowest index (-0 equals +0, NaN counts as
+ *   -inf); past the row's end id -1 and -inf.
+ * A token outside [0, vocab) sets DOE_DEVICE_ERR_POSITION and gets -inf.  A row
+ * of nothing but -inf gives logprob -inf, entropy 0 and top_logprobs -inf; a row
+ * with a NaN or +inf gives NaN for all three.  logprob (with tokens) and entropy
+ * may be null; top_ids and top_logprobs are null when top_k is 0.  Sums are f32;
+ * results do not depend on timing.                                          */
+#define DOE_LOGPROBS_MAX_TOP 32u
+int doe_token_logprobs(const void* logits, uint32_t dtype, uint64_t rows, uint32_t vocab,
+                       uint64_t row_stride, const int32_t* tokens, uint32_t top_k,
+                       float* logprob, float* entropy, int32_t* top_ids,
+                       float* top_logprobs, const doe_launch* launch);
 /* gather.wgsl (:1-24): out[s, d] = table[ids[s] * dim + d] for s < seq_len,
  * d < dim; an id >= table_rows sets DOE_DEVICE_ERR_PAGE and writes zeros.   */
 int doe_gather_rows_f32(const uint32_t* ids, const float* table, uint64_t table_rows,
@@ -677,7 +731,28 @@ int doe_kv_pool_create(uint32_t num_pages, uint32_t page_size,
 int doe_kv_pool_destroy(doe_kv_pool* pool);
 /* Make sequence `seq` able to hold `tokens` tokens (allocates pages).      */
 int doe_kv_pool_reserve(doe_kv_pool* pool, uint32_t seq, uint32_t tokens);
+/* Gives back every page of `seq`: a page is free once no sequence holds it. */
 int doe_kv_pool_release(doe_kv_pool* pool, uint32_t seq);
+/* Gives back the pages of `seq` past its first `tokens` tokens.            */
+int doe_kv_pool_truncate(doe_kv_pool* pool, uint32_t seq, uint32_t tokens);
+/* Sequence `to` (which must hold no page) shares the pages of `from`'s first
+ * `tokens` tokens.                                                          */
+int doe_kv_pool_fork(doe_kv_pool* pool, uint32_t from, uint32_t to, uint32_t tokens);
+/* Call before tokens [first_token, + tokens) of `seq` are written: pages of
+ * that range that other sequences share are replaced by free ones.  Writes
+ * the (old, new) pages to copy (doe_paged_copy_pages, every layer's cache)
+ * into pairs [max_pairs][2] and their number into num_pairs.  Too few free
+ * pages return DOE_OUT_OF_RANGE, too small a list DOE_INVALID_ARGUMENT;
+ * nothing changes then.                                                     */
+int doe_kv_pool_make_writable(doe_kv_pool* pool, uint32_t seq, uint32_t first_token,
+                              uint32_t tokens, int32_t* pairs, uint32_t max_pairs,
+                              uint32_t* num_pairs);
+/* Moves the live pages into the lowest page ids (shared pages once); the
+ * pairs are given as by doe_kv_pool_make_writable, no target is a source.   */
+int doe_kv_pool_compact(doe_kv_pool* pool, int32_t* pairs, uint32_t max_pairs,
+                        uint32_t* num_pairs);
+/* Sequences that hold `page` (0: free).                                     */
+int doe_kv_pool_page_refs(const doe_kv_pool* pool, uint32_t page, uint32_t* out);
 int doe_kv_pool_free_pages(const doe_kv_pool* pool, uint32_t* out);
 int doe_kv_pool_seq_pages(const doe_kv_pool* pool, uint32_t seq, uint32_t* out);
 /* Writes the [max_seqs, max_pages_per_seq] int32 table (-1 = unmapped).    */

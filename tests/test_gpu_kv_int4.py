@@ -1,0 +1,353 @@
+"""GPU parity of the 4-bit paged KV cache: append and read (exact), attention.
+
+Attention tolerance, from the kernel's roundings: every p and every product of
+p with a V scale is rounded to f16 (2^-11 relative each at most), sums and
+statistics are f32, scores are off by at most about 1e-5 (f32 accumulation of
+128 products) and exponentials by 2^-22:
+  |o - ref| <= 2^-10 (1 + 2^-4) A + 2e-5 max|v|,  A = sum p |v| / sum p,
+bf16 outputs are rounded once more (2^-8 |ref|).
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from doe_b200 import ops
+from doe_b200._abi import DOE_DEVICE_ERR_LENGTH, DOE_DEVICE_ERR_PAGE, DOE_DEVICE_ERR_POSITION, DoeError
+from doe_b200.decoder import rope_table
+from doe_b200.kv import PagedKVCache
+from oracle import kv_int4
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def _t(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def _table(g, lens, page, spare=1):
+    need = [-(-int(n) // page) for n in lens]
+    total = sum(need) + spare
+    perm = g.permutation(total).astype(np.int32)
+    table = np.full((len(lens), max(need) + 1), -1, np.int32)
+    o = 0
+    for b, n in enumerate(need):
+        table[b, :n] = perm[o:o + n]
+        o += n
+    return table, total
+
+
+def _rows(g, shape, std=1.0):
+    return (g.standard_normal(shape) * std).astype(np.float16)
+
+
+class Case:
+    """Sequences of `lens` tokens in an int4 cache, filled through the oracle."""
+
+    def __init__(self, seed, lens, Hkv=2, group=4, page=16, std=1.0, vstd=1.0):
+        g = self.g = np.random.default_rng(seed)
+        self.lens, self.Hkv, self.H, self.page = np.asarray(lens, np.int32), Hkv, Hkv * group, page
+        self.table, self.pages = _table(g, self.lens, page)
+        B, T = len(lens), int(max(lens))
+        self.k, self.v = _rows(g, (B, T, Hkv, 128), std), _rows(g, (B, T, Hkv, 128), vstd)
+        # unwritten bytes hold anything, also scales that are infinite or NaN
+        self.kp, self.vp = (g.integers(0, 256, (self.pages, Hkv, page // 16, 1152)).astype(np.uint8) for _ in range(2))
+        for b in range(B):
+            n = int(self.lens[b])
+            if n:
+                kv_int4.append(self.kp, self.vp, self.table[b:b + 1], page, self.k[b:b + 1, :n], self.v[b:b + 1, :n],
+                               np.zeros(1, np.int64))
+        self.q = _rows(g, (B, self.H, 128))
+
+    def cache(self):
+        return PagedKVCache.from_pools(_t(self.kp), _t(self.vp), page_size=self.page, num_kv_heads=self.Hkv,
+                                       head_dim=128, block_table=_t(self.table), kv_dtype="int4")
+
+    def values(self, b, k=None, v=None):
+        out = []
+        for x in (self.k if k is None else k, self.v if v is None else v):
+            out.append(kv_int4.values(*kv_int4.quantize(x[b, :self.lens[b]])))
+        return out
+
+    def check(self, out, scale, window=0, softcap=0.0, q=None, k=None, v=None, bf16=False):
+        q = self.q if q is None else q
+        for b in range(len(self.lens)):
+            kk, vv = self.values(b, k, v)
+            ref, a = kv_int4.attend(q[b], kk, vv, scale, window, softcap)
+            bound = 2.0 ** -10 * (1 + 2.0 ** -4) * a + 2e-5 * (np.abs(vv).max() if len(vv) else 0.0) + 1e-30
+            if bf16:
+                bound = bound + 2.0 ** -8 * np.abs(ref)
+            err = np.abs(out[b].astype(np.float64) - ref)
+            assert (err <= bound).all(), (b, self.lens[b], float((err / bound).max()))
+
+
+def _decode(c, cache=None, **kw):
+    status = ops.status_word()
+    out = ops.paged_decode(cache or c.cache(), _t(c.q), _t(c.lens), kw.pop("scale", 128 ** -0.5), status=status, **kw)
+    assert int(status.item()) == 0
+    return out.float().cpu().numpy()
+
+
+@pytest.mark.parametrize("Hkv,group", [(1, 1), (2, 2), (1, 3), (2, 4), (1, 5), (1, 6), (1, 7), (2, 8)])
+def test_decode_head_groups(Hkv, group):
+    c = Case(Hkv * 10 + group, [0, 1, 2, 15, 16, 17, 33, 64, 65, 300], Hkv, group)
+    c.check(_decode(c), 128 ** -0.5)
+
+
+@pytest.mark.parametrize("page", [16, 32, 48, 64])
+@pytest.mark.parametrize("split_pages", [0, 1, 3])
+def test_decode_pages_and_splits(page, split_pages):
+    c = Case(page + split_pages, [1, 47, 48, 49, 700, 0, 129], 2, 4, page)
+    out = _decode(c, split_pages=split_pages)
+    c.check(out, 128 ** -0.5)
+    assert np.array_equal(out, _decode(c, split_pages=split_pages)), "results depend on timing"
+
+
+@pytest.mark.parametrize("window,softcap", [(1, 0.0), (16, 0.0), (17, 30.0), (100, 0.0), (5000, 5.0), (0, 50.0)])
+def test_decode_window_and_softcap(window, softcap):
+    c = Case(window, [0, 1, 16, 17, 99, 100, 101, 257], 1, 4)
+    c.check(_decode(c, sliding_window=window, softcap=softcap, scale=0.3), 0.3, window, softcap)
+    c.check(_decode(c, sliding_window=window, softcap=softcap, scale=0.3, split_pages=2), 0.3, window, softcap)
+
+
+@pytest.mark.parametrize("std,vstd,scale", [(1.0, 1e-4, 0.1), (1.0, 3e-6, 0.1), (1.0, 900.0, 0.1), (6.0, 12000.0, 0.2),
+                                            (100.0, 1.0, 1.0), (1e-3, 1.0, 0.1), (1.0, 1.0, 0.0)])
+def test_decode_magnitudes(std, vstd, scale):
+    """V from f16's subnormals to its largest values, one-hot and flat softmaxes."""
+    c = Case(7, [1, 40, 333], 1, 4, std=std, vstd=vstd)
+    c.v = np.clip(c.v.astype(np.float32), -65504, 65504).astype(np.float16)
+    c = _refill(c)
+    out = _decode(c, scale=scale)
+    assert np.isfinite(out).all()
+    # scores of hundreds are off by 2^-23 of their size
+    for b in range(3):
+        kk, vv = c.values(b)
+        ref, a = kv_int4.attend(c.q[b], kk, vv, scale)
+        sc = np.abs(np.einsum("hd,td->ht", np.abs(c.q[b].astype(np.float64)), np.abs(kk[:, 0]))).max() * scale
+        bound = (2.0 ** -10 * (1 + 2.0 ** -4) + sc * 2.0 ** -22) * a + 2e-5 * np.abs(vv).max()
+        assert (np.abs(out[b] - ref) <= bound).all()
+
+
+def _refill(c):
+    for b in range(len(c.lens)):
+        n = int(c.lens[b])
+        kv_int4.append(c.kp, c.vp, c.table[b:b + 1], c.page, c.k[b:b + 1, :n], c.v[b:b + 1, :n], np.zeros(1, np.int64))
+    return c
+
+
+def test_decode_reference_follows_scores_and_scales():
+    """Scores that rise along the sequence and V scales that jump late."""
+    c = Case(8, [400], 1, 4, std=0.2)
+    ramp = np.linspace(0, 6, 400)[None, :, None, None]
+    c.k = (np.sign(c.q[:, :1, None, :].transpose(0, 1, 2, 3)) * ramp).astype(np.float16).reshape(1, 400, 1, 128)
+    c.v = c.v * np.where(np.arange(400) == 390, 2000.0, 0.05)[None, :, None, None].astype(np.float16)
+    c.v = c.v.astype(np.float16)
+    c = _refill(c)
+    c.check(_decode(c, scale=0.3), 0.3)
+    c.check(_decode(c, scale=-0.3, split_pages=1), -0.3)
+
+
+@pytest.mark.parametrize("rope", [False, True])
+@pytest.mark.parametrize("stable", [False, True])
+def test_decode_fused_append(rope, stable):
+    c = Case(21, [1, 2, 15, 16, 17, 31, 32, 33, 65, 300], 2, 4)
+    B = len(c.lens)
+    nk, nv = _rows(c.g, (B, 2, 128)), _rows(c.g, (B, 2, 128), 3.0)
+    cis = rope_table(301, 128, 10000.0)
+    last = c.lens.astype(np.int64) - 1
+    rk, q = (kv_int4.rotate(nk, last, cis), kv_int4.rotate(c.q, last, cis)) if rope else (nk, c.q)
+    cache = c.cache()
+    out = _decode(c, cache, new_k=_t(nk), new_v=_t(nv), freq_cis=_t(cis) if rope else None, inputs_stable=stable,
+                  split_pages=1)
+    k, v = c.k.copy(), c.v.copy()
+    for b in range(B):
+        k[b, last[b]], v[b, last[b]] = rk[b], nv[b]
+    c.check(out, 128 ** -0.5, q=q, k=k, v=v)
+    kv_int4.append(c.kp, c.vp, c.table, 16, rk[:, None], nv[:, None], last)
+    assert np.array_equal(cache.k_pool.cpu().numpy(), c.kp), "the append wrote other K bytes"
+    assert np.array_equal(cache.v_pool.cpu().numpy(), c.vp), "the append wrote other V bytes"
+
+
+def test_decode_bf16_and_kept_workspace():
+    c = Case(22, [5, 700, 64], 2, 4)
+    cache = c.cache()
+    ws = ops.decode_workspace(cache, 3, c.H, split_pages=2)
+    for _ in range(3):
+        out = _decode(c, cache, split_pages=2, ws=ws, out_dtype=torch.bfloat16)
+        c.check(out, 128 ** -0.5, bf16=True)
+
+
+def test_decode_on_a_side_stream():
+    c = Case(23, [260, 31], 1, 4)
+    cache, q, n = c.cache(), _t(c.q), _t(c.lens)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    out = ops.paged_decode(cache, q, n, 128 ** -0.5, stream=s)
+    s.synchronize()
+    c.check(out.cpu().numpy(), 128 ** -0.5)
+
+
+def test_decode_reports_bad_pages_and_lengths():
+    c = Case(24, [40, 40], 1, 4)
+    cache = c.cache()
+    status = ops.status_word()
+    table = c.table.copy()
+    table[0, 1] = c.pages + 3
+    cache.set_block_table(table)
+    ops.paged_decode(cache, _t(c.q), _t(c.lens), 0.1, status=status)
+    assert int(status.item()) == DOE_DEVICE_ERR_PAGE
+    status.zero_()
+    cache.set_block_table(c.table)
+    long = c.lens.copy()
+    long[1] = 10 ** 6  # clamped to the block table's row, which ends unmapped
+    out = ops.paged_decode(cache, _t(c.q), _t(long), 128 ** -0.5, status=status)
+    assert int(status.item()) & DOE_DEVICE_ERR_LENGTH
+    ref, a = kv_int4.attend(c.q[0], *c.values(0), 128 ** -0.5)
+    assert (np.abs(out[0].cpu().numpy() - ref) <= 2.0 ** -9 * a + 1e-4).all()
+    status.zero_()
+    neg = c.lens.copy()
+    neg[0] = -5
+    out = ops.paged_decode(cache, _t(c.q), _t(neg), 0.1, status=status)
+    assert int(status.item()) == DOE_DEVICE_ERR_LENGTH and not out[0].any()
+
+
+def test_decode_long_sequence_splits_and_far_pages():
+    """130k tokens in 64-token pages: many splits per row, page walks across every prefetch register."""
+    g = np.random.default_rng(3)
+    n, page = 130001, 64
+    np_pages = -(-n // page)
+    cache = PagedKVCache(num_pages=np_pages, page_size=page, num_kv_heads=1, head_dim=128,
+                         block_table=g.permutation(np_pages).astype(np.int32)[None], kv_dtype="int4")
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    k = torch.randn((1, n, 1, 128), generator=gen, device="cuda").half()
+    v = torch.randn((1, n, 1, 128), generator=gen, device="cuda").half()
+    ops.paged_append(cache, k, v, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    q = torch.randn((1, 8, 128), generator=gen, device="cuda").half()
+    kk, vv = ops.paged_read(cache, torch.zeros(1, dtype=torch.int32, device="cuda"), n, dtype=torch.float32)
+    x = (q[0].double() @ kk[0, :, 0].double().T) / 128 ** 0.5
+    p = torch.softmax(x, -1)
+    ref, a = p @ vv[0, :, 0].double(), p @ vv[0, :, 0].double().abs()
+    for split in (0, 8, 100):
+        out = ops.paged_decode(cache, q, torch.tensor([n], dtype=torch.int32, device="cuda"), 128 ** -0.5,
+                               split_pages=split)[0].double()
+        assert bool(((out - ref).abs() <= 2.0 ** -10 * 1.1 * a + 1e-4).all())
+
+
+@pytest.mark.parametrize("rope", [False, True])
+@pytest.mark.parametrize("Hkv,page,T", [(1, 16, 1), (2, 16, 2), (8, 16, 15), (2, 32, 16), (1, 48, 17), (4, 16, 50), (3, 64, 33)])
+def test_append_is_exact(Hkv, page, T, rope):
+    g = np.random.default_rng(T)
+    starts = np.array([0, 1, 7, 8, 15, 16, 31, 90], np.int32)
+    table, pages = _table(g, starts + T, page)
+    k, v = _rows(g, (8, T, Hkv, 128), 2.0), _rows(g, (8, T, Hkv, 128), 0.01)
+    k[0, 0] = 0
+    v[1, 0, 0, :40] = 65504
+    v[2, 0, 0] = 6e-8
+    k[3, 0, 0, :7] = np.array([7, 0.5, 1.5, 2.5, -0.5, -1.5, 6.5])  # ties where that group's scale is 1
+    k[3, 0, 0, 7:32] = 0
+    cis = rope_table(200, 128, 10000.0) if rope else None
+    kp, vp = (g.integers(0, 256, (pages, Hkv, page // 16, 1152)).astype(np.uint8) for _ in range(2))
+    cache = PagedKVCache.from_pools(_t(kp), _t(vp), page_size=page, num_kv_heads=Hkv, head_dim=128,
+                                    block_table=_t(table), kv_dtype="int4")
+    status = ops.status_word()
+    ops.paged_append(cache, _t(k), _t(v), _t(starts), status=status, freq_cis=_t(cis) if rope else None)
+    kv_int4.append(kp, vp, table, page, k, v, starts.astype(np.int64), cis)
+    assert int(status.item()) == 0
+    assert np.array_equal(cache.k_pool.cpu().numpy(), kp)
+    assert np.array_equal(cache.v_pool.cpu().numpy(), vp)
+    # and back, as values: exact in f32, rounded once in f16 and bf16
+    rk = kv_int4.rotate(k, starts[:, None] + np.arange(T), cis) if rope else k
+    want = [kv_int4.values(*kv_int4.quantize(x)) for x in (rk, v)]
+    for dt in (torch.float32, torch.float16, torch.bfloat16):
+        got = ops.paged_read(cache, _t(starts), T, dtype=dt, status=status)
+        for a, w in zip(got, want):
+            assert torch.equal(a.cpu(), torch.from_numpy(w.astype(np.float32)).to(dt))
+    assert int(status.item()) == 0
+
+
+def test_append_every_scale_and_code():
+    """Rows over f16's whole exponent range, so scales reach its subnormals, zero and 9358."""
+    g = np.random.default_rng(5)
+    mag = 2.0 ** np.linspace(-25, 16, 512)
+    k = np.clip(g.standard_normal((1, 512, 1, 128)) * mag[None, :, None, None], -65504, 65504).astype(np.float16)
+    v = (g.integers(-14, 15, (1, 512, 1, 128)) / 2 * mag[::-1][None, :, None, None] / 16).astype(np.float16)  # ties
+    table, pages = _table(g, [512], 16)
+    cache = PagedKVCache(num_pages=pages, page_size=16, num_kv_heads=1, head_dim=128, block_table=table, kv_dtype="int4")
+    kp, vp = (np.zeros((pages, 1, 1, 1152), np.uint8) for _ in range(2))
+    ops.paged_append(cache, _t(k), _t(v), torch.zeros(1, dtype=torch.int32, device="cuda"))
+    kv_int4.append(kp, vp, table, 16, k, v, np.zeros(1, np.int64))
+    assert np.array_equal(cache.k_pool.cpu().numpy(), kp)
+    assert np.array_equal(cache.v_pool.cpu().numpy(), vp)
+
+
+def test_append_and_read_leave_unmapped_rows():
+    g = np.random.default_rng(6)
+    table = np.array([[0, -1], [1, 2], [3, 3]], np.int32)
+    cache = PagedKVCache(num_pages=3, page_size=16, num_kv_heads=2, head_dim=128, block_table=table, kv_dtype="int4")
+    k, v = _rows(g, (3, 20, 2, 128)), _rows(g, (3, 20, 2, 128))
+    starts = np.array([4, 30, -1], np.int32)  # runs into unmapped pages, off the table, negative
+    kp, vp = (np.zeros((3, 2, 1, 1152), np.uint8) for _ in range(2))
+    status = ops.status_word()
+    ops.paged_append(cache, _t(k), _t(v), _t(starts), status=status)
+    assert int(status.item()) == DOE_DEVICE_ERR_PAGE
+    kv_int4.append(kp, vp, table[:2], 16, k[:2], v[:2], starts[:2].astype(np.int64))
+    assert np.array_equal(cache.k_pool.cpu().numpy(), kp) and np.array_equal(cache.v_pool.cpu().numpy(), vp)
+    status.zero_()
+    out = [torch.full((3, 20, 2, 128), 9.0, device="cuda") for _ in range(2)]
+    ops.paged_read(cache, _t(starts), 20, dtype=torch.float32, out=out, status=status)
+    assert int(status.item()) == DOE_DEVICE_ERR_PAGE
+    got = out[0].cpu().numpy()
+    want = kv_int4.values(*kv_int4.quantize(k))
+    assert np.array_equal(got[0, :12], want[0, :12].astype(np.float32)) and (got[0, 12:] == 9).all()
+    assert np.array_equal(got[1, :2], want[1, :2].astype(np.float32)) and (got[1, 2:] == 9).all()
+    assert (got[2] == 9).all()
+
+
+def test_append_rope_beyond_the_table_reports():
+    cache = PagedKVCache(num_pages=2, page_size=16, num_kv_heads=1, head_dim=128, block_table=np.array([[0, 1]]),
+                         kv_dtype="int4")
+    k = torch.ones((1, 4, 1, 128), dtype=torch.float16, device="cuda")
+    status = ops.status_word()
+    ops.paged_append(cache, k, k, torch.tensor([8], dtype=torch.int32, device="cuda"), status=status,
+                     freq_cis=_t(rope_table(10, 128, 10000.0)))
+    assert int(status.item()) == DOE_DEVICE_ERR_POSITION
+
+
+@pytest.mark.parametrize("kv_dtype", ["f16", "int8"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_read_of_f16_and_int8_caches(kv_dtype, D):
+    g = np.random.default_rng(D)
+    starts, T = np.array([0, 3, 16, 40], np.int32), 19
+    table, pages = _table(g, starts + T, 16)
+    cache = PagedKVCache(num_pages=pages, page_size=16, num_kv_heads=3, head_dim=D, block_table=table, kv_dtype=kv_dtype)
+    k, v = _rows(g, (4, T, 3, D)), _rows(g, (4, T, 3, D), 5.0)
+    ops.paged_append(cache, _t(k), _t(v), _t(starts))
+    for dt in (torch.float32, torch.float16, torch.bfloat16):
+        got = ops.paged_read(cache, _t(starts), T, dtype=dt)
+        for a, x in zip(got, (k, v)):
+            w = torch.from_numpy(x).float()
+            if kv_dtype == "int8":
+                s = (w.abs().amax(-1, keepdim=True) / 127).half().float()
+                w = torch.clamp(torch.round(w / s), -127, 127) * s
+            assert torch.equal(a.cpu(), w.to(dt))
+
+
+def test_refusals():
+    cache = PagedKVCache(num_pages=2, page_size=16, num_kv_heads=1, head_dim=128, block_table=np.array([[0, 1]]),
+                         kv_dtype="int4")
+    with pytest.raises(DoeError):
+        ops.paged_gather(cache, 0, 0, 4)
+    with pytest.raises(ValueError):
+        ops.paged_read(cache, torch.zeros(2, dtype=torch.int32, device="cuda"), 1)  # two sequences, one table row
+    with pytest.raises(ValueError):
+        ops.paged_read(cache, torch.zeros(1, dtype=torch.int32, device="cuda"), 1, dtype=torch.int8)
+    with pytest.raises(ValueError):
+        PagedKVCache(num_pages=2, page_size=16, num_kv_heads=1, head_dim=64, block_table=np.array([[0]]), kv_dtype="int4")
+    with pytest.raises(ValueError):
+        PagedKVCache.from_pools(cache.k_pool[:1], cache.v_pool, page_size=16, num_kv_heads=1, head_dim=128,
+                                block_table=cache.block_table, kv_dtype="int4")
+    with pytest.raises(ValueError):
+        PagedKVCache.from_pools(cache.k_pool, cache.v_pool, page_size=16, num_kv_heads=1, head_dim=128,
+                                block_table=cache.block_table.cpu(), kv_dtype="int4")

@@ -27,17 +27,29 @@
 // subnormals whatever the magnitude of V.  It is lazy: it moves only when a
 // score exceeds it by 2^8 or a V scale exceeds the exponent.
 //
-// Loads: one warp consumes one 16-token block per step out of a ring of its own
-// that two bulk copies (K block, V block, 1152 contiguous bytes each) fill.
+// Loads: a warp walks its blocks kStep at a time out of a ring of its own in
+// shared memory, filled with cp.async: a block is 1024 + 128 contiguous bytes
+// of K and of V, 5 instructions for the warp.  (One elected lane issuing two
+// bulk copies costs the warp some 45 instructions, waits included, of about 270
+// a block: 128 us for 64 sequences of 1k-8k tokens.)
+//
+// Splits: see plan().  Where a row has many, up to 8 of them form a cluster and
+// join in distributed shared memory, each CTA a slice of the dims; the clusters
+// are stitched per slice by the last one to arrive.  Sums go in split order, so
+// results do not depend on timing.
+#include <cooperative_groups.h>
+
 #include "int4.cuh"
-#include "tma.cuh"
 
 namespace doe {
 namespace i4 {
 
+namespace cg = cooperative_groups;
+
 constexpr int kD = 128;
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
+constexpr int kStep = 2;                       // blocks per loop step
+constexpr int kStages = 6;                     // ring slots, a multiple of kStep
 constexpr int kPageRegs = 4;                   // page ids per lane: 128 blocks per warp, 512 per split
 constexpr int kMaxSplitTiles = kWarps * 32 * kPageRegs;
 constexpr int kSlot = 2 * kI4Block;            // K block, V block
@@ -54,9 +66,9 @@ struct Args {
   const __half* new_k;  // [B, Hkv, 128] or null
   const __half* new_v;
   float* out;           // [B, H, 128] f32, or bf16 storage when out_bf16
-  float* part_o;        // [B * Hkv * max_splits, group, 128]
-  float* part_ml;       // [B * Hkv * max_splits, group, 2]
-  unsigned* counters;   // [B * Hkv], zero at launch, left zero by the stitch
+  float* part_o;        // [B * Hkv * max_parts, group, 128]
+  float* part_ml;       // [B * Hkv * max_parts, slices, group, 2]
+  unsigned* counters;   // [B * Hkv, slices], zero at launch, left zero by the stitch
   int32_t* status;
   const float* freq_cis;
   int rope_positions;
@@ -65,7 +77,7 @@ struct Args {
   float scale;
   int num_heads, num_kv_heads, group, num_pages, page_size, max_pages;
   int tiles_per_page, tile_shift;  // page_size / 16 and its log2 (-1: not a power of two)
-  int split_tiles, max_splits;
+  int split_tiles, max_parts;  // blocks per split; clusters (or single splits) per row
   int out_bf16;
   int inputs_stable;
 };
@@ -74,6 +86,24 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+// mma_16816 with a start value apart from the result
+__device__ __forceinline__ void mma_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
@@ -125,7 +155,7 @@ struct AppendRow {
       rope_table<2>(a.freq_cis, a.rope_positions, kD / 2, pos, 4 * (lane & 15), a.status, lane == 0, rc, rsn);
   }
 
-  // Ends with the fence that lets this warp's later bulk copies read the row.
+  // Ends with the barrier that lets the warp's later copies read the row.
   __device__ __forceinline__ void store(const Args& a, int g, int lane) {
     if ((unsigned)page >= (unsigned)a.num_pages) {
       if (lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
@@ -170,19 +200,21 @@ struct AppendRow {
           *reinterpret_cast<__half*>(dst + kI4Codes + (((tok >> 1) * 4 + group) * 2 + (tok & 1)) * 2) = sh;
       }
     }
-    asm volatile("fence.proxy.async.global;\n" ::: "memory");
+    __threadfence_block();
     __syncwarp();
   }
 };
 
+constexpr float kNone = -1e30f;  // the reference of a head without keys: below any score
 constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
 constexpr float kTwo24 = 16777216.0f;
 
 template <bool CAP>
-__global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Args a) {
+__global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
   extern __shared__ __align__(128) uint8_t ring[];
   if (!a.inputs_stable) pdl_wait();
   const int split = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
+  const int slices = (int)cg::this_cluster().num_blocks();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
   const int Hkv = a.num_kv_heads, group = a.group;
@@ -196,23 +228,17 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Args a) {
   const int tile_origin = min_key >> 4;
   const int ntiles = ((seq_len + 15) >> 4) - tile_origin;
   const int nsplits = max(1, (ntiles + a.split_tiles - 1) / a.split_tiles);
-  if (split >= nsplits) return;
+  const int part = split / slices, nparts = (nsplits + slices - 1) / slices;
+  if (part >= nparts) return;  // the whole cluster; a split past the last one joins with nothing
   const int tile_begin = split * a.split_tiles;  // relative to tile_origin
   const int tile_end = min(ntiles, tile_begin + a.split_tiles);
   const int32_t* table = a.block_table + (size_t)b * a.max_pages;
 
   __shared__ float sm_m[kWarps][8];
   __shared__ float sm_l[kWarps][8];
+  __shared__ float cta_ml[8][2];
   __shared__ int sm_last;
   __shared__ int sm_pg[kWarps][32 * kPageRegs];
-  __shared__ __align__(8) uint64_t ring_bar[kWarps][kStages];
-
-  if (lane == 0) {
-#pragma unroll
-    for (int st = 0; st < kStages; ++st) mbar_init(smem_addr(&ring_bar[warp][st]), 1);
-    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-  }
-  __syncwarp();
 
   // this warp's blocks: first + kWarps * k, k < nt; page ids up front
   const int first = tile_origin + tile_begin + warp;
@@ -225,40 +251,45 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Args a) {
   __syncwarp();
 
   const uint32_t wbase = smem_addr(ring) + warp * kWarpBytes;
-  // Fills slot k % kStages with block k (whole warp calls, one lane issues).  A
-  // block of a bad page gets a plain arrival; the consumer reports the page.
+  const size_t head_bytes = (size_t)a.tiles_per_page * kI4Block;
+  const uint8_t* k_head = a.k_pool + g * head_bytes + 16 * lane;
+  const uint8_t* v_head = a.v_pool + g * head_bytes + 16 * lane;
+  // lanes 0-7 copy the K scales, 8-15 the V scales
+  const ptrdiff_t s_off = (lane < 8 ? k_head : v_head - 128) + kI4Codes - k_head;
+  const uint32_t s_dst = kI4Codes + 16 * lane + (lane < 8 ? 0 : kI4Block - 128);
+  const size_t page_bytes = (size_t)Hkv * head_bytes;
+  // Fills slot k % kStages with block k (nothing past the walk, or for a bad page)
   auto issue = [&](int k) {
-    if (lane != 0) return;
-    const int page = sm_pg[warp][k];
-    const uint32_t bar = smem_addr(&ring_bar[warp][k % kStages]);
-    if ((unsigned)page >= (unsigned)a.num_pages) {
-      mbar_arrive(bar);
-      return;
+    if (k < nt) {
+      const int page = sm_pg[warp][k];
+      if ((unsigned)page < (unsigned)a.num_pages) {
+        const int tile = first + kWarps * k;
+        const size_t off =
+            (size_t)page * page_bytes + (size_t)((tile - page_index(tile) * a.tiles_per_page) * kI4Block);
+        const uint32_t dst = wbase + (uint32_t)(k % kStages) * kSlot;
+        copy16(dst + 16 * lane, k_head + off);
+        copy16(dst + 16 * lane + 512, k_head + off + 512);
+        copy16(dst + 16 * lane + kI4Block, v_head + off);
+        copy16(dst + 16 * lane + kI4Block + 512, v_head + off + 512);
+        if (lane < 16) copy16(dst + s_dst, k_head + off + s_off);
+      }
     }
-    const int tile = first + kWarps * k;
-    const int in_page = tile - page_index(tile) * a.tiles_per_page;
-    const size_t off = (((size_t)page * Hkv + g) * a.tiles_per_page + in_page) * kI4Block;
-    const uint32_t dst = wbase + (k % kStages) * kSlot;
-    // this warp read the slot's previous block through the generic proxy
-    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    mbar_expect_tx(bar, kSlot);
-    bulk_load(dst, a.k_pool + off, kI4Block, bar);
-    bulk_load(dst + kI4Block, a.v_pool + off, kI4Block, bar);
   };
 
   // first copies before the query work (and before griddepcontrol.wait when the
-  // caller vouches for the inputs), except the block the append writes
+  // caller vouches for the inputs), from the block the append writes on after it
   const bool appends = a.new_k != nullptr && split == nsplits - 1 && seq_len > 0;
   const int new_tile = ((seq_len - 1) >> 4) - tile_origin - tile_begin;  // split-relative
-  int issued = 0;
-  for (; issued < kStages - 1 && issued < nt; ++issued)
-    if (appends && new_tile == warp + kWarps * issued) break;
-    else issue(issued);
+  // the warp whose walk holds the new row's block appends the row itself; that
+  // block is the walk's last
+  const bool append_pending = appends && new_tile % kWarps == warp;
+  const int early = min(kStages - kStep, append_pending ? nt - 1 : nt);
+  for (int k = 0; k < early; ++k) {
+    issue(k);
+    if (k % kStep == kStep - 1) copy_commit();
+  }
   if (a.inputs_stable) pdl_wait();
   pdl_trigger();
-
-  // the warp whose walk holds the new row's block appends the row itself
-  const bool append_pending = appends && new_tile % kWarps == warp;
   AppendRow app;
   if (append_pending) app.load(a, b, g, seq_len - 1, table, lane);
 
@@ -309,9 +340,10 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Args a) {
   }
 
   // heads 2 t and 2 t + 1 of this lane's accumulator columns
-  float m_ref[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
-  int v_exp = -3;             // every V scale seen is below 2^v_exp (or at the clamp)
+  float m_ref[2] = {kNone, kNone}, l_run[2] = {0.0f, 0.0f};
+  int v_exp = -3;                // every V scale seen is at most 2^v_exp (or infinite)
   uint32_t v_lim = 0x30003000u;  // 2^v_exp as an f16 pair
+  float slack = 15.0f;           // 12 - v_exp: a score 2^8 over its maximum
   float acc[8][4], off[4][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
@@ -319,85 +351,104 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Args a) {
   for (int i = 0; i < 4; ++i) off[i][0] = off[i][1] = off[i][2] = off[i][3] = 0.0f;
 
   if (append_pending) app.store(a, g, lane);
-  for (int s0 = issued; s0 < kStages - 1; ++s0)
-    if (s0 < nt) issue(s0);
+  for (int k = max(early, 0); k < kStages - kStep; ++k) {
+    issue(k);
+    if (k % kStep == kStep - 1) copy_commit();
+  }
 
   const float to_log2 = CAP ? a.scale * kTwo24 / a.softcap : a.scale * kLog2e * kTwo24;
   const float cap_log2 = CAP ? a.softcap * kLog2e : 0.0f;
-  for (int k = 0; k < nt; ++k) {
+  for (int k = 0; k < nt; k += kStep) {
+    __syncwarp();  // the slots refilled here were read in the last step
+#pragma unroll
+    for (int u = 0; u < kStep; ++u) issue(k + kStages - kStep + u);
+    copy_commit();
+    copy_wait<kStages / kStep - 1>();
     __syncwarp();
-    if (k + kStages - 1 < nt) issue(k + kStages - 1);
-    // block k has landed (bounded: a timeout ends this warp's walk)
-    if (!__all_sync(0xffffffffu,
-                    mbar_wait_bounded(smem_addr(&ring_bar[warp][k % kStages]), (k / kStages) & 1))) {
-      if (lane == 0) report(a.status, DOE_DEVICE_ERR_TIMEOUT);
-      // the ring is reused below: wait (bounded) for the copies in flight
-      for (int i = k + 1; i < nt && i < k + kStages; ++i)
-        mbar_wait_bounded(smem_addr(&ring_bar[warp][i % kStages]), (i / kStages) & 1);
-      break;
-    }
-    if ((unsigned)sm_pg[warp][k] >= (unsigned)a.num_pages) {
-      if (lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
-      continue;
-    }
-    const int pos0 = (first + kWarps * k) << 4;
-    const uint32_t kb = wbase + (k % kStages) * kSlot, vb = kb + kI4Block;
-    uint4 kw[2], vw[2], vs[2];
-    uint2 ks[2];
+    float x[kStep][4];
+    uint4 vw[kStep][2], vs[kStep][2];
+    uint32_t vmax = 0;
+    const uint32_t slot0 = wbase + (uint32_t)(k % kStages) * kSlot;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      kw[h] = lds128(kb + 512 * h + 16 * lane);             // token r + 8 h
-      ks[h] = lds64(kb + kI4Codes + 64 * h + 8 * r);
-      vw[h] = lds128(vb + 512 * h + 16 * lane);             // tokens 2 t, 2 t + 1 (+ 8 h)
-      vs[h] = lds128(vb + kI4Codes + 64 * h + 16 * t);
-    }
-
-    // ---- S = K Q^T: rows token r / r + 8, columns heads 2 t, 2 t + 1 -----------
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const uint32_t w0 = word(kw[0], n), w1 = word(kw[1], n);
-      const uint32_t y0 = w0 >> 8, y1 = w1 >> 8;
-      float c[4] = {qinit[n][0], qinit[n][1], qinit[n][0], qinit[n][1]};
-      mma_16816(c, w0 & kLo, w1 & kLo, y0 & kLo, y1 & kLo, qb[n][0], qb[n][2]);
-      mma_16816(c, w0 & kHi, w1 & kHi, y0 & kHi, y1 & kHi, qb[n][1], qb[n][3]);
-      const float2 sa = f2(n < 2 ? ks[0].x : ks[0].y), sb = f2(n < 2 ? ks[1].x : ks[1].y);
-      const float s0 = (n & 1) ? sa.y : sa.x, s1 = (n & 1) ? sb.y : sb.x;
-      s[0] = fmaf(s0, c[0], s[0]);
-      s[1] = fmaf(s0, c[1], s[1]);
-      s[2] = fmaf(s1, c[2], s[2]);
-      s[3] = fmaf(s1, c[3], s[3]);
-    }
-    float x[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = CAP ? cap_log2 * tanhf(s[i] * to_log2) : s[i] * to_log2;
-    // only the window's first block and the sequence's last hold dead keys; what
-    // stands there (codes, scales) may be anything
-    if (pos0 < min_key || pos0 + 16 > seq_len) {
-      const bool live0 = pos0 + r >= min_key && pos0 + r < seq_len;
-      const bool live1 = pos0 + r + 8 >= min_key && pos0 + r + 8 < seq_len;
-      if (!live0) x[0] = x[1] = -INFINITY;
-      if (!live1) x[2] = x[3] = -INFINITY;
+    for (int u = 0; u < kStep; ++u) {
+      const uint32_t kb = slot0 + u * kSlot, vb = kb + kI4Block;
+      uint4 kw[2];
+      uint2 ks[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int key = pos0 + 2 * t + 8 * h;
-        const uint32_t keep = (key >= min_key && key < seq_len ? 0x0000ffffu : 0u) |
-                              (key + 1 >= min_key && key + 1 < seq_len ? 0xffff0000u : 0u);
-        vs[h].x &= keep; vs[h].y &= keep; vs[h].z &= keep; vs[h].w &= keep;
+        kw[h] = lds128(kb + 512 * h + 16 * lane);     // token r + 8 h
+        ks[h] = lds64(kb + kI4Codes + 64 * h + 8 * r);
+        vw[u][h] = lds128(vb + 512 * h + 16 * lane);  // tokens 2 t, 2 t + 1 (+ 8 h)
+        vs[u][h] = lds128(vb + kI4Codes + 64 * h + 16 * t);
+      }
+      // ---- S = K Q^T: rows token r / r + 8, columns heads 2 t, 2 t + 1 ---------
+      float s[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint32_t w0 = word(kw[0], n), w1 = word(kw[1], n);
+        const uint32_t y0 = w0 >> 8, y1 = w1 >> 8;
+        float c[4];
+        mma_from(c, w0 & kLo, w1 & kLo, y0 & kLo, y1 & kLo, qb[n][0], qb[n][2], qinit[n][0], qinit[n][1], qinit[n][0],
+                 qinit[n][1]);
+        mma_16816(c, w0 & kHi, w1 & kHi, y0 & kHi, y1 & kHi, qb[n][1], qb[n][3]);
+        const float2 sa = f2(n < 2 ? ks[0].x : ks[0].y), sb = f2(n < 2 ? ks[1].x : ks[1].y);
+        const float s0 = (n & 1) ? sa.y : sa.x, s1 = (n & 1) ? sb.y : sb.x;
+        s[0] = n ? fmaf(s0, c[0], s[0]) : s0 * c[0];
+        s[1] = n ? fmaf(s0, c[1], s[1]) : s0 * c[1];
+        s[2] = n ? fmaf(s1, c[2], s[2]) : s1 * c[2];
+        s[3] = n ? fmaf(s1, c[3], s[3]) : s1 * c[3];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[u][i] = CAP ? cap_log2 * tanhf(s[i] * to_log2) : s[i] * to_log2;
+    }
+    // dead keys: in the window's first block, the sequence's last, blocks past the
+    // walk and blocks of bad pages; what stands there (codes, scales) may be anything
+    const int pos_k = (first + kWarps * k) << 4;
+    bool edge = pos_k < min_key || pos_k + 16 * (kWarps * (kStep - 1) + 1) > seq_len || k + kStep > nt;
+    int page[kStep];
+#pragma unroll
+    for (int u = 0; u < kStep; ++u) {
+      page[u] = sm_pg[warp][min(k + u, nt - 1)];
+      edge |= (unsigned)page[u] >= (unsigned)a.num_pages;
+    }
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) {
+        const int pos0 = pos_k + 16 * kWarps * u;
+        const bool bad = (unsigned)page[u] >= (unsigned)a.num_pages;
+        if (bad && k + u < nt && lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
+        const int lo = min_key, hi = bad || k + u >= nt ? 0 : seq_len;
+        if (pos0 + r < lo || pos0 + r >= hi) x[u][0] = x[u][1] = -INFINITY;
+        if (pos0 + r + 8 < lo || pos0 + r + 8 >= hi) x[u][2] = x[u][3] = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = pos0 + 2 * t + 8 * h;
+          const uint32_t keep = (key >= lo && key < hi ? 0x0000ffffu : 0u) |
+                                (key + 1 >= lo && key + 1 < hi ? 0xffff0000u : 0u);
+          vs[u][h].x &= keep; vs[u][h].y &= keep; vs[u][h].z &= keep; vs[u][h].w &= keep;
+        }
       }
     }
 
     // ---- the reference moves when a score or a V scale outgrows it -------------
-    const uint32_t vmax = hmax2(hmax2(hmax2(vs[0].x, vs[0].y), hmax2(vs[0].z, vs[0].w)),
-                                hmax2(hmax2(vs[1].x, vs[1].y), hmax2(vs[1].z, vs[1].w)));
-    const bool grow = fmaxf(x[0], x[2]) > m_ref[0] + 8.0f || fmaxf(x[1], x[3]) > m_ref[1] + 8.0f ||
+    float mx[2] = {fmaxf(x[0][0], x[0][2]), fmaxf(x[0][1], x[0][3])};
+#pragma unroll
+    for (int u = 0; u < kStep; ++u) {
+      if (u) {
+        mx[0] = fmaxf(mx[0], fmaxf(x[u][0], x[u][2]));
+        mx[1] = fmaxf(mx[1], fmaxf(x[u][1], x[u][3]));
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        vmax = hmax2(vmax, hmax2(hmax2(vs[u][h].x, vs[u][h].y), hmax2(vs[u][h].z, vs[u][h].w)));
+    }
+    const bool grow = mx[0] > m_ref[0] + slack || mx[1] > m_ref[1] + slack ||
                       !__hble2(*reinterpret_cast<const __half2*>(&vmax), *reinterpret_cast<const __half2*>(&v_lim));
     if (__any_sync(0xffffffffu, grow)) {
       const float2 vf = f2(vmax);
       const float vm = warp_max(fmaxf(vf.x, vf.y));
       int e = v_exp;
       if (vm > 0.0f) e = max(e, min(15, (int)((__float_as_uint(vm) >> 23) & 255) - 126));
-      float mx[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -405,8 +456,8 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Args a) {
         // reference = score maximum + exponent of the V scales - 4: p <= 2^15
         // and s p <= 2^12 while a score may still outgrow the maximum by 2^8
         const float base = m_ref[j] - (float)(v_exp - 4);
-        const float m_new = (mx[j] > base + 8.0f || base == -INFINITY ? mx[j] : base) + (float)(e - 4);
-        const float corr = m_ref[j] == -INFINITY ? 0.0f : ex2(m_ref[j] - m_new);
+        const float m_new = fmaxf(base, mx[j]) + (float)(e - 4);
+        const float corr = ex2(m_ref[j] - m_new);
         m_ref[j] = m_new;
         l_run[j] *= corr;
 #pragma unroll
@@ -418,32 +469,38 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Args a) {
         for (int i = 0; i < 4; ++i) off[i][j] *= corr;
       }
       v_exp = e;
-      v_lim = e >= 16 ? 0x7bff7bffu : (uint32_t)(e + 15) * 0x04000400u;
+      v_lim = (uint32_t)(e + 15) * 0x04000400u;
+      slack = (float)(12 - e);
     }
 
-    float p[4];
-    p[0] = ex2(x[0] - m_ref[0]);
-    p[1] = ex2(x[1] - m_ref[1]);
-    p[2] = ex2(x[2] - m_ref[0]);
-    p[3] = ex2(x[3] - m_ref[1]);
-    l_run[0] += p[0] + p[2];
-    l_run[1] += p[1] + p[3];
-    const uint32_t p0 = transpose8x8(pack_half2(p[0], p[1]));  // head r, tokens 2 t, 2 t + 1
-    const uint32_t p1 = transpose8x8(pack_half2(p[2], p[3]));  // tokens + 8
-
-    // ---- O^T += V^T (s P)^T: m-block 2 n + j = dims 32 n + 4 row' + {2 j, 2 j + 1}
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const uint32_t b0 = hmul2(p0, word(vs[0], n)), b1 = hmul2(p1, word(vs[1], n));
-      const uint32_t w0 = word(vw[0], n), w1 = word(vw[1], n);
-      const uint32_t y0 = w0 >> 8, y1 = w1 >> 8;
-      mma_16816(acc[2 * n], w0 & kLo, w0 & kHi, w1 & kLo, w1 & kHi, b0, b1);
-      mma_16816(acc[2 * n + 1], y0 & kLo, y0 & kHi, y1 & kLo, y1 & kHi, b0, b1);
-      mma_16816(off[n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0, b1);
+    for (int u = 0; u < kStep; ++u) {
+      float p[4];
+      p[0] = ex2(x[u][0] - m_ref[0]);
+      p[1] = ex2(x[u][1] - m_ref[1]);
+      p[2] = ex2(x[u][2] - m_ref[0]);
+      p[3] = ex2(x[u][3] - m_ref[1]);
+      l_run[0] += p[0] + p[2];
+      l_run[1] += p[1] + p[3];
+      const uint32_t p0 = transpose8x8(pack_half2(p[0], p[1]));  // head r, tokens 2 t, 2 t + 1
+      const uint32_t p1 = transpose8x8(pack_half2(p[2], p[3]));  // tokens + 8
+
+      // ---- O^T += V^T (s P)^T: m-block 2 n + j = dims 32 n + 4 row' + {2 j, 2 j + 1}
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint32_t b0 = hmul2(p0, word(vs[u][0], n)), b1 = hmul2(p1, word(vs[u][1], n));
+        const uint32_t w0 = word(vw[u][0], n), w1 = word(vw[u][1], n);
+        const uint32_t y0 = w0 >> 8, y1 = w1 >> 8;
+        mma_16816(acc[2 * n], w0 & kLo, w0 & kHi, w1 & kLo, w1 & kHi, b0, b1);
+        mma_16816(acc[2 * n + 1], y0 & kLo, y0 & kHi, y1 & kLo, y1 & kHi, b0, b1);
+        mma_16816(off[n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0, b1);
+      }
     }
   }
 
-  // ---- merge the warps of this split (O staged in this warp's own ring) --------
+  // ---- join the warps of this split (O staged in this warp's own ring) ---------
+  copy_wait<0>();
+  __syncwarp();
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -454,7 +511,6 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Args a) {
     }
   }
   float* my_o = reinterpret_cast<float*>(ring + warp * kWarpBytes);  // [8][128]
-  __syncwarp();
 #pragma unroll
   for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -468,65 +524,130 @@ __global__ void __launch_bounds__(kWarps * 32) decode_kernel(const Args a) {
 
   const int dim = threadIdx.x;  // 128 threads == head dim
   const size_t out_row = ((size_t)b * a.num_heads + (size_t)g * group) * kD;
-  auto store = [&](int h, float v) {
+  auto store = [&](int h, int d, float o, float l) {
+    const float v = l != 0.0f ? o / l : 0.0f;
     if (a.out_bf16)
-      reinterpret_cast<__nv_bfloat16*>(a.out)[out_row + (size_t)h * kD + dim] = __float2bfloat16_rn(v);
+      reinterpret_cast<__nv_bfloat16*>(a.out)[out_row + (size_t)h * kD + d] = __float2bfloat16_rn(v);
     else
-      a.out[out_row + (size_t)h * kD + dim] = v;
+      a.out[out_row + (size_t)h * kD + d] = v;
   };
-  const size_t base = ((size_t)b * Hkv + g) * a.max_splits;
+  const size_t row = (size_t)b * Hkv + g, base = row * a.max_parts;
+  float* cta_o = reinterpret_cast<float*>(ring);  // [8][128], over the first warp's
   for (int h = 0; h < group; ++h) {
-    float M = -INFINITY, O = 0.0f, L = 0.0f;
+    float M = kNone, O = 0.0f, L = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][h]);
-    if (M != -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2f(sm_m[w][h] - M);  // -inf -> 0
-        O += f * reinterpret_cast<const float*>(ring + w * kWarpBytes)[h * kD + dim];
-        L += f * sm_l[w][h];
-      }
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2(sm_m[w][h] - M);
+      O += f * reinterpret_cast<const float*>(ring + w * kWarpBytes)[h * kD + dim];
+      L += f * sm_l[w][h];
     }
     if (nsplits == 1) {
-      store(h, L != 0.0f ? O / L : 0.0f);
-    } else {
-      const size_t prow = (base + split) * group + h;
-      a.part_o[prow * kD + dim] = O;
+      if (split == 0) store(h, dim, O, L);
+    } else if (slices == 1) {
+      a.part_o[((base + part) * group + h) * kD + dim] = O;
       if (dim == 0) {
-        a.part_ml[prow * 2] = M;
-        a.part_ml[prow * 2 + 1] = L;
+        a.part_ml[((base + part) * group + h) * 2] = M;
+        a.part_ml[((base + part) * group + h) * 2 + 1] = L;
+      }
+    } else {
+      cta_o[h * kD + dim] = O;  // read only by this thread before
+      if (dim == 0) {
+        cta_ml[h][0] = M;
+        cta_ml[h][1] = L;
       }
     }
   }
   if (nsplits == 1) return;
-  // ---- the last split of (b, g) to finish stitches them, in split order --------
+
+  // ---- the splits of a cluster: this CTA joins its slice of the dims ------------
+  int rank = 0;
+  const int width = kD / slices;
+  if (slices > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    rank = (int)cluster.block_rank();
+    cluster.sync();
+    for (int i = threadIdx.x; i < group * width; i += kWarps * 32) {
+      const int h = i / width, d = rank * width + i % width;
+      float M = kNone, O = 0.0f, L = 0.0f;
+      float m[8], o[8], l[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < slices) {
+          const float* ml = cluster.map_shared_rank(&cta_ml[h][0], c);
+          m[c] = ml[0];
+          l[c] = ml[1];
+          o[c] = cluster.map_shared_rank(cta_o, c)[h * kD + d];
+          M = fmaxf(M, m[c]);
+        }
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < slices) {
+          const float f = ex2(m[c] - M);
+          O += f * o[c];
+          L += f * l[c];
+        }
+      if (nparts == 1) {
+        store(h, d, O, L);
+      } else {
+        a.part_o[((base + part) * group + h) * kD + d] = O;
+        if (i % width == 0) {
+          float* ml = a.part_ml + (((base + part) * slices + rank) * group + h) * 2;
+          ml[0] = M;
+          ml[1] = L;
+        }
+      }
+    }
+    cluster.sync();  // the others have read this CTA's partials
+  }
+  if (nparts == 1) return;
+  // ---- the last part of (b, g, slice) to finish stitches them, in order --------
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) {
-    const unsigned old = atomicAdd(&a.counters[(size_t)b * Hkv + g], 1u);
-    sm_last = old == (unsigned)(nsplits - 1);
-    if (sm_last) a.counters[(size_t)b * Hkv + g] = 0u;  // ready for the next launch
+    unsigned* counter = &a.counters[row * slices + rank];
+    sm_last = atomicAdd(counter, 1u) == (unsigned)(nparts - 1);
+    if (sm_last) *counter = 0u;  // ready for the next launch
   }
   __syncthreads();
   if (!sm_last) return;
   __threadfence();
-  for (int h = 0; h < group; ++h) {
-    float M = -INFINITY, O = 0.0f, L = 0.0f;
-    for (int sp = 0; sp < nsplits; ++sp) M = fmaxf(M, __ldcg(a.part_ml + ((base + sp) * group + h) * 2));
-    if (M != -INFINITY) {
-      for (int sp = 0; sp < nsplits; ++sp) {
-        const size_t prow = (base + sp) * group + h;
-        const float f = exp2f(__ldcg(a.part_ml + prow * 2) - M);
-        O += f * __ldcg(a.part_o + prow * kD + dim);
-        L += f * __ldcg(a.part_ml + prow * 2 + 1);
+  for (int i = threadIdx.x; i < group * width; i += kWarps * 32) {
+    const int h = i / width, d = rank * width + i % width;
+    float M = kNone, O = 0.0f, L = 0.0f;
+    // a running reference, so that the loads of several parts are in flight
+    constexpr int kBatch = 8;
+    for (int p0 = 0; p0 < nparts; p0 += kBatch) {
+      float2 ml[kBatch];
+      float o[kBatch];
+#pragma unroll
+      for (int c = 0; c < kBatch; ++c) {
+        const size_t at = base + min(p0 + c, nparts - 1);
+        ml[c] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + (at * slices + rank) * group + h);
+        o[c] = __ldcg(a.part_o + (at * group + h) * kD + d);
       }
+      float m = M;
+#pragma unroll
+      for (int c = 0; c < kBatch; ++c) m = fmaxf(m, ml[c].x);
+      const float f0 = ex2(M - m);
+      O *= f0;
+      L *= f0;
+      M = m;
+#pragma unroll
+      for (int c = 0; c < kBatch; ++c)
+        if (p0 + c < nparts) {
+          const float f = ex2(ml[c].x - M);
+          O += f * o[c];
+          L += f * ml[c].y;
+        }
     }
-    store(h, L != 0.0f ? O / L : 0.0f);
+    store(h, d, O, L);
   }
 }
 
 template <bool CAP>
-int launch_cap(const Args& a, dim3 grid, cudaStream_t st) {
+int launch_cap(const Args& a, dim3 grid, unsigned slices, cudaStream_t st) {
   static std::atomic<bool> attr[kMaxDevices];
   const int rc = once_per_device(attr, [] {
     return cuda_status(
@@ -534,20 +655,50 @@ int launch_cap(const Args& a, dim3 grid, cudaStream_t st) {
         "cudaFuncSetAttribute(paged_decode_int4)");
   });
   if (rc != DOE_OK) return rc;
-  return cuda_status(launch_pdl(decode_kernel<CAP>, grid, dim3(kWarps * 32), kSmem, st, a), "paged_decode_int4");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = slices;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cuda_status(cudaLaunchKernelEx(&cfg, decode_kernel<CAP>, a), "paged_decode_int4");
 }
 
-// Blocks per split.  Long splits amortise a CTA's pipeline fill and stitch;
-// where the (sequence, kv head) rows are few the length is cut until there are
-// about two CTAs per SM.
-uint32_t auto_split_tiles(uint64_t rows, uint64_t max_tiles) {
-  const uint64_t want = (max_tiles * rows + 1775) / 1776;
-  if (want >= 128) return 128;
-  uint64_t s = (max_tiles + 127) / 128;
-  const uint64_t fill = (280 + rows - 1) / rows;
-  if (s < fill) s = fill;
-  const uint64_t t = (max_tiles + s - 1) / s;
-  return (uint32_t)(t < 4 ? 4 : t);
+// How a launch is cut: blocks per split, splits per cluster, and the sizes
+// that follow.
+struct Plan {
+  uint64_t split_tiles, slices, max_parts, grid_x;
+};
+
+// Long splits amortise a CTA's prologue and join; where the (sequence, kv head)
+// rows are few the length is cut until there are about two CTAs per SM.
+Plan plan(uint64_t rows, uint64_t max_tiles, uint64_t tiles_per_page, uint64_t split_pages) {
+  uint64_t t = split_pages * tiles_per_page;
+  if (t == 0) {
+    const uint64_t want = (max_tiles * rows + 1775) / 1776;
+    if (want >= 128) {
+      t = 128;
+    } else {
+      uint64_t s = (max_tiles + 127) / 128;
+      const uint64_t fill = (280 + rows - 1) / rows;
+      if (s < fill) s = fill;
+      t = (max_tiles + s - 1) / s;
+      if (t < 4) t = 4;
+    }
+  }
+  if (t > kMaxSplitTiles) t = kMaxSplitTiles;  // prefetched page ids
+  const uint64_t splits = (max_tiles + t - 1) / t;
+  const uint64_t slices = splits > 16 ? 8 : 1;
+  const uint64_t parts = (splits + slices - 1) / slices;
+  return {t, slices, parts, parts * slices};
 }
 
 }  // namespace i4
@@ -561,12 +712,10 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   const uint32_t tpp = kv->page_size / 16;
   const uint64_t max_tiles = (uint64_t)kv->max_pages_per_seq * tpp;
   const uint64_t rows = (uint64_t)num_seqs * Hkv;
-  uint64_t split_tiles = split_pages ? (uint64_t)split_pages * tpp : auto_split_tiles(rows ? rows : 1, max_tiles);
-  if (split_tiles > kMaxSplitTiles) split_tiles = kMaxSplitTiles;  // prefetched page ids
-  const uint64_t max_splits = (max_tiles + split_tiles - 1) / split_tiles;
-  const uint64_t parts = rows * max_splits * group;
-  const uint64_t ctr_off = (parts * (kD + 2) * sizeof(float) + 255) / 256 * 256;
-  const uint64_t ws = ctr_off + rows * sizeof(unsigned);
+  const Plan pl = plan(rows ? rows : 1, max_tiles, tpp, split_pages);
+  const uint64_t parts = rows * pl.max_parts * group;
+  const uint64_t ctr_off = (parts * (kD + 2 * pl.slices) * sizeof(float) + 255) / 256 * 256;
+  const uint64_t ws = ctr_off + rows * pl.slices * sizeof(unsigned);
   if (ws_needed_out) {
     *ws_needed_out = ws;
     return DOE_OK;
@@ -580,7 +729,7 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
                  (unsigned long long)launch->workspace_bytes);
     return DOE_INVALID_ARGUMENT;
   }
-  if (max_tiles * 16 > 0x7fffffffull || max_splits > 0x7fffffffull || Hkv > 65535u) {
+  if (max_tiles * 16 > 0x7fffffffull || pl.grid_x > 0x7fffffffull || Hkv > 65535u) {
     set_op_error("doe_paged_decode: a block-table row spans more than 2^31 - 1 tokens, or over 65535 kv heads");
     return DOE_INVALID_ARGUMENT;
   }
@@ -622,18 +771,19 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   a.tile_shift = -1;
   for (int s = 0; s < 27; ++s)
     if (tpp == (1u << s)) a.tile_shift = s;
-  a.split_tiles = (int)split_tiles;
-  a.max_splits = (int)max_splits;
+  a.split_tiles = (int)pl.split_tiles;
+  a.max_parts = (int)pl.max_parts;
   a.out_bf16 = (opts && (opts->flags & DOE_DECODE_OUT_BF16)) ? 1 : 0;
   a.inputs_stable = (opts && (opts->flags & DOE_DECODE_INPUTS_STABLE)) ? 1 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(launch->stream);
-  if (max_splits > 1 && !(opts && (opts->flags & DOE_DECODE_COUNTERS_ZEROED))) {
+  if (pl.max_parts > 1 && !(opts && (opts->flags & DOE_DECODE_COUNTERS_ZEROED))) {
     const int rc =
-        cuda_status(cudaMemsetAsync(a.counters, 0, rows * sizeof(unsigned), st), "cudaMemsetAsync(split counters)");
+        cuda_status(cudaMemsetAsync(a.counters, 0, rows * pl.slices * sizeof(unsigned), st), "cudaMemsetAsync(split counters)");
     if (rc != DOE_OK) return rc;
   }
-  const dim3 grid((unsigned)max_splits, Hkv, num_seqs);
-  return a.softcap > 0.0f ? launch_cap<true>(a, grid, st) : launch_cap<false>(a, grid, st);
+  const dim3 grid((unsigned)pl.grid_x, Hkv, num_seqs);
+  return a.softcap > 0.0f ? launch_cap<true>(a, grid, (unsigned)pl.slices, st)
+                          : launch_cap<false>(a, grid, (unsigned)pl.slices, st);
 }
 
 }  // namespace doe

@@ -206,7 +206,7 @@ struct AppendRow {
 };
 
 constexpr float kNone = -1e30f;  // the reference of a head without keys: below any score
-constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
+constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u, kBoth = 0x00ff00ffu;
 constexpr float kTwo24 = 16777216.0f;
 
 template <bool CAP>
@@ -238,41 +238,44 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
   __shared__ float sm_l[kWarps][8];
   __shared__ float cta_ml[8][2];
   __shared__ int sm_last;
-  __shared__ int sm_pg[kWarps][32 * kPageRegs];
+  __shared__ __align__(8) int sm_blk[kWarps][32 * kPageRegs + kStages];
 
-  // this warp's blocks: first + kWarps * k, k < nt; page ids up front
+  // this warp's blocks: first + kWarps * k, k < nt, as block numbers in the pools
+  // up front; -1 past the walk and on pages outside the pool
   const int first = tile_origin + tile_begin + warp;
   const int span = tile_end - tile_begin - warp;
   const int nt = span > 0 ? (span + kWarps - 1) / kWarps : 0;
-  auto page_index = [&](int tile) { return a.tile_shift >= 0 ? tile >> a.tile_shift : tile / a.tiles_per_page; };
-#pragma unroll
-  for (int i = 0; i < kPageRegs; ++i)
-    if (lane + 32 * i < nt) sm_pg[warp][lane + 32 * i] = table[page_index(first + kWarps * (lane + 32 * i))];
+  for (int i = lane; i < nt + kStages; i += 32) {
+    int blk = -1;
+    if (i < nt) {
+      const int tile = first + kWarps * i;
+      const int pidx = a.tile_shift >= 0 ? tile >> a.tile_shift : tile / a.tiles_per_page;
+      const int page = table[pidx];
+      if ((unsigned)page < (unsigned)a.num_pages)
+        blk = (page * Hkv + g) * a.tiles_per_page + (tile - pidx * a.tiles_per_page);
+      else
+        report(a.status, DOE_DEVICE_ERR_PAGE);
+    }
+    sm_blk[warp][i] = blk;
+  }
   __syncwarp();
 
   const uint32_t wbase = smem_addr(ring) + warp * kWarpBytes;
-  const size_t head_bytes = (size_t)a.tiles_per_page * kI4Block;
-  const uint8_t* k_head = a.k_pool + g * head_bytes + 16 * lane;
-  const uint8_t* v_head = a.v_pool + g * head_bytes + 16 * lane;
+  const uint8_t* k_lane = a.k_pool + 16 * lane;
+  const uint8_t* v_lane = a.v_pool + 16 * lane;
   // lanes 0-7 copy the K scales, 8-15 the V scales
-  const ptrdiff_t s_off = (lane < 8 ? k_head : v_head - 128) + kI4Codes - k_head;
-  const uint32_t s_dst = kI4Codes + 16 * lane + (lane < 8 ? 0 : kI4Block - 128);
-  const size_t page_bytes = (size_t)Hkv * head_bytes;
-  // Fills slot k % kStages with block k (nothing past the walk, or for a bad page)
-  auto issue = [&](int k) {
-    if (k < nt) {
-      const int page = sm_pg[warp][k];
-      if ((unsigned)page < (unsigned)a.num_pages) {
-        const int tile = first + kWarps * k;
-        const size_t off =
-            (size_t)page * page_bytes + (size_t)((tile - page_index(tile) * a.tiles_per_page) * kI4Block);
-        const uint32_t dst = wbase + (uint32_t)(k % kStages) * kSlot;
-        copy16(dst + 16 * lane, k_head + off);
-        copy16(dst + 16 * lane + 512, k_head + off + 512);
-        copy16(dst + 16 * lane + kI4Block, v_head + off);
-        copy16(dst + 16 * lane + kI4Block + 512, v_head + off + 512);
-        if (lane < 16) copy16(dst + s_dst, k_head + off + s_off);
-      }
+  const uint8_t* s_lane = (lane < 8 ? k_lane : v_lane - 128) + kI4Codes;
+  const uint32_t lane_dst = wbase + 16 * lane;
+  const uint32_t s_dst = lane_dst + kI4Codes + (lane < 8 ? 0 : kI4Block - 128);
+  // Fills the slot at byte `slot` of the ring with block number blk
+  auto issue = [&](int blk, uint32_t slot) {
+    if (blk >= 0) {
+      const size_t at = (size_t)(uint32_t)blk * kI4Block;
+      copy16(lane_dst + slot, k_lane + at);
+      copy16(lane_dst + slot + 512, k_lane + at + 512);
+      copy16(lane_dst + slot + kI4Block, v_lane + at);
+      copy16(lane_dst + slot + kI4Block + 512, v_lane + at + 512);
+      if (lane < 16) copy16(s_dst + slot, s_lane + at);
     }
   };
 
@@ -285,7 +288,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
   const bool append_pending = appends && new_tile % kWarps == warp;
   const int early = min(kStages - kStep, append_pending ? nt - 1 : nt);
   for (int k = 0; k < early; ++k) {
-    issue(k);
+    issue(sm_blk[warp][k], k * kSlot);
     if (k % kStep == kStep - 1) copy_commit();
   }
   if (a.inputs_stable) pdl_wait();
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
       float qs = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t w = word(qv[n], i);
+        uint32_t w = word(qv[n], i) ^ (!CAP && a.scale < 0.0f ? 0x80008000u : 0u);
         float mult = 1.0f;
         if (i & 1) {  // meets codes read as n 2^-20; q 2^-4 loses bits only below |q| = 2^-10, 2^-21 absolute
           w = hmul2(w, 0x2c002c00u);
@@ -343,7 +346,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
   float m_ref[2] = {kNone, kNone}, l_run[2] = {0.0f, 0.0f};
   int v_exp = -3;                // every V scale seen is at most 2^v_exp (or infinite)
   uint32_t v_lim = 0x30003000u;  // 2^v_exp as an f16 pair
-  float slack = 15.0f;           // 12 - v_exp: a score 2^8 over its maximum
+  float m_lim[2] = {kNone, kNone};  // x of a score 2^8 over its maximum
   float acc[8][4], off[4][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
@@ -351,27 +354,34 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
   for (int i = 0; i < 4; ++i) off[i][0] = off[i][1] = off[i][2] = off[i][3] = 0.0f;
 
   if (append_pending) app.store(a, g, lane);
-  for (int k = max(early, 0); k < kStages - kStep; ++k) {
-    issue(k);
+  for (int k = early; k < kStages - kStep; ++k) {
+    issue(sm_blk[warp][k], k * kSlot);
     if (k % kStep == kStep - 1) copy_commit();
   }
 
-  const float to_log2 = CAP ? a.scale * kTwo24 / a.softcap : a.scale * kLog2e * kTwo24;
-  const float cap_log2 = CAP ? a.softcap * kLog2e : 0.0f;
+  // x is the softcapped score in the log2 domain (CAP) or the bare product, which
+  // c > 0 takes there: the sign of the scale is in Q, and a scale of 0 becomes
+  // tiny so that the -inf of a dead key stays -inf
+  const float to_cap = a.scale * kTwo24 / a.softcap, cap_log2 = a.softcap * kLog2e;  // CAP only
+  const float c_log2 = CAP ? 1.0f : fmaxf(fabsf(a.scale) * (kLog2e * kTwo24), 1e-30f), inv_c = 1.0f / c_log2;
+  const bool window_edge = first * 16 < min_key;
+  uint32_t slot = 0, refill = (kStages - kStep) * kSlot;  // byte offsets in the ring
   for (int k = 0; k < nt; k += kStep) {
+    const int2 next = *reinterpret_cast<const int2*>(&sm_blk[warp][k + kStages - kStep]);
+    const int2 blk = *reinterpret_cast<const int2*>(&sm_blk[warp][k]);
+    static_assert(kStep == 2, "block numbers are read in pairs");
     __syncwarp();  // the slots refilled here were read in the last step
-#pragma unroll
-    for (int u = 0; u < kStep; ++u) issue(k + kStages - kStep + u);
+    issue(next.x, refill);
+    issue(next.y, refill + kSlot);
     copy_commit();
     copy_wait<kStages / kStep - 1>();
     __syncwarp();
     float x[kStep][4];
     uint4 vw[kStep][2], vs[kStep][2];
-    uint32_t vmax = 0;
-    const uint32_t slot0 = wbase + (uint32_t)(k % kStages) * kSlot;
+    uint32_t vmax = v_lim;  // scales are not negative, so they order as 16-bit integers
 #pragma unroll
     for (int u = 0; u < kStep; ++u) {
-      const uint32_t kb = slot0 + u * kSlot, vb = kb + kI4Block;
+      const uint32_t kb = wbase + slot + u * kSlot, vb = kb + kI4Block;
       uint4 kw[2];
       uint2 ks[2];
 #pragma unroll
@@ -399,25 +409,17 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
         s[3] = n ? fmaf(s1, c[3], s[3]) : s1 * c[3];
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[u][i] = CAP ? cap_log2 * tanhf(s[i] * to_log2) : s[i] * to_log2;
+      for (int i = 0; i < 4; ++i) x[u][i] = CAP ? cap_log2 * tanhf(s[i] * to_cap) : s[i];
     }
+    refill = slot;
+    slot = slot == (kStages - kStep) * kSlot ? 0 : slot + kStep * kSlot;
     // dead keys: in the window's first block, the sequence's last, blocks past the
     // walk and blocks of bad pages; what stands there (codes, scales) may be anything
-    const int pos_k = (first + kWarps * k) << 4;
-    bool edge = pos_k < min_key || pos_k + 16 * (kWarps * (kStep - 1) + 1) > seq_len || k + kStep > nt;
-    int page[kStep];
-#pragma unroll
-    for (int u = 0; u < kStep; ++u) {
-      page[u] = sm_pg[warp][min(k + u, nt - 1)];
-      edge |= (unsigned)page[u] >= (unsigned)a.num_pages;
-    }
-    if (edge) {
+    if (k + kStep >= nt || (blk.x | blk.y) < 0 || (k == 0 && window_edge)) {
 #pragma unroll
       for (int u = 0; u < kStep; ++u) {
-        const int pos0 = pos_k + 16 * kWarps * u;
-        const bool bad = (unsigned)page[u] >= (unsigned)a.num_pages;
-        if (bad && k + u < nt && lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
-        const int lo = min_key, hi = bad || k + u >= nt ? 0 : seq_len;
+        const int pos0 = (first + kWarps * (k + u)) << 4;
+        const int lo = min_key, hi = (u ? blk.y : blk.x) < 0 ? 0 : seq_len;
         if (pos0 + r < lo || pos0 + r >= hi) x[u][0] = x[u][1] = -INFINITY;
         if (pos0 + r + 8 < lo || pos0 + r + 8 >= hi) x[u][2] = x[u][3] = -INFINITY;
 #pragma unroll
@@ -440,15 +442,14 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        vmax = hmax2(vmax, hmax2(hmax2(vs[u][h].x, vs[u][h].y), hmax2(vs[u][h].z, vs[u][h].w)));
+        vmax = __vimax3_u16x2(__vimax3_u16x2(vmax, vs[u][h].x, vs[u][h].y), vs[u][h].z, vs[u][h].w);
     }
-    const bool grow = mx[0] > m_ref[0] + slack || mx[1] > m_ref[1] + slack ||
-                      !__hble2(*reinterpret_cast<const __half2*>(&vmax), *reinterpret_cast<const __half2*>(&v_lim));
+    const bool grow = mx[0] > m_lim[0] || mx[1] > m_lim[1] || vmax != v_lim;
     if (__any_sync(0xffffffffu, grow)) {
-      const float2 vf = f2(vmax);
+      const float2 vf = f2(vmax);  // at least 2^v_exp
       const float vm = warp_max(fmaxf(vf.x, vf.y));
       int e = v_exp;
-      if (vm > 0.0f) e = max(e, min(15, (int)((__float_as_uint(vm) >> 23) & 255) - 126));
+      if (vm > f2(v_lim).x) e = min(15, (int)((__float_as_uint(vm) >> 23) & 255) - 126);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -456,9 +457,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
         // reference = score maximum + exponent of the V scales - 4: p <= 2^15
         // and s p <= 2^12 while a score may still outgrow the maximum by 2^8
         const float base = m_ref[j] - (float)(v_exp - 4);
-        const float m_new = fmaxf(base, mx[j]) + (float)(e - 4);
+        const float top = fmaxf(base, mx[j] * c_log2), m_new = top + (float)(e - 4);
         const float corr = ex2(m_ref[j] - m_new);
         m_ref[j] = m_new;
+        m_lim[j] = (top + 8.0f) * inv_c;
         l_run[j] *= corr;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -470,16 +472,15 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
       }
       v_exp = e;
       v_lim = (uint32_t)(e + 15) * 0x04000400u;
-      slack = (float)(12 - e);
     }
 
 #pragma unroll
     for (int u = 0; u < kStep; ++u) {
       float p[4];
-      p[0] = ex2(x[u][0] - m_ref[0]);
-      p[1] = ex2(x[u][1] - m_ref[1]);
-      p[2] = ex2(x[u][2] - m_ref[0]);
-      p[3] = ex2(x[u][3] - m_ref[1]);
+      p[0] = ex2(fmaf(x[u][0], c_log2, -m_ref[0]));
+      p[1] = ex2(fmaf(x[u][1], c_log2, -m_ref[1]));
+      p[2] = ex2(fmaf(x[u][2], c_log2, -m_ref[0]));
+      p[3] = ex2(fmaf(x[u][3], c_log2, -m_ref[1]));
       l_run[0] += p[0] + p[2];
       l_run[1] += p[1] + p[3];
       const uint32_t p0 = transpose8x8(pack_half2(p[0], p[1]));  // head r, tokens 2 t, 2 t + 1
@@ -490,9 +491,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
       for (int n = 0; n < 4; ++n) {
         const uint32_t b0 = hmul2(p0, word(vs[u][0], n)), b1 = hmul2(p1, word(vs[u][1], n));
         const uint32_t w0 = word(vw[u][0], n), w1 = word(vw[u][1], n);
-        const uint32_t y0 = w0 >> 8, y1 = w1 >> 8;
-        mma_16816(acc[2 * n], w0 & kLo, w0 & kHi, w1 & kLo, w1 & kHi, b0, b1);
-        mma_16816(acc[2 * n + 1], y0 & kLo, y0 & kHi, y1 & kLo, y1 & kHi, b0, b1);
+        const uint32_t y0 = prmt(w0, 0u, 0x4341u), y1 = prmt(w1, 0u, 0x4341u);  // bytes 1 and 3
+        mma_16816(acc[2 * n], w0 & kLo, w0 & kBoth, w1 & kLo, w1 & kBoth, b0, b1);
+        mma_16816(acc[2 * n + 1], y0 & kLo, y0, y1 & kLo, y1, b0, b1);
         mma_16816(off[n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0, b1);
       }
     }
@@ -516,8 +517,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const float o8 = off[n][j];
-      const float4 v = make_float4((acc[2 * n][j] - o8) * kTwo24, (acc[2 * n][2 + j] * 0.0625f - o8) * kTwo24,
-                                   (acc[2 * n + 1][j] - o8) * kTwo24, (acc[2 * n + 1][2 + j] * 0.0625f - o8) * kTwo24);
+      const float lo0 = acc[2 * n][j], lo1 = acc[2 * n + 1][j];
+      const float hi0 = (acc[2 * n][2 + j] - lo0) * 0.0625f, hi1 = (acc[2 * n + 1][2 + j] - lo1) * 0.0625f;
+      const float4 v = make_float4((lo0 - o8) * kTwo24, (hi0 - o8) * kTwo24, (lo1 - o8) * kTwo24, (hi1 - o8) * kTwo24);
       *reinterpret_cast<float4*>(my_o + (2 * t + j) * kD + 32 * n + 4 * r) = v;
     }
   __syncthreads();
@@ -729,8 +731,10 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
                  (unsigned long long)launch->workspace_bytes);
     return DOE_INVALID_ARGUMENT;
   }
-  if (max_tiles * 16 > 0x7fffffffull || pl.grid_x > 0x7fffffffull || Hkv > 65535u) {
-    set_op_error("doe_paged_decode: a block-table row spans more than 2^31 - 1 tokens, or over 65535 kv heads");
+  if (max_tiles * 16 > 0x7fffffffull || pl.grid_x > 0x7fffffffull || Hkv > 65535u ||
+      (uint64_t)kv->num_pages * Hkv * tpp > 0x7fffffffull) {
+    set_op_error("doe_paged_decode: more than 2^31 - 1 tokens in a block-table row or blocks in a pool, or over 65535 "
+                 "kv heads");
     return DOE_INVALID_ARGUMENT;
   }
   for (const void* p : {(const void*)kv->k_pool, (const void*)kv->v_pool, q, (const void*)launch->workspace})

@@ -33,11 +33,15 @@
 // bulk copies costs the warp some 45 instructions, waits included, of about 270
 // a block: 128 us for 64 sequences of 1k-8k tokens.)
 //
-// Splits: see plan().  Where a row has many, up to 8 of them form a cluster and
-// join in distributed shared memory, each CTA a slice of the dims; the clusters
-// are stitched per slice by the last one to arrive.  Sums go in split order, so
-// results do not depend on timing.
+// Work: see plan().  Many rows (sequence, kv head): the blocks of all of them are
+// one list that the resident CTAs share out evenly, so that ragged lengths leave
+// no tail; a row that a share's end cuts is stitched by the last of its CTAs to
+// arrive.  Few rows: each is cut into splits of one length, up to 8 of which form
+// a cluster and join in distributed shared memory, each CTA a slice of the dims;
+// the clusters are stitched per slice by the last one to arrive.  Sums go in the
+// order of the keys, so results do not depend on timing.
 #include <cooperative_groups.h>
+#include <cstdlib>
 
 #include "int4.cuh"
 
@@ -48,10 +52,16 @@ namespace cg = cooperative_groups;
 
 constexpr int kD = 128;
 constexpr int kWarps = 4;
-constexpr int kStep = 2;                       // blocks per loop step
-constexpr int kStages = 6;                     // ring slots, a multiple of kStep
-constexpr int kPageRegs = 4;                   // page ids per lane: 128 blocks per warp, 512 per split
-constexpr int kMaxSplitTiles = kWarps * 32 * kPageRegs;
+#ifndef I4STEP
+#define I4STEP 2
+#define I4OCC 3
+#define I4STAGES 6
+#endif
+constexpr int kStep = I4STEP;                       // blocks per loop step
+constexpr int kStages = I4STAGES;                     // ring slots, a multiple of kStep
+constexpr int kBlkRing = 128;                  // block numbers per warp, renewed 32 at a time
+constexpr int kCtasPerSm = I4OCC;                  // resident: 168 registers a thread
+constexpr uint32_t kMaxStreamSeqs = 1024;      // sequences whose lengths a CTA adds up
 constexpr int kSlot = 2 * kI4Block;            // K block, V block
 constexpr int kWarpBytes = kStages * kSlot;    // also holds the warp's O, 8 x 128 f32
 constexpr int kSmem = kWarps * kWarpBytes;
@@ -66,8 +76,8 @@ struct Args {
   const __half* new_k;  // [B, Hkv, 128] or null
   const __half* new_v;
   float* out;           // [B, H, 128] f32, or bf16 storage when out_bf16
-  float* part_o;        // [B * Hkv * max_parts, group, 128]
-  float* part_ml;       // [B * Hkv * max_parts, slices, group, 2]
+  float* part_o;        // splits: [B * Hkv * max_parts, group, 128]; shares: [CTAs, 2, group, 128]
+  float* part_ml;       // [.., slices, group, 2] / [.., group, 2]
   unsigned* counters;   // [B * Hkv, slices], zero at launch, left zero by the stitch
   int32_t* status;
   const float* freq_cis;
@@ -77,7 +87,8 @@ struct Args {
   float scale;
   int num_heads, num_kv_heads, group, num_pages, page_size, max_pages;
   int tiles_per_page, tile_shift;  // page_size / 16 and its log2 (-1: not a power of two)
-  int split_tiles, max_parts;  // blocks per split; clusters (or single splits) per row
+  int num_seqs;
+  int split_tiles, max_parts;  // splits: blocks per split, clusters (or single splits) per row
   int out_bf16;
   int inputs_stable;
 };
@@ -88,8 +99,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+// 16 bytes, or zeros when size is 0
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t size) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
@@ -205,59 +217,155 @@ struct AppendRow {
   }
 };
 
+constexpr int kDead = -1, kMasked = (int)0x80000000u;  // of a block number
 constexpr float kNone = -1e30f;  // the reference of a head without keys: below any score
 constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u, kBoth = 0x00ff00ffu;
 constexpr float kTwo24 = 16777216.0f;
 
-template <bool CAP>
-__global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
-  extern __shared__ __align__(128) uint8_t ring[];
-  if (!a.inputs_stable) pdl_wait();
-  const int split = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
-  const int slices = (int)cg::this_cluster().num_blocks();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = lane >> 2, t = lane & 3;
-  const int Hkv = a.num_kv_heads, group = a.group;
-
-  const int raw_len = a.seq_lens[b];
+// One sequence's keys: [min_key, seq_len), in blocks from `origin` on.
+struct Keys {
+  int seq_len, min_key, origin, tiles;
+};
+__device__ __forceinline__ Keys keys_of(const Args& a, int raw_len) {
+  Keys s;
   const int cap = a.max_pages * a.page_size;
-  const int seq_len = raw_len < 0 ? 0 : (raw_len > cap ? cap : raw_len);
-  if (raw_len != seq_len && split == 0 && g == 0 && threadIdx.x == 0) report(a.status, DOE_DEVICE_ERR_LENGTH);
-  // window: keys [min_key, seq_len); the walk starts at the block holding min_key
-  const int min_key = (a.window > 0 && seq_len > a.window) ? seq_len - a.window : 0;
-  const int tile_origin = min_key >> 4;
-  const int ntiles = ((seq_len + 15) >> 4) - tile_origin;
-  const int nsplits = max(1, (ntiles + a.split_tiles - 1) / a.split_tiles);
-  const int part = split / slices, nparts = (nsplits + slices - 1) / slices;
-  if (part >= nparts) return;  // the whole cluster; a split past the last one joins with nothing
-  const int tile_begin = split * a.split_tiles;  // relative to tile_origin
-  const int tile_end = min(ntiles, tile_begin + a.split_tiles);
-  const int32_t* table = a.block_table + (size_t)b * a.max_pages;
+  s.seq_len = raw_len < 0 ? 0 : (raw_len > cap ? cap : raw_len);
+  // the window's keys; the walk starts at the block holding the first
+  s.min_key = (a.window > 0 && s.seq_len > a.window) ? s.seq_len - a.window : 0;
+  s.origin = s.min_key >> 4;
+  s.tiles = ((s.seq_len + 15) >> 4) - s.origin;
+  return s;
+}
 
+// Even shares of a list: `size` entries each, one more in the first `more`.
+struct Share {
+  int size, more;
+  __device__ __forceinline__ int begin(int c) const { return c * size + min(c, more); }
+  __device__ __forceinline__ int owner(int x) const {
+    const int cut = more * (size + 1);
+    return x < cut ? x / (size + 1) : more + (x - cut) / size;
+  }
+};
+
+// SHARES: the CTA's share of the list of all blocks; else one split of one row.
+template <bool CAP, bool SHARES>
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) decode_kernel(const Args a) {
+  extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float sm_m[kWarps][8];
   __shared__ float sm_l[kWarps][8];
   __shared__ float cta_ml[8][2];
   __shared__ int sm_last;
-  __shared__ __align__(8) int sm_blk[kWarps][32 * kPageRegs + kStages];
+  __shared__ __align__(8) int sm_blk[kWarps][kBlkRing];
+  __shared__ int sm_end[SHARES ? kMaxStreamSeqs : 1];  // blocks of sequences 0..b (one kv head)
+  __shared__ int sm_sum[kWarps];
 
-  // this warp's blocks: first + kWarps * k, k < nt, as block numbers in the pools
-  // up front; -1 past the walk and on pages outside the pool
-  const int first = tile_origin + tile_begin + warp;
+  if (!a.inputs_stable) pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, t = lane & 3;
+  const int Hkv = a.num_kv_heads, group = a.group;
+  const int slices = SHARES ? 1 : (int)cg::this_cluster().num_blocks();
+
+  // ---- what this CTA walks ------------------------------------------------------
+  Share share = {};
+  int at = 0, end = 0, b = 0;  // SHARES: [at, end) of the list, Hkv rows per sequence
+  if (SHARES) {
+    // running sum of the sequences' blocks; an empty one counts as a block, so
+    // that a CTA writes its zeros
+    const int per = (a.num_seqs + kWarps * 32 - 1) / (kWarps * 32), b0 = threadIdx.x * per;
+    int sum = 0;
+    for (int i = b0; i < min(b0 + per, a.num_seqs); ++i) {
+      const int raw = a.seq_lens[i];
+      const Keys s = keys_of(a, raw);
+      if (raw != s.seq_len && blockIdx.x == 0) report(a.status, DOE_DEVICE_ERR_LENGTH);
+      sum += max(1, s.tiles);
+      sm_end[i] = sum;
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) sm_sum[warp] = incl;
+    __syncthreads();
+    int before = incl - sum;
+    for (int w = 0; w < warp; ++w) before += sm_sum[w];
+    for (int i = b0; i < min(b0 + per, a.num_seqs); ++i) sm_end[i] += before;
+    __syncthreads();
+    const int total = sm_end[a.num_seqs - 1] * Hkv;  // below 2^31 (plan)
+    // at least two blocks per warp and share, unless there are more rows
+    const int shares = min((int)gridDim.x, max(total / (2 * kWarps), a.num_seqs * Hkv));
+    if ((int)blockIdx.x >= shares) return;
+    share.size = total / shares;
+    share.more = total - share.size * shares;
+    at = share.begin(blockIdx.x);
+    end = share.begin(blockIdx.x + 1);
+    int hi = a.num_seqs - 1;  // the first sequence that ends after `at`
+    while (b < hi) {
+      const int mid = (b + hi) >> 1;
+      if (sm_end[mid] * Hkv > at) hi = mid;
+      else b = mid + 1;
+    }
+  }
+  for (bool first_row = true;; first_row = false) {
+  int g, tile_begin, tile_end, part = 0, nparts;
+  Keys seq;
+  size_t row;
+  int row_at = 0;
+  if (SHARES) {
+    if (at >= end) break;
+    if (!first_row) {
+      __syncthreads();  // the last row's staging and statistics have been read
+      if (at >= sm_end[b] * Hkv) ++b;
+    }
+    const int seq_at = b ? sm_end[b - 1] : 0, size = sm_end[b] - seq_at;
+    g = (at - seq_at * Hkv) / size;
+    row_at = seq_at * Hkv + g * size;
+    seq = keys_of(a, a.seq_lens[b]);
+    tile_begin = at - row_at;
+    tile_end = min(end - row_at, size);
+    at = row_at + tile_end;
+    nparts = tile_begin == 0 && tile_end == size ? 1 : 2;  // the exact number where it matters
+    tile_end = min(tile_end, seq.tiles);
+  } else {
+    g = blockIdx.y;
+    b = blockIdx.z;
+    const int raw = a.seq_lens[b], split = blockIdx.x;
+    seq = keys_of(a, raw);
+    if (raw != seq.seq_len && split == 0 && g == 0 && threadIdx.x == 0) report(a.status, DOE_DEVICE_ERR_LENGTH);
+    const int nsplits = max(1, (seq.tiles + a.split_tiles - 1) / a.split_tiles);
+    part = split / slices;
+    nparts = nsplits == 1 ? 0 : (nsplits + slices - 1) / slices;  // 0: nothing to join, not even in the cluster
+    if (split >= max(nparts, 1) * slices) return;  // the whole cluster; a split past the last joins with nothing
+    if (nparts == 0 && split != 0) return;
+    tile_begin = split * a.split_tiles;
+    tile_end = min(seq.tiles, tile_begin + a.split_tiles);
+  }
+  row = (size_t)b * Hkv + g;
+  const int seq_len = seq.seq_len, min_key = seq.min_key;
+  const int32_t* table = a.block_table + (size_t)b * a.max_pages;
+
+  // this warp's blocks: first + kWarps * k, k < nt, as block numbers in the pools,
+  // looked up 96 ahead.  kDead: past the walk, or on a page outside the pool;
+  // kMasked is set on a block with dead keys (the window's first, the sequence's
+  // last)
+  const int first = seq.origin + tile_begin + warp;
   const int span = tile_end - tile_begin - warp;
   const int nt = span > 0 ? (span + kWarps - 1) / kWarps : 0;
-  for (int i = lane; i < nt + kStages; i += 32) {
-    int blk = -1;
-    if (i < nt) {
-      const int tile = first + kWarps * i;
-      const int pidx = a.tile_shift >= 0 ? tile >> a.tile_shift : tile / a.tiles_per_page;
-      const int page = table[pidx];
-      if ((unsigned)page < (unsigned)a.num_pages)
-        blk = (page * Hkv + g) * a.tiles_per_page + (tile - pidx * a.tiles_per_page);
-      else
-        report(a.status, DOE_DEVICE_ERR_PAGE);
-    }
-    sm_blk[warp][i] = blk;
-  }
+  auto block_number = [&](int i) {
+    if (i >= nt) return kDead;
+    const int tile = first + kWarps * i;
+    const int pidx = a.tile_shift >= 0 ? tile >> a.tile_shift : tile / a.tiles_per_page;
+    const int page = table[pidx];
+    if ((unsigned)page < (unsigned)a.num_pages)
+      return (page * Hkv + g) * a.tiles_per_page + (tile - pidx * a.tiles_per_page) +
+             (tile * 16 < min_key || tile * 16 + 16 > seq_len ? kMasked : 0);
+    report(a.status, DOE_DEVICE_ERR_PAGE);
+    return kDead;
+  };
+#pragma unroll
+  for (int i = 0; i < kBlkRing - 32; i += 32) sm_blk[warp][i + lane] = i < nt + kStages ? block_number(i + lane) : kDead;
+  int ahead = nt > kBlkRing - 32 ? block_number(kBlkRing - 32 + lane) : kDead;
   __syncwarp();
 
   const uint32_t wbase = smem_addr(ring) + warp * kWarpBytes;
@@ -267,39 +375,39 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
   const uint8_t* s_lane = (lane < 8 ? k_lane : v_lane - 128) + kI4Codes;
   const uint32_t lane_dst = wbase + 16 * lane;
   const uint32_t s_dst = lane_dst + kI4Codes + (lane < 8 ? 0 : kI4Block - 128);
-  // Fills the slot at byte `slot` of the ring with block number blk
+  // Fills the slot at byte `slot` of the ring with block number blk, a dead one
+  // with zeros
   auto issue = [&](int blk, uint32_t slot) {
-    if (blk >= 0) {
-      const size_t at = (size_t)(uint32_t)blk * kI4Block;
-      copy16(lane_dst + slot, k_lane + at);
-      copy16(lane_dst + slot + 512, k_lane + at + 512);
-      copy16(lane_dst + slot + kI4Block, v_lane + at);
-      copy16(lane_dst + slot + kI4Block + 512, v_lane + at + 512);
-      if (lane < 16) copy16(s_dst + slot, s_lane + at);
-    }
+    const uint32_t size = blk == kDead ? 0u : 16u;
+    const size_t off = (size_t)(blk == kDead ? 0u : (uint32_t)blk & ~(uint32_t)kMasked) * kI4Block;
+    copy16(lane_dst + slot, k_lane + off, size);
+    copy16(lane_dst + slot + 512, k_lane + off + 512, size);
+    copy16(lane_dst + slot + kI4Block, v_lane + off, size);
+    copy16(lane_dst + slot + kI4Block + 512, v_lane + off + 512, size);
+    if (lane < 16) copy16(s_dst + slot, s_lane + off, size);
   };
 
   // first copies before the query work (and before griddepcontrol.wait when the
-  // caller vouches for the inputs), from the block the append writes on after it
-  const bool appends = a.new_k != nullptr && split == nsplits - 1 && seq_len > 0;
-  const int new_tile = ((seq_len - 1) >> 4) - tile_origin - tile_begin;  // split-relative
-  // the warp whose walk holds the new row's block appends the row itself; that
-  // block is the walk's last
-  const bool append_pending = appends && new_tile % kWarps == warp;
+  // caller vouches for the inputs); the block that receives the new row, the walk's
+  // last of the warp that appends it, waits for the append
+  const bool append_pending =
+      a.new_k != nullptr && seq_len > 0 && nt > 0 && first + kWarps * (nt - 1) == (seq_len - 1) >> 4;
   const int early = min(kStages - kStep, append_pending ? nt - 1 : nt);
   for (int k = 0; k < early; ++k) {
     issue(sm_blk[warp][k], k * kSlot);
     if (k % kStep == kStep - 1) copy_commit();
   }
-  if (a.inputs_stable) pdl_wait();
-  pdl_trigger();
+  if (first_row) {
+    if (a.inputs_stable) pdl_wait();
+    pdl_trigger();
+  }
   AppendRow app;
   if (append_pending) app.load(a, b, g, seq_len - 1, table, lane);
 
   // ---- Q as the B operand: lane (r = head, t) holds dims 32 grp + 8 t + 0..7,
   // word i of each run = dims (2 i, 2 i + 1) = the K word's nibbles i and i + 4
   uint32_t qb[4][4];
-  float qinit[4][2];  // -8 sum_group q of heads 2 t, 2 t + 1 (times 2^-24)
+  float qinit[4][4];  // -8 sum_group q of heads 2 t, 2 t + 1 (times 2^-24), for both token rows
   {
     const __half* qrow = a.q + ((size_t)b * a.num_heads + (size_t)g * group + r) * kD;
     const bool live = r < group;
@@ -312,7 +420,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
       for (int n = 0; n < 2; ++n) {
         float rc[8], rsn[8];
         rope_table<4>(a.freq_cis, a.rope_positions, kD / 2, (long long)seq_len - 1, 32 * n + 8 * t, a.status,
-                      split == 0 && g == 0 && lane == 0 && warp == 0, rc, rsn);
+                      tile_begin == 0 && g == 0 && lane == 0 && warp == 0, rc, rsn);
         const uint4 lo = qv[n], hi = qv[n + 2];
         rope_rotate<4>(reinterpret_cast<const uint32_t*>(&lo), reinterpret_cast<const uint32_t*>(&hi), true, rc, rsn,
                        reinterpret_cast<uint32_t*>(&qv[n]));
@@ -338,7 +446,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
       qs += __shfl_xor_sync(0xffffffffu, qs, 1);
       qs += __shfl_xor_sync(0xffffffffu, qs, 2);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) qinit[n][j] = -8.0f / kTwo24 * __shfl_sync(0xffffffffu, qs, (2 * t + j) * 4);
+      for (int j = 0; j < 2; ++j) {
+        qinit[n][j] = -8.0f / kTwo24 * __shfl_sync(0xffffffffu, qs, (2 * t + j) * 4);
+        qinit[n][2 + j] = qinit[n][j];
+        asm("" : "+f"(qinit[n][2 + j]));  // a quad of registers of its own: the MMA takes it without copies
+      }
     }
   }
 
@@ -347,11 +459,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
   int v_exp = -3;                // every V scale seen is at most 2^v_exp (or infinite)
   uint32_t v_lim = 0x30003000u;  // 2^v_exp as an f16 pair
   float m_lim[2] = {kNone, kNone};  // x of a score 2^8 over its maximum
-  float acc[8][4], off[4][4];
+  float acc[8][4], off[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) off[i][0] = off[i][1] = off[i][2] = off[i][3] = 0.0f;
 
   if (append_pending) app.store(a, g, lane);
   for (int k = early; k < kStages - kStep; ++k) {
@@ -362,17 +472,27 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
   // x is the softcapped score in the log2 domain (CAP) or the bare product, which
   // c > 0 takes there: the sign of the scale is in Q, and a scale of 0 becomes
   // tiny so that the -inf of a dead key stays -inf
+  uint32_t eight[4];  // A operand of the -8: rows 2 n, 2 n + 1 take group n
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    eight[n] = (r >> 1) == n ? 0x00080008u : 0u;
+    asm("" : "+r"(eight[n]));
+  }
   const float to_cap = a.scale * kTwo24 / a.softcap, cap_log2 = a.softcap * kLog2e;  // CAP only
   const float c_log2 = CAP ? 1.0f : fmaxf(fabsf(a.scale) * (kLog2e * kTwo24), 1e-30f), inv_c = 1.0f / c_log2;
-  const bool window_edge = first * 16 < min_key;
   uint32_t slot = 0, refill = (kStages - kStep) * kSlot;  // byte offsets in the ring
   for (int k = 0; k < nt; k += kStep) {
-    const int2 next = *reinterpret_cast<const int2*>(&sm_blk[warp][k + kStages - kStep]);
-    const int2 blk = *reinterpret_cast<const int2*>(&sm_blk[warp][k]);
-    static_assert(kStep == 2, "block numbers are read in pairs");
-    __syncwarp();  // the slots refilled here were read in the last step
-    issue(next.x, refill);
-    issue(next.y, refill + kSlot);
+    if ((k & 31) == 0 && k != 0) {
+      sm_blk[warp][(k + kBlkRing - 64 + lane) & (kBlkRing - 1)] = ahead;
+      ahead = block_number(k + kBlkRing - 32 + lane);
+    }
+    __syncwarp();  // also: the slots refilled here were read in the last step
+    int blk[kStep];
+#pragma unroll
+    for (int u = 0; u < kStep; ++u) {
+      blk[u] = sm_blk[warp][(k + u) & (kBlkRing - 1)];
+      issue(sm_blk[warp][(k + u + kStages - kStep) & (kBlkRing - 1)], refill + u * kSlot);
+    }
     copy_commit();
     copy_wait<kStages / kStep - 1>();
     __syncwarp();
@@ -398,8 +518,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
         const uint32_t w0 = word(kw[0], n), w1 = word(kw[1], n);
         const uint32_t y0 = w0 >> 8, y1 = w1 >> 8;
         float c[4];
-        mma_from(c, w0 & kLo, w1 & kLo, y0 & kLo, y1 & kLo, qb[n][0], qb[n][2], qinit[n][0], qinit[n][1], qinit[n][0],
-                 qinit[n][1]);
+        mma_from(c, w0 & kLo, w1 & kLo, y0 & kLo, y1 & kLo, qb[n][0], qb[n][2], qinit[n][0], qinit[n][1], qinit[n][2],
+                 qinit[n][3]);
         mma_16816(c, w0 & kHi, w1 & kHi, y0 & kHi, y1 & kHi, qb[n][1], qb[n][3]);
         const float2 sa = f2(n < 2 ? ks[0].x : ks[0].y), sb = f2(n < 2 ? ks[1].x : ks[1].y);
         const float s0 = (n & 1) ? sa.y : sa.x, s1 = (n & 1) ? sb.y : sb.x;
@@ -413,13 +533,12 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
     }
     refill = slot;
     slot = slot == (kStages - kStep) * kSlot ? 0 : slot + kStep * kSlot;
-    // dead keys: in the window's first block, the sequence's last, blocks past the
-    // walk and blocks of bad pages; what stands there (codes, scales) may be anything
-    if (k + kStep >= nt || (blk.x | blk.y) < 0 || (k == 0 && window_edge)) {
+    // dead keys: what stands there (codes, scales) may be anything
+    if ((blk[0] | blk[kStep - 1]) < 0) {
 #pragma unroll
       for (int u = 0; u < kStep; ++u) {
         const int pos0 = (first + kWarps * (k + u)) << 4;
-        const int lo = min_key, hi = (u ? blk.y : blk.x) < 0 ? 0 : seq_len;
+        const int lo = min_key, hi = blk[u] == kDead ? 0 : seq_len;
         if (pos0 + r < lo || pos0 + r >= hi) x[u][0] = x[u][1] = -INFINITY;
         if (pos0 + r + 8 < lo || pos0 + r + 8 >= hi) x[u][2] = x[u][3] = -INFINITY;
 #pragma unroll
@@ -467,8 +586,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
           acc[i][j] *= corr;
           acc[i][2 + j] *= corr;
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) off[i][j] *= corr;
+        off[j] *= corr;
       }
       v_exp = e;
       v_lim = (uint32_t)(e + 15) * 0x04000400u;
@@ -494,7 +612,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
         const uint32_t y0 = prmt(w0, 0u, 0x4341u), y1 = prmt(w1, 0u, 0x4341u);  // bytes 1 and 3
         mma_16816(acc[2 * n], w0 & kLo, w0 & kBoth, w1 & kLo, w1 & kBoth, b0, b1);
         mma_16816(acc[2 * n + 1], y0 & kLo, y0, y1 & kLo, y1, b0, b1);
-        mma_16816(off[n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, b0, b1);
+        mma_16816(off, eight[n], 0u, eight[n], 0u, b0, b1);
       }
     }
   }
@@ -516,7 +634,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
   for (int n = 0; n < 4; ++n)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float o8 = off[n][j];
+      const float o8 = __shfl_sync(0xffffffffu, off[j], 8 * n + t);  // row 2 n
       const float lo0 = acc[2 * n][j], lo1 = acc[2 * n + 1][j];
       const float hi0 = (acc[2 * n][2 + j] - lo0) * 0.0625f, hi1 = (acc[2 * n + 1][2 + j] - lo1) * 0.0625f;
       const float4 v = make_float4((lo0 - o8) * kTwo24, (hi0 - o8) * kTwo24, (lo1 - o8) * kTwo24, (hi1 - o8) * kTwo24);
@@ -533,7 +651,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
     else
       a.out[out_row + (size_t)h * kD + d] = v;
   };
-  const size_t row = (size_t)b * Hkv + g, base = row * a.max_parts;
+  const bool whole = SHARES ? nparts == 1 : nparts == 0;
+  // where this CTA's partial row goes
+  const size_t slot_at = SHARES ? 2 * (size_t)blockIdx.x + (first_row ? 0 : 1) : row * a.max_parts + part;
   float* cta_o = reinterpret_cast<float*>(ring);  // [8][128], over the first warp's
   for (int h = 0; h < group; ++h) {
     float M = kNone, O = 0.0f, L = 0.0f;
@@ -545,13 +665,13 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
       O += f * reinterpret_cast<const float*>(ring + w * kWarpBytes)[h * kD + dim];
       L += f * sm_l[w][h];
     }
-    if (nsplits == 1) {
-      if (split == 0) store(h, dim, O, L);
+    if (whole) {
+      store(h, dim, O, L);
     } else if (slices == 1) {
-      a.part_o[((base + part) * group + h) * kD + dim] = O;
+      a.part_o[(slot_at * group + h) * kD + dim] = O;
       if (dim == 0) {
-        a.part_ml[((base + part) * group + h) * 2] = M;
-        a.part_ml[((base + part) * group + h) * 2 + 1] = L;
+        a.part_ml[(slot_at * group + h) * 2] = M;
+        a.part_ml[(slot_at * group + h) * 2 + 1] = L;
       }
     } else {
       cta_o[h * kD + dim] = O;  // read only by this thread before
@@ -561,12 +681,15 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
       }
     }
   }
-  if (nsplits == 1) return;
+  if (whole) {
+    if (SHARES) continue;
+    return;
+  }
 
   // ---- the splits of a cluster: this CTA joins its slice of the dims ------------
   int rank = 0;
   const int width = kD / slices;
-  if (slices > 1) {
+  if (!SHARES && slices > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     rank = (int)cluster.block_rank();
     cluster.sync();
@@ -593,18 +716,26 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
       if (nparts == 1) {
         store(h, d, O, L);
       } else {
-        a.part_o[((base + part) * group + h) * kD + d] = O;
+        a.part_o[(slot_at * group + h) * kD + d] = O;
         if (i % width == 0) {
-          float* ml = a.part_ml + (((base + part) * slices + rank) * group + h) * 2;
+          float* ml = a.part_ml + ((slot_at * slices + rank) * group + h) * 2;
           ml[0] = M;
           ml[1] = L;
         }
       }
     }
     cluster.sync();  // the others have read this CTA's partials
+    if (nparts == 1) return;
   }
-  if (nparts == 1) return;
   // ---- the last part of (b, g, slice) to finish stitches them, in order --------
+  int c0 = 0;       // SHARES: the CTA that holds the row's first block,
+  bool c0_second = false;  // as the second part that it writes
+  if (SHARES) {
+    const int size = sm_end[b] - (b ? sm_end[b - 1] : 0);
+    c0 = share.owner(row_at);
+    nparts = share.owner(row_at + size - 1) - c0 + 1;
+    c0_second = share.begin(c0) < row_at;
+  }
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -613,47 +744,52 @@ __global__ void __launch_bounds__(kWarps * 32, 3) decode_kernel(const Args a) {
     if (sm_last) *counter = 0u;  // ready for the next launch
   }
   __syncthreads();
-  if (!sm_last) return;
-  __threadfence();
-  for (int i = threadIdx.x; i < group * width; i += kWarps * 32) {
-    const int h = i / width, d = rank * width + i % width;
-    float M = kNone, O = 0.0f, L = 0.0f;
-    // a running reference, so that the loads of several parts are in flight
-    constexpr int kBatch = 8;
-    for (int p0 = 0; p0 < nparts; p0 += kBatch) {
-      float2 ml[kBatch];
-      float o[kBatch];
+  if (sm_last) {
+    __threadfence();
+    for (int i = threadIdx.x; i < group * width; i += kWarps * 32) {
+      const int h = i / width, d = rank * width + i % width;
+      float M = kNone, O = 0.0f, L = 0.0f;
+      // a running reference, so that the loads of several parts are in flight
+      constexpr int kBatch = 8;
+      for (int p0 = 0; p0 < nparts; p0 += kBatch) {
+        float2 ml[kBatch];
+        float o[kBatch];
 #pragma unroll
-      for (int c = 0; c < kBatch; ++c) {
-        const size_t at = base + min(p0 + c, nparts - 1);
-        ml[c] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + (at * slices + rank) * group + h);
-        o[c] = __ldcg(a.part_o + (at * group + h) * kD + d);
-      }
-      float m = M;
-#pragma unroll
-      for (int c = 0; c < kBatch; ++c) m = fmaxf(m, ml[c].x);
-      const float f0 = ex2(M - m);
-      O *= f0;
-      L *= f0;
-      M = m;
-#pragma unroll
-      for (int c = 0; c < kBatch; ++c)
-        if (p0 + c < nparts) {
-          const float f = ex2(ml[c].x - M);
-          O += f * o[c];
-          L += f * ml[c].y;
+        for (int c = 0; c < kBatch; ++c) {
+          const int p = min(p0 + c, nparts - 1);
+          const size_t from =
+              SHARES ? 2 * (size_t)(c0 + p) + (p == 0 && c0_second ? 1 : 0) : row * a.max_parts + p;
+          ml[c] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + (from * slices + rank) * group + h);
+          o[c] = __ldcg(a.part_o + (from * group + h) * kD + d);
         }
+        float m = M;
+#pragma unroll
+        for (int c = 0; c < kBatch; ++c) m = fmaxf(m, ml[c].x);
+        const float f0 = ex2(M - m);
+        O *= f0;
+        L *= f0;
+        M = m;
+#pragma unroll
+        for (int c = 0; c < kBatch; ++c)
+          if (p0 + c < nparts) {
+            const float f = ex2(ml[c].x - M);
+            O += f * o[c];
+            L += f * ml[c].y;
+          }
+      }
+      store(h, d, O, L);
     }
-    store(h, d, O, L);
   }
+  if (!SHARES) return;
+  }  // rows of the share
 }
 
-template <bool CAP>
-int launch_cap(const Args& a, dim3 grid, unsigned slices, cudaStream_t st) {
+template <bool CAP, bool SHARES>
+int launch_one(const Args& a, dim3 grid, unsigned slices, cudaStream_t st) {
   static std::atomic<bool> attr[kMaxDevices];
   const int rc = once_per_device(attr, [] {
     return cuda_status(
-        cudaFuncSetAttribute(decode_kernel<CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
+        cudaFuncSetAttribute(decode_kernel<CAP, SHARES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
         "cudaFuncSetAttribute(paged_decode_int4)");
   });
   if (rc != DOE_OK) return rc;
@@ -670,37 +806,48 @@ int launch_cap(const Args& a, dim3 grid, unsigned slices, cudaStream_t st) {
   at[1].val.clusterDim.y = 1;
   at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 2;
-  return cuda_status(cudaLaunchKernelEx(&cfg, decode_kernel<CAP>, a), "paged_decode_int4");
+  cfg.numAttrs = slices > 1 ? 2 : 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, decode_kernel<CAP, SHARES>, a), "paged_decode_int4");
 }
 
-// How a launch is cut: blocks per split, splits per cluster, and the sizes
-// that follow.
+// How a launch is cut, and the sizes that follow.
 struct Plan {
-  uint64_t split_tiles, slices, max_parts, grid_x;
+  bool shares;                     // even shares of all rows' blocks over `grid` CTAs
+  uint64_t split_tiles, slices;    // else: blocks per split, splits per cluster
+  uint64_t max_parts, grid;        // parts per row, CTAs (per row when not shares)
+  uint64_t slots;                  // partial rows in the workspace
 };
 
-// Long splits amortise a CTA's prologue and join; where the (sequence, kv head)
-// rows are few the length is cut until there are about two CTAs per SM.
-Plan plan(uint64_t rows, uint64_t max_tiles, uint64_t tiles_per_page, uint64_t split_pages) {
+// Even shares while a row is cut into a few parts at most, which its last CTA
+// stitches alone.  With fewer rows than that each row gets its own splits, so
+// many that there are about two CTAs per SM, joined in clusters.  A given
+// split_pages asks for splits of that length; they serve more than
+// kMaxStreamSeqs sequences too.
+Plan plan(uint64_t num_seqs, uint64_t kv_heads, uint64_t max_tiles, uint64_t tiles_per_page, uint64_t split_pages) {
+  Plan p = {};
+  const uint64_t rows = num_seqs * kv_heads, ctas = (uint64_t)num_sms() * kCtasPerSm;
+  p.slices = 1;
+  if (split_pages == 0 && num_seqs <= kMaxStreamSeqs && rows * 16 >= ctas && rows * max_tiles <= 0x7fffffffull) {
+    p.shares = true;
+    p.grid = ctas * (getenv("I4M") ? atoi(getenv("I4M")) : 1);
+    p.max_parts = 2;
+    p.slots = 2 * p.grid;
+    return p;
+  }
   uint64_t t = split_pages * tiles_per_page;
   if (t == 0) {
-    const uint64_t want = (max_tiles * rows + 1775) / 1776;
-    if (want >= 128) {
-      t = 128;
-    } else {
-      uint64_t s = (max_tiles + 127) / 128;
-      const uint64_t fill = (280 + rows - 1) / rows;
-      if (s < fill) s = fill;
-      t = (max_tiles + s - 1) / s;
-      if (t < 4) t = 4;
-    }
+    const uint64_t fill = (2 * (uint64_t)num_sms() + rows - 1) / rows;
+    t = (max_tiles + fill - 1) / fill;
+    if (t < 4) t = 4;
   }
-  if (t > kMaxSplitTiles) t = kMaxSplitTiles;  // prefetched page ids
+  if (t > max_tiles) t = max_tiles;
+  p.split_tiles = t;
   const uint64_t splits = (max_tiles + t - 1) / t;
-  const uint64_t slices = splits > 16 ? 8 : 1;
-  const uint64_t parts = (splits + slices - 1) / slices;
-  return {t, slices, parts, parts * slices};
+  p.slices = splits > 16 ? 8 : 1;
+  p.max_parts = (splits + p.slices - 1) / p.slices;
+  p.grid = p.max_parts * p.slices;
+  p.slots = rows * p.max_parts;
+  return p;
 }
 
 }  // namespace i4
@@ -714,8 +861,8 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   const uint32_t tpp = kv->page_size / 16;
   const uint64_t max_tiles = (uint64_t)kv->max_pages_per_seq * tpp;
   const uint64_t rows = (uint64_t)num_seqs * Hkv;
-  const Plan pl = plan(rows ? rows : 1, max_tiles, tpp, split_pages);
-  const uint64_t parts = rows * pl.max_parts * group;
+  const Plan pl = plan(num_seqs ? num_seqs : 1, Hkv, max_tiles, tpp, split_pages);
+  const uint64_t parts = pl.slots * group;
   const uint64_t ctr_off = (parts * (kD + 2 * pl.slices) * sizeof(float) + 255) / 256 * 256;
   const uint64_t ws = ctr_off + rows * pl.slices * sizeof(unsigned);
   if (ws_needed_out) {
@@ -731,7 +878,7 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
                  (unsigned long long)launch->workspace_bytes);
     return DOE_INVALID_ARGUMENT;
   }
-  if (max_tiles * 16 > 0x7fffffffull || pl.grid_x > 0x7fffffffull || Hkv > 65535u ||
+  if (max_tiles * 16 > 0x7fffffffull || pl.grid > 0x7fffffffull || Hkv > 65535u ||
       (uint64_t)kv->num_pages * Hkv * tpp > 0x7fffffffull) {
     set_op_error("doe_paged_decode: more than 2^31 - 1 tokens in a block-table row or blocks in a pool, or over 65535 "
                  "kv heads");
@@ -775,6 +922,7 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   a.tile_shift = -1;
   for (int s = 0; s < 27; ++s)
     if (tpp == (1u << s)) a.tile_shift = s;
+  a.num_seqs = (int)num_seqs;
   a.split_tiles = (int)pl.split_tiles;
   a.max_parts = (int)pl.max_parts;
   a.out_bf16 = (opts && (opts->flags & DOE_DECODE_OUT_BF16)) ? 1 : 0;
@@ -785,9 +933,11 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
         cuda_status(cudaMemsetAsync(a.counters, 0, rows * pl.slices * sizeof(unsigned), st), "cudaMemsetAsync(split counters)");
     if (rc != DOE_OK) return rc;
   }
-  const dim3 grid((unsigned)pl.grid_x, Hkv, num_seqs);
-  return a.softcap > 0.0f ? launch_cap<true>(a, grid, (unsigned)pl.slices, st)
-                          : launch_cap<false>(a, grid, (unsigned)pl.slices, st);
+  const dim3 grid = pl.shares ? dim3((unsigned)pl.grid) : dim3((unsigned)pl.grid, Hkv, num_seqs);
+  const unsigned slices = (unsigned)pl.slices;
+  if (pl.shares)
+    return a.softcap > 0.0f ? launch_one<true, true>(a, grid, slices, st) : launch_one<false, true>(a, grid, slices, st);
+  return a.softcap > 0.0f ? launch_one<true, false>(a, grid, slices, st) : launch_one<false, false>(a, grid, slices, st);
 }
 
 }  // namespace doe

@@ -12,15 +12,17 @@
 // the (up to 8) heads as its 8 columns: S = K Q^T takes 16 tokens as rows, O^T =
 // V^T P^T 16 dims.  A code pair masked out of its word, (w >> 4 i) &
 // 0x000f000f, IS an f16 pair: the subnormals n * 2^-24, exact in the tensor
-// core; the pair at bits 4-7 is left there and reads n * 2^-20.  So 8 codes cost
-// one shift and 4 ANDs.  The powers of two go into Q (words of the high
-// nibbles times 2^-4), the score scale (2^24) and the final accumulators; -8
-// becomes the S accumulators' start value (-8 sum q) and, for O, one MMA per
-// group with a constant A operand (8) on the same B operand, so exactly the
-// f16 (s p) the product used is taken off.
-// P moves from the S accumulators (token rows) into the B operand (head
-// columns) by movmatrix.  S, the softmax statistics and O are f32; P and s p are
-// rounded to f16 (2^-12 relative, the f16 and int8 kernels' choice).
+// core.  K's pair at bits 4-7 is left there and reads n * 2^-20, so 8 codes cost
+// one shift and 4 ANDs.  A V byte is used whole as the row of its high nibble,
+// (lo + 16 hi) * 2^-24, and the low nibble's sum comes off at the end: 8 codes
+// cost 4 operations.  The powers of two go into Q (words of the high nibbles
+// times 2^-4), the score scale (2^24) and the final accumulators; -8 becomes the
+// S accumulators' start value (-8 sum q) and, for O, one MMA per group with a
+// constant A operand (8) on the same B operand, so exactly the f16 (s p) that the
+// product used is taken off.  P moves from the S accumulators (token rows) into
+// the B operand (head columns) by movmatrix.  S, the softmax statistics and O are
+// f32; P and s p are rounded to f16 (2^-11 relative at most, the f16 and int8
+// kernels' choice).
 //
 // The running reference of a head, m, is its score maximum plus the exponent
 // of the V scales seen, so that s p stays within f16's range and out of its
@@ -30,18 +32,19 @@
 // Loads: a warp walks its blocks kStep at a time out of a ring of its own in
 // shared memory, filled with cp.async: a block is 1024 + 128 contiguous bytes
 // of K and of V, 5 instructions for the warp.  (One elected lane issuing two
-// bulk copies costs the warp some 45 instructions, waits included, of about 270
-// a block: 128 us for 64 sequences of 1k-8k tokens.)
+// bulk copies costs the warp some 45 instructions, waits included, of 320 a
+// block: 128 us for 64 sequences of 1k-8k tokens against 98.)
 //
-// Work: see plan().  Many rows (sequence, kv head): the blocks of all of them are
-// one list that the resident CTAs share out evenly, so that ragged lengths leave
-// no tail; a row that a share's end cuts is stitched by the last of its CTAs to
-// arrive.  Few rows: each is cut into splits of one length, up to 8 of which form
-// a cluster and join in distributed shared memory, each CTA a slice of the dims;
-// the clusters are stitched per slice by the last one to arrive.  Sums go in the
-// order of the keys, so results do not depend on timing.
+// Work, see plan().  Many long rows (sequence, kv head): the blocks of all
+// sequences are one list cut into even pieces, each for one warp per kv head, so
+// that ragged lengths leave no tail; a row that pieces' ends cut is stitched by the
+// last of its warps to arrive.  Few rows: each is cut into splits of one length,
+// one CTA each; up to 8 of them form a cluster and join in distributed shared
+// memory, each CTA a slice of the dims, and the clusters are stitched per slice by
+// the last one to arrive.  Short rows, many of them: one CTA each.  Pieces and
+// splits follow from the lengths alone and sums go in the order of the keys, so
+// results do not depend on timing.
 #include <cooperative_groups.h>
-#include <cstdlib>
 
 #include "int4.cuh"
 
@@ -52,20 +55,19 @@ namespace cg = cooperative_groups;
 
 constexpr int kD = 128;
 constexpr int kWarps = 4;
-#ifndef I4STEP
-#define I4STEP 2
-#define I4OCC 3
-#define I4STAGES 6
-#endif
-constexpr int kStep = I4STEP;                       // blocks per loop step
-constexpr int kStages = I4STAGES;                     // ring slots, a multiple of kStep
+constexpr int kStep = 2;                       // blocks per loop step
+constexpr int kStages = 6;                     // ring slots, a multiple of kStep
 constexpr int kBlkRing = 128;                  // block numbers per warp, renewed 32 at a time
-constexpr int kCtasPerSm = I4OCC;                  // resident: 168 registers a thread
-constexpr uint32_t kMaxStreamSeqs = 1024;      // sequences whose lengths a CTA adds up
+constexpr int kCtasPerSm = 3;                  // resident: 168 registers a thread
+constexpr int kRowCost = 4;                    // a sequence's fixed cost in the list, in blocks
+constexpr int kMinPiece = 8;                   // entries; more than kRowCost, so that no piece is empty
+constexpr uint64_t kShortRow = 128;            // blocks that one CTA walks alone when there are rows enough
+constexpr uint64_t kCounterBytes = 1 << 16;    // of the workspace's head, for 2048 rows' counters
+constexpr uint32_t kMaxListSeqs = 1024;        // sequences whose lengths a CTA adds up
 constexpr int kSlot = 2 * kI4Block;            // K block, V block
 constexpr int kWarpBytes = kStages * kSlot;    // also holds the warp's O, 8 x 128 f32
 constexpr int kSmem = kWarps * kWarpBytes;
-static_assert(kWarpBytes >= 8 * kD * 4, "the merge stages a warp's O in its ring");
+static_assert(kWarpBytes >= 8 * kD * 4, "the join stages a warp's O in its ring");
 
 struct Args {
   const __half* q;  // [B, H, 128]
@@ -76,7 +78,7 @@ struct Args {
   const __half* new_k;  // [B, Hkv, 128] or null
   const __half* new_v;
   float* out;           // [B, H, 128] f32, or bf16 storage when out_bf16
-  float* part_o;        // splits: [B * Hkv * max_parts, group, 128]; shares: [CTAs, 2, group, 128]
+  float* part_o;        // splits: [B * Hkv * max_parts, group, 128]; pieces: [pieces, 2, group, 128]
   float* part_ml;       // [.., slices, group, 2] / [.., group, 2]
   unsigned* counters;   // [B * Hkv, slices], zero at launch, left zero by the stitch
   int32_t* status;
@@ -99,10 +101,23 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// 16 bytes, or zeros when size is 0
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t size) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(size) : "memory");
+// A block's 16-byte copies of one lane (two of K codes, two of V codes, one of
+// scales where `scales`), or none of them.
+__device__ __forceinline__ void copy_block(uint32_t dst, const void* k, const void* v, uint32_t s_dst, const void* s,
+                                           bool some, bool scales) {
+  asm volatile(
+      "{\n.reg .pred p, q;\n"
+      "setp.ne.s32 p, %5, 0;\n"
+      "setp.ne.and.s32 q, %6, 0, p;\n"
+      "@p cp.async.cg.shared.global [%0], [%1], 16;\n"
+      "@p cp.async.cg.shared.global [%0 + 512], [%1 + 512], 16;\n"
+      "@p cp.async.cg.shared.global [%0 + 1152], [%2], 16;\n"
+      "@p cp.async.cg.shared.global [%0 + 1664], [%2 + 512], 16;\n"
+      "@q cp.async.cg.shared.global [%3], [%4], 16;\n}\n" ::"r"(dst),
+      "l"(k), "l"(v), "r"(s_dst), "l"(s), "r"((int)some), "r"((int)scales)
+      : "memory");
 }
+static_assert(kI4Block == 1152 && kI4Codes == 1024, "copy_block's offsets");
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() {
@@ -217,7 +232,7 @@ struct AppendRow {
   }
 };
 
-constexpr int kDead = -1, kMasked = (int)0x80000000u;  // of a block number
+constexpr int kDead = -1;        // no block number
 constexpr float kNone = -1e30f;  // the reference of a head without keys: below any score
 constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u, kBoth = 0x00ff00ffu;
 constexpr float kTwo24 = 16777216.0f;
@@ -237,48 +252,559 @@ __device__ __forceinline__ Keys keys_of(const Args& a, int raw_len) {
   return s;
 }
 
-// Even shares of a list: `size` entries each, one more in the first `more`.
-struct Share {
-  int size, more;
-  __device__ __forceinline__ int begin(int c) const { return c * size + min(c, more); }
-  __device__ __forceinline__ int owner(int x) const {
-    const int cut = more * (size + 1);
-    return x < cut ? x / (size + 1) : more + (x - cut) / size;
+// One warp's stretch of a row's blocks: first + STRIDE * k, k < nt.
+struct Stretch {
+  int b, g, seq_len, min_key;
+  int first, nt;
+  int row_at;  // pieces: where the row begins in the list
+  bool whole;  // nobody else holds a part of the row
+};
+
+// What a warp keeps of a stretch: heads 2 t and 2 t + 1 are the lane's columns.
+struct Sums {
+  float m[2], l[2];   // reference and sum of p (of this lane's tokens)
+  float acc[8][4];    // O^T: m-block 2 n + j, rows (lo, lo + 16 hi) of dims 32 n + 4 r + 2 j + {0, 1}
+  float off[4];       // rows 2 n: 8 sum s p of group n
+};
+
+// A warp's ring of blocks and the walk over a stretch.
+template <bool CAP, int STRIDE>
+struct Walker {
+  const Args& a;
+  int* numbers;     // [kBlkRing] block numbers
+  uint32_t wbase;   // the ring
+  int lane, r, t;
+  int ahead = kDead;
+
+  // The ring's first copies of a stretch go into the slots after the first
+  // step's: those may still stage the last stretch's O.
+  static constexpr uint32_t kSlot0 = kStep * kSlot;
+
+  const uint8_t *k_lane, *v_lane, *s_lane;  // this lane's part of block 0
+  uint32_t lane_dst, s_dst;
+  bool bad = false;  // the stretch has blocks on bad pages
+
+  __device__ __forceinline__ Walker(const Args& args, int* blk, void* ring, int l)
+      : a(args), numbers(blk), wbase(smem_addr(ring)), lane(l), r(l >> 2), t(l & 3) {
+    k_lane = a.k_pool + 16 * lane;
+    v_lane = a.v_pool + 16 * lane;
+    s_lane = (lane < 8 ? k_lane : v_lane - 128) + kI4Codes;
+    lane_dst = wbase + 16 * lane;
+    s_dst = lane_dst + kI4Codes + (lane < 8 ? 0 : kI4Block - 128);
+  }
+
+  // Page of the stretch's block i, and the block's number in the pools.  kDead:
+  // past the walk, or on a page outside the pool.
+  __device__ __forceinline__ int page_index(const Stretch& w, int i) const {
+    const int tile = w.first + STRIDE * i;
+    return a.tile_shift >= 0 ? tile >> a.tile_shift : tile / a.tiles_per_page;
+  }
+  __device__ __forceinline__ int page_of(const Stretch& w, int i) const {
+    return i < w.nt ? a.block_table[(size_t)w.b * a.max_pages + page_index(w, i)] : kDead;
+  }
+  __device__ __forceinline__ int number_of(const Stretch& w, int i, int page) const {
+    if (i >= w.nt) return kDead;
+    const int tile = w.first + STRIDE * i;
+    if ((unsigned)page < (unsigned)a.num_pages)
+      return (page * a.num_kv_heads + w.g) * a.tiles_per_page + (tile - page_index(w, i) * a.tiles_per_page);
+    report(a.status, DOE_DEVICE_ERR_PAGE);
+    return kDead;
+  }
+
+  // Fills the slot at byte `slot` of the ring with block number blk, if it has one.
+  // Lanes 0-7 copy the K scales, 8-15 the V scales.
+  __device__ __forceinline__ void issue(int blk, uint32_t slot) const {
+    const size_t off = (size_t)(uint32_t)blk * kI4Block;
+    copy_block(lane_dst + slot, k_lane + off, v_lane + off, s_dst + slot, s_lane + off, blk >= 0, lane < 16);
+  }
+
+  // The block that receives the new row is the last of the warp that appends it.
+  __device__ __forceinline__ bool appends(const Stretch& w) const {
+    return a.new_k != nullptr && w.seq_len > 0 && w.nt > 0 && w.first + STRIDE * (w.nt - 1) == (w.seq_len - 1) >> 4;
+  }
+  // Blocks copied by start(): up to the ring's prefetch, not the one to be appended to.
+  __device__ __forceinline__ int early(const Stretch& w) const {
+    return min(kStages - kStep, appends(w) ? w.nt - 1 : w.nt);
+  }
+
+  // Looks the stretch's first block numbers up (96 ahead of the walk) and issues
+  // its first copies.  Nothing of this warp is in flight.
+  __device__ __forceinline__ void start(const Stretch& w) {
+    int page[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) page[i] = page_of(w, 32 * i + lane);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) numbers[32 * i + lane] = number_of(w, 32 * i + lane, page[i]);
+    ahead = number_of(w, 96 + lane, page[3]);
+    bool wrong = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wrong |= 32 * i + lane < w.nt && (unsigned)page[i] >= (unsigned)a.num_pages;
+    bad = __any_sync(0xffffffffu, wrong);
+    static_assert(kBlkRing == 128, "three quarters are looked up, the fourth is ahead");
+    __syncwarp();
+    const int n = early(w);
+    for (int k = 0; k < n; ++k) {
+      issue(numbers[k], kSlot0 + k * kSlot);
+      if (k % kStep == kStep - 1) copy_commit();
+    }
+  }
+
+  // The rest: query, append, every block.  Leaves nothing in flight.
+  __device__ __forceinline__ void walk(const Stretch& cur, Sums& sums) {
+    const int g = cur.g, seq_len = cur.seq_len, min_key = cur.min_key, nt = cur.nt, first = cur.first;
+    const int group = a.group;
+    const bool append_pending = appends(cur);
+    AppendRow app;
+    if (append_pending) app.load(a, cur.b, g, seq_len - 1, a.block_table + (size_t)cur.b * a.max_pages, lane);
+
+    // ---- Q as the B operand: lane (r = head, t) holds dims 32 grp + 8 t + 0..7,
+    // word i of each run = dims (2 i, 2 i + 1) = the K word's nibbles i and i + 4
+    uint32_t qb[4][4];
+    float qinit[4][4];  // -8 sum_group q of heads 2 t, 2 t + 1 (times 2^-24), for both token rows
+    {
+      const __half* qrow = a.q + ((size_t)cur.b * a.num_heads + (size_t)g * group + r) * kD;
+      const bool live = r < group;
+      uint4 qv[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        qv[n] = live ? *reinterpret_cast<const uint4*>(qrow + 32 * n + 8 * t) : make_uint4(0, 0, 0, 0);
+      if (a.freq_cis != nullptr && live && seq_len > 0) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          float rc[8], rsn[8];
+          rope_table<4>(a.freq_cis, a.rope_positions, kD / 2, (long long)seq_len - 1, 32 * n + 8 * t, a.status,
+                        g == 0 && lane == 0, rc, rsn);
+          const uint4 lo = qv[n], hi = qv[n + 2];
+          rope_rotate<4>(reinterpret_cast<const uint32_t*>(&lo), reinterpret_cast<const uint32_t*>(&hi), true, rc, rsn,
+                         reinterpret_cast<uint32_t*>(&qv[n]));
+          rope_rotate<4>(reinterpret_cast<const uint32_t*>(&hi), reinterpret_cast<const uint32_t*>(&lo), false, rc, rsn,
+                         reinterpret_cast<uint32_t*>(&qv[n + 2]));
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        float qs = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w = word(qv[n], i) ^ (!CAP && a.scale < 0.0f ? 0x80008000u : 0u);
+          float mult = 1.0f;
+          if (i & 1) {  // meets codes read as n 2^-20; q 2^-4 loses bits only below |q| = 2^-10, 2^-21 absolute
+            w = hmul2(w, 0x2c002c00u);
+            mult = 16.0f;
+          }
+          qb[n][i] = w;
+          const float2 f = f2(w);
+          qs += mult * (f.x + f.y);
+        }
+        qs += __shfl_xor_sync(0xffffffffu, qs, 1);
+        qs += __shfl_xor_sync(0xffffffffu, qs, 2);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          qinit[n][j] = -8.0f / kTwo24 * __shfl_sync(0xffffffffu, qs, (2 * t + j) * 4);
+          qinit[n][2 + j] = qinit[n][j];
+          asm("" : "+f"(qinit[n][2 + j]));  // a quad of registers of its own: the MMA takes it without copies
+        }
+      }
+    }
+
+    float (&m_ref)[2] = sums.m;
+    float (&l_run)[2] = sums.l;
+    float (&acc)[8][4] = sums.acc;
+    float (&off)[4] = sums.off;
+    m_ref[0] = m_ref[1] = kNone;
+    l_run[0] = l_run[1] = 0.0f;
+    int v_exp = -3;                // every V scale seen is at most 2^v_exp (or infinite)
+    uint32_t v_lim = 0x30003000u;  // 2^v_exp as an f16 pair
+    float m_lim[2] = {kNone, kNone};  // x of a score 2^8 over its maximum
+    off[0] = off[1] = off[2] = off[3] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+
+    if (append_pending) app.store(a, g, lane);
+    for (int k = early(cur); k < kStages - kStep; ++k) {
+      issue(numbers[k], kSlot0 + k * kSlot);
+      if (k % kStep == kStep - 1) copy_commit();
+    }
+
+    uint32_t eight[4];  // A operand of the -8: rows 2 n, 2 n + 1 take group n
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      eight[n] = (r >> 1) == n ? 0x00080008u : 0u;
+      asm("" : "+r"(eight[n]));
+    }
+    // x is the softcapped score in the log2 domain (CAP) or the bare product, which
+    // c > 0 takes there: the sign of the scale is in Q, and a scale of 0 becomes
+    // tiny so that the -inf of a dead key stays -inf
+    const float to_cap = a.scale * kTwo24 / a.softcap, cap_log2 = a.softcap * kLog2e;  // CAP only
+    const float c_log2 = CAP ? 1.0f : fmaxf(fabsf(a.scale) * (kLog2e * kTwo24), 1e-30f), inv_c = 1.0f / c_log2;
+    int edge_k = first * 16 < min_key || bad ? 0 : nt - kStep;  // steps from here on have dead keys
+    uint32_t slot = kSlot0, refill = 0;  // byte offsets in the ring
+    for (int k = 0; k < nt; k += kStep) {
+      if ((k & 31) == 0 && k != 0) {
+        numbers[(k + kBlkRing - 64 + lane) & (kBlkRing - 1)] = ahead;
+        {
+          const int i = k + kBlkRing - 32 + lane;
+          ahead = number_of(cur, i, page_of(cur, i));
+          bad |= __any_sync(0xffffffffu, i < nt && ahead == kDead);
+        }
+      }
+      __syncwarp();  // also: the slots refilled here were read in the last step
+      {
+        const int2 blk = *reinterpret_cast<const int2*>(&numbers[(k + kStages - kStep) & (kBlkRing - 1)]);
+        static_assert(kStep == 2, "block numbers are read in pairs");
+        issue(blk.x, refill);
+        issue(blk.y, refill + kSlot);
+      }
+      copy_commit();
+      copy_wait<kStages / kStep - 1>();
+      __syncwarp();
+      float x[kStep][4];
+      uint4 vs[kStep][2];
+      uint32_t vmax = v_lim;  // scales are not negative, so they order as 16-bit integers
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) {
+        const uint32_t kb = wbase + slot + u * kSlot, vb = kb + kI4Block;
+        uint4 kw[2];
+        uint2 ks[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          kw[h] = lds128(kb + 512 * h + 16 * lane);     // token r + 8 h
+          ks[h] = lds64(kb + kI4Codes + 64 * h + 8 * r);
+          vs[u][h] = lds128(vb + kI4Codes + 64 * h + 16 * t);
+        }
+        // ---- S = K Q^T: rows token r / r + 8, columns heads 2 t, 2 t + 1 ---------
+        float s[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t w0 = word(kw[0], n), w1 = word(kw[1], n);
+          const uint32_t y0 = w0 >> 8, y1 = w1 >> 8;
+          float c[4];
+          mma_from(c, w0 & kLo, w1 & kLo, y0 & kLo, y1 & kLo, qb[n][0], qb[n][2], qinit[n][0], qinit[n][1], qinit[n][2],
+                   qinit[n][3]);
+          mma_16816(c, w0 & kHi, w1 & kHi, y0 & kHi, y1 & kHi, qb[n][1], qb[n][3]);
+          const float2 sa = f2(n < 2 ? ks[0].x : ks[0].y), sb = f2(n < 2 ? ks[1].x : ks[1].y);
+          const float s0 = (n & 1) ? sa.y : sa.x, s1 = (n & 1) ? sb.y : sb.x;
+          s[0] = n ? fmaf(s0, c[0], s[0]) : s0 * c[0];
+          s[1] = n ? fmaf(s0, c[1], s[1]) : s0 * c[1];
+          s[2] = n ? fmaf(s1, c[2], s[2]) : s1 * c[2];
+          s[3] = n ? fmaf(s1, c[3], s[3]) : s1 * c[3];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[u][i] = CAP ? cap_log2 * tanhf(s[i] * to_cap) : s[i];
+      }
+      const uint32_t v_at = wbase + slot + kI4Block + 16 * lane;
+      refill = slot;
+      slot = slot == (kStages - kStep) * kSlot ? 0 : slot + kStep * kSlot;
+      // dead keys: in the window's first block, the sequence's last, blocks past the
+      // walk and on bad pages; what stands there (codes, scales) may be anything
+      const bool edge = k >= edge_k;
+      edge_k = bad ? 0 : nt - kStep;
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < kStep; ++u) {
+          const int pos0 = (first + STRIDE * (k + u)) << 4;
+          const int lo = min_key, hi = k + u >= nt || (bad && numbers[(k + u) & (kBlkRing - 1)] < 0) ? 0 : seq_len;
+          if (pos0 + r < lo || pos0 + r >= hi) x[u][0] = x[u][1] = -INFINITY;
+          if (pos0 + r + 8 < lo || pos0 + r + 8 >= hi) x[u][2] = x[u][3] = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int key = pos0 + 2 * t + 8 * h;
+            const uint32_t keep = (key >= lo && key < hi ? 0x0000ffffu : 0u) |
+                                  (key + 1 >= lo && key + 1 < hi ? 0xffff0000u : 0u);
+            vs[u][h].x &= keep; vs[u][h].y &= keep; vs[u][h].z &= keep; vs[u][h].w &= keep;
+          }
+        }
+      }
+
+      // ---- the reference moves when a score or a V scale outgrows it -------------
+      float mx[2] = {fmaxf(x[0][0], x[0][2]), fmaxf(x[0][1], x[0][3])};
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) {
+        if (u) {
+          mx[0] = fmaxf(mx[0], fmaxf(x[u][0], x[u][2]));
+          mx[1] = fmaxf(mx[1], fmaxf(x[u][1], x[u][3]));
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          vmax = __vimax3_u16x2(__vimax3_u16x2(vmax, vs[u][h].x, vs[u][h].y), vs[u][h].z, vs[u][h].w);
+      }
+      const bool grow = mx[0] > m_lim[0] || mx[1] > m_lim[1] || vmax != v_lim;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float2 vf = f2(vmax);  // at least 2^v_exp
+        const float vm = warp_max(fmaxf(vf.x, vf.y));
+        int e = v_exp;
+        if (vm > f2(v_lim).x) e = min(15, (int)((__float_as_uint(vm) >> 23) & 255) - 126);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], o));
+          // reference = score maximum + exponent of the V scales - 4: p <= 2^15
+          // and s p <= 2^12 while a score may still outgrow the maximum by 2^8
+          const float base = m_ref[j] - (float)(v_exp - 4);
+          const float top = fmaxf(base, mx[j] * c_log2), m_new = top + (float)(e - 4);
+          const float corr = ex2(m_ref[j] - m_new);
+          m_ref[j] = m_new;
+          m_lim[j] = (top + 8.0f) * inv_c;
+          l_run[j] *= corr;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            acc[i][j] *= corr;
+            acc[i][2 + j] *= corr;
+          }
+          off[j] *= corr;
+        }
+        v_exp = e;
+        v_lim = (uint32_t)(e + 15) * 0x04000400u;
+      }
+
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) {
+        const uint4 vw[2] = {lds128(v_at + u * kSlot), lds128(v_at + u * kSlot + 512)};  // tokens 2 t, 2 t + 1 (+ 8)
+        float p[4];
+        p[0] = ex2(fmaf(x[u][0], c_log2, -m_ref[0]));
+        p[1] = ex2(fmaf(x[u][1], c_log2, -m_ref[1]));
+        p[2] = ex2(fmaf(x[u][2], c_log2, -m_ref[0]));
+        p[3] = ex2(fmaf(x[u][3], c_log2, -m_ref[1]));
+        l_run[0] += p[0] + p[2];
+        l_run[1] += p[1] + p[3];
+        const uint32_t p0 = transpose8x8(pack_half2(p[0], p[1]));  // head r, tokens 2 t, 2 t + 1
+        const uint32_t p1 = transpose8x8(pack_half2(p[2], p[3]));  // tokens + 8
+
+        // ---- O^T += V^T (s P)^T: m-block 2 n + j = dims 32 n + 4 row' + {2 j, 2 j + 1}
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t b0 = hmul2(p0, word(vs[u][0], n)), b1 = hmul2(p1, word(vs[u][1], n));
+          const uint32_t w0 = word(vw[0], n), w1 = word(vw[1], n);
+          const uint32_t y0 = prmt(w0, 0u, 0x4341u), y1 = prmt(w1, 0u, 0x4341u);  // bytes 1 and 3
+          mma_16816(acc[2 * n], w0 & kLo, w0 & kBoth, w1 & kLo, w1 & kBoth, b0, b1);
+          mma_16816(acc[2 * n + 1], y0 & kLo, y0, y1 & kLo, y1, b0, b1);
+          mma_16816(off, eight[n], 0u, eight[n], 0u, b0, b1);
+        }
+      }
+    }
+    copy_wait<0>();
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l_run[j] += __shfl_xor_sync(0xffffffffu, l_run[j], o);
+  }
+
+  // Calls put(column j, dim, four values) for the lane's share of O (not yet
+  // divided by l): head 2 t + j, dims dim .. dim + 3.
+  template <typename F>
+  __device__ __forceinline__ void each(const Sums& s, F&& put) const {
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float o8 = __shfl_sync(0xffffffffu, s.off[j], 8 * n + t);  // row 2 n
+        const float lo0 = s.acc[2 * n][j], lo1 = s.acc[2 * n + 1][j];
+        const float hi0 = (s.acc[2 * n][2 + j] - lo0) * 0.0625f, hi1 = (s.acc[2 * n + 1][2 + j] - lo1) * 0.0625f;
+        put(j, 32 * n + 4 * r,
+            make_float4((lo0 - o8) * kTwo24, (hi0 - o8) * kTwo24, (lo1 - o8) * kTwo24, (hi1 - o8) * kTwo24));
+      }
   }
 };
 
-// SHARES: the CTA's share of the list of all blocks; else one split of one row.
-template <bool CAP, bool SHARES>
-__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) decode_kernel(const Args a) {
+// Output row (sequence, head), dims d .. d + 3: o / l, or 0 without keys.
+__device__ __forceinline__ void store_out(const Args& a, size_t row, int d, float4 o, float l) {
+  const float i = l != 0.0f ? 1.0f / l : 0.0f;
+  const float4 v = make_float4(o.x * i, o.y * i, o.z * i, o.w * i);
+  if (a.out_bf16) {
+    const __nv_bfloat162 p[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + row * kD + d) =
+        *reinterpret_cast<const uint2*>(p);
+  } else {
+    *reinterpret_cast<float4*>(a.out + row * kD + d) = v;
+  }
+}
+
+// Counts one part of a row in; true for the last of n.  The caller's threads have
+// met at a barrier after their writes and meet at one before they read the parts.
+__device__ __forceinline__ bool arrive_last(unsigned* counter, int n) {
+  asm volatile("fence.acq_rel.gpu;\n" ::: "memory");
+  const bool last = atomicAdd(counter, 1u) == (unsigned)(n - 1);
+  if (last) *counter = 0u;  // ready for the next launch
+  asm volatile("fence.acq_rel.gpu;\n" ::: "memory");
+  return last;
+}
+
+// A running sum of parts (m, l, o): eight are loaded together, then added in order.
+struct Joined {
+  float m = kNone, l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  // at(p, m l, o): the loads of part p < n
+  template <typename F>
+  __device__ __forceinline__ void add(int n, F&& at) {
+    constexpr int kBatch = 8;
+    for (int p0 = 0; p0 < n; p0 += kBatch) {
+      float2 ml[kBatch];
+      float4 po[kBatch];
+#pragma unroll
+      for (int c = 0; c < kBatch; ++c) at(min(p0 + c, n - 1), ml[c], po[c]);
+      float top = m;
+#pragma unroll
+      for (int c = 0; c < kBatch; ++c) top = fmaxf(top, ml[c].x);
+      float f = ex2(m - top);
+      o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+      l *= f;
+      m = top;
+#pragma unroll
+      for (int c = 0; c < kBatch; ++c)
+        if (p0 + c < n) {
+          f = ex2(ml[c].x - m);
+          o = make_float4(o.x + f * po[c].x, o.y + f * po[c].y, o.z + f * po[c].z, o.w + f * po[c].w);
+          l += f * ml[c].y;
+        }
+    }
+  }
+};
+
+// ---- few rows: one CTA per split --------------------------------------------------
+template <bool CAP>
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) splits_kernel(const Args a) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float sm_m[kWarps][8];
   __shared__ float sm_l[kWarps][8];
-  __shared__ float cta_ml[8][2];
+  __shared__ __align__(8) float cta_ml[8][2];
   __shared__ int sm_last;
   __shared__ __align__(8) int sm_blk[kWarps][kBlkRing];
-  __shared__ int sm_end[SHARES ? kMaxStreamSeqs : 1];  // blocks of sequences 0..b (one kv head)
-  __shared__ int sm_sum[kWarps];
-
   if (!a.inputs_stable) pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = lane >> 2, t = lane & 3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int Hkv = a.num_kv_heads, group = a.group;
-  const int slices = SHARES ? 1 : (int)cg::this_cluster().num_blocks();
+  const int slices = (int)cg::this_cluster().num_blocks();
+  const int split = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
 
-  // ---- what this CTA walks ------------------------------------------------------
-  Share share = {};
-  int at = 0, end = 0, b = 0;  // SHARES: [at, end) of the list, Hkv rows per sequence
-  if (SHARES) {
-    // running sum of the sequences' blocks; an empty one counts as a block, so
-    // that a CTA writes its zeros
+  const int raw = a.seq_lens[b];
+  const Keys seq = keys_of(a, raw);
+  if (raw != seq.seq_len && split == 0 && g == 0 && threadIdx.x == 0) report(a.status, DOE_DEVICE_ERR_LENGTH);
+  const int nsplits = max(1, (seq.tiles + a.split_tiles - 1) / a.split_tiles);
+  const int part = split / slices, nparts = (nsplits + slices - 1) / slices;
+  if (part >= nparts) return;             // the whole cluster; a split past the last joins with nothing
+  if (nsplits == 1 && split != 0) return;  // nothing to join
+  const int tile_begin = split * a.split_tiles, tile_end = min(seq.tiles, tile_begin + a.split_tiles);
+  const int span = tile_end - tile_begin - warp;
+  const Stretch w = {b, g, seq.seq_len, seq.min_key, seq.origin + tile_begin + warp,
+                     span > 0 ? (span + kWarps - 1) / kWarps : 0, 0, nsplits == 1};
+  Walker<CAP, kWarps> walker(a, sm_blk[warp], ring + warp * kWarpBytes, lane);
+  // the first copies go out before the query work, and before griddepcontrol.wait
+  // when the caller vouches for the inputs
+  walker.start(w);
+  if (a.inputs_stable) pdl_wait();
+  pdl_trigger();
+  Sums sums;
+  walker.walk(w, sums);
+
+  // ---- join the warps: O staged in the ring's first slots ---------------------------
+  if (r == 0)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      sm_m[warp][2 * t + j] = sums.m[j];
+      sm_l[warp][2 * t + j] = sums.l[j];
+    }
+  float* my_o = reinterpret_cast<float*>(ring + warp * kWarpBytes);  // [8][128]
+  walker.each(sums, [&](int j, int d, const float4& v) {
+    *reinterpret_cast<float4*>(my_o + (2 * t + j) * kD + d) = v;
+  });
+  __syncthreads();
+  const size_t row = (size_t)b * Hkv + g, part_row = row * a.max_parts + part;
+  float* cta_o = reinterpret_cast<float*>(ring);  // [8][128], over the first warp's
+  for (int i = threadIdx.x; i < group * (kD / 4); i += kWarps * 32) {
+    const int h = i / (kD / 4), d = i % (kD / 4) * 4;
+    float M = kNone, L = 0.0f;
+    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int c = 0; c < kWarps; ++c) M = fmaxf(M, sm_m[c][h]);
+#pragma unroll
+    for (int c = 0; c < kWarps; ++c) {
+      const float f = ex2(sm_m[c][h] - M);
+      const float4 o = *reinterpret_cast<const float4*>(ring + c * kWarpBytes + (h * kD + d) * 4);
+      O = make_float4(O.x + f * o.x, O.y + f * o.y, O.z + f * o.z, O.w + f * o.w);
+      L += f * sm_l[c][h];
+    }
+    if (nsplits == 1) {
+      store_out(a, row * group + h, d, O, L);
+    } else {
+      float* ml = slices == 1 ? a.part_ml + (part_row * group + h) * 2 : cta_ml[h];
+      // over what only this thread has read
+      *reinterpret_cast<float4*>(slices == 1 ? a.part_o + (part_row * group + h) * kD + d : cta_o + h * kD + d) = O;
+      if (d == 0) {
+        ml[0] = M;
+        ml[1] = L;
+      }
+    }
+  }
+  if (nsplits == 1) return;
+
+  // ---- join the cluster: this CTA its slice of the dims -------------------------------
+  const int quads = kD / 4 / slices;
+  int rank = 0;
+  if (slices > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    rank = (int)cluster.block_rank();
+    cluster.sync();
+    for (int i = threadIdx.x; i < group * quads; i += kWarps * 32) {
+      const int h = i / quads, d = (rank * quads + i % quads) * 4;
+      Joined sum;
+      sum.add(slices, [&](int c, float2& ml, float4& o) {
+        ml = *reinterpret_cast<const float2*>(cluster.map_shared_rank(cta_ml[h], c));
+        o = *reinterpret_cast<const float4*>(cluster.map_shared_rank(cta_o, c) + h * kD + d);
+      });
+      if (nparts == 1) {
+        store_out(a, row * group + h, d, sum.o, sum.l);
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + (part_row * group + h) * kD + d) = sum.o;
+        if (i % quads == 0)
+          *reinterpret_cast<float2*>(a.part_ml + ((part_row * slices + rank) * group + h) * 2) =
+              make_float2(sum.m, sum.l);
+      }
+    }
+    cluster.sync();  // the others have read this CTA's part
+  }
+  if (nparts == 1) return;
+  // ---- the last part of a (row, slice) to finish stitches them, in key order ---------
+  __syncthreads();
+  if (threadIdx.x == 0) sm_last = arrive_last(&a.counters[row * slices + rank], nparts);
+  __syncthreads();
+  if (!sm_last) return;
+  for (int i = threadIdx.x; i < group * quads; i += kWarps * 32) {
+    const int h = i / quads, d = (rank * quads + i % quads) * 4;
+    Joined sum;
+    sum.add(nparts, [&](int p, float2& ml, float4& o) {
+      const size_t from = row * a.max_parts + p;
+      ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + (from * slices + rank) * group + h);
+      o = __ldcg(reinterpret_cast<const float4*>(a.part_o + (from * group + h) * kD + d));
+    });
+    store_out(a, row * group + h, d, sum.o, sum.l);
+  }
+}
+
+// ---- many rows: pieces of one list, a warp each -------------------------------------
+template <bool CAP>
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) pieces_kernel(const Args a) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(8) int sm_blk[kWarps][kBlkRing];
+  __shared__ int sm_end[kMaxListSeqs];  // entries of sequences 0..b
+  __shared__ int sm_len[kMaxListSeqs];
+  __shared__ int sm_sum[kWarps];
+  if (!a.inputs_stable) pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int Hkv = a.num_kv_heads, group = a.group;
+
+  // the list has the sequences one after another, each as kRowCost entries for
+  // its fixed cost and one per block (an empty one as if it had one, so that
+  // somebody writes its zeros)
+  {
     const int per = (a.num_seqs + kWarps * 32 - 1) / (kWarps * 32), b0 = threadIdx.x * per;
     int sum = 0;
     for (int i = b0; i < min(b0 + per, a.num_seqs); ++i) {
       const int raw = a.seq_lens[i];
       const Keys s = keys_of(a, raw);
       if (raw != s.seq_len && blockIdx.x == 0) report(a.status, DOE_DEVICE_ERR_LENGTH);
-      sum += max(1, s.tiles);
+      sum += kRowCost + max(1, s.tiles);
       sm_end[i] = sum;
+      sm_len[i] = raw;
     }
     int incl = sum;
 #pragma unroll
@@ -292,505 +818,177 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) decode_kernel(const A
     for (int w = 0; w < warp; ++w) before += sm_sum[w];
     for (int i = b0; i < min(b0 + per, a.num_seqs); ++i) sm_end[i] += before;
     __syncthreads();
-    const int total = sm_end[a.num_seqs - 1] * Hkv;  // below 2^31 (plan)
-    // at least two blocks per warp and share, unless there are more rows
-    const int shares = min((int)gridDim.x, max(total / (2 * kWarps), a.num_seqs * Hkv));
-    if ((int)blockIdx.x >= shares) return;
-    share.size = total / shares;
-    share.more = total - share.size * shares;
-    at = share.begin(blockIdx.x);
-    end = share.begin(blockIdx.x + 1);
-    int hi = a.num_seqs - 1;  // the first sequence that ends after `at`
-    while (b < hi) {
-      const int mid = (b + hi) >> 1;
-      if (sm_end[mid] * Hkv > at) hi = mid;
-      else b = mid + 1;
-    }
   }
-  for (bool first_row = true;; first_row = false) {
-  int g, tile_begin, tile_end, part = 0, nparts;
-  Keys seq;
-  size_t row;
-  int row_at = 0;
-  if (SHARES) {
-    if (at >= end) break;
-    if (!first_row) {
-      __syncthreads();  // the last row's staging and statistics have been read
-      if (at >= sm_end[b] * Hkv) ++b;
-    }
-    const int seq_at = b ? sm_end[b - 1] : 0, size = sm_end[b] - seq_at;
-    g = (at - seq_at * Hkv) / size;
-    row_at = seq_at * Hkv + g * size;
-    seq = keys_of(a, a.seq_lens[b]);
-    tile_begin = at - row_at;
-    tile_end = min(end - row_at, size);
-    at = row_at + tile_end;
-    nparts = tile_begin == 0 && tile_end == size ? 1 : 2;  // the exact number where it matters
-    tile_end = min(tile_end, seq.tiles);
-  } else {
-    g = blockIdx.y;
-    b = blockIdx.z;
-    const int raw = a.seq_lens[b], split = blockIdx.x;
-    seq = keys_of(a, raw);
-    if (raw != seq.seq_len && split == 0 && g == 0 && threadIdx.x == 0) report(a.status, DOE_DEVICE_ERR_LENGTH);
-    const int nsplits = max(1, (seq.tiles + a.split_tiles - 1) / a.split_tiles);
-    part = split / slices;
-    nparts = nsplits == 1 ? 0 : (nsplits + slices - 1) / slices;  // 0: nothing to join, not even in the cluster
-    if (split >= max(nparts, 1) * slices) return;  // the whole cluster; a split past the last joins with nothing
-    if (nparts == 0 && split != 0) return;
-    tile_begin = split * a.split_tiles;
-    tile_end = min(seq.tiles, tile_begin + a.split_tiles);
-  }
-  row = (size_t)b * Hkv + g;
-  const int seq_len = seq.seq_len, min_key = seq.min_key;
-  const int32_t* table = a.block_table + (size_t)b * a.max_pages;
+  // An item is a piece of one kv head, the head fastest: the warps of neighbouring
+  // items read neighbouring blocks of the same pages at about the same time
+  // (pieces of one head after another took 118 us where this takes 86).
+  const int total = sm_end[a.num_seqs - 1];  // below 2^29 (plan)
+  const int most = (int)gridDim.x * kWarps / Hkv;                   // pieces (at least one: plan)
+  const int size = max(kMinPiece, (total + most - 1) / most);        // of a piece
+  const int items = (total + size - 1) / size * Hkv;
+  int item = blockIdx.x * kWarps + warp;
+  if (item >= items) return;
 
-  // this warp's blocks: first + kWarps * k, k < nt, as block numbers in the pools,
-  // looked up 96 ahead.  kDead: past the walk, or on a page outside the pool;
-  // kMasked is set on a block with dead keys (the window's first, the sequence's
-  // last)
-  const int first = seq.origin + tile_begin + warp;
-  const int span = tile_end - tile_begin - warp;
-  const int nt = span > 0 ? (span + kWarps - 1) / kWarps : 0;
-  auto block_number = [&](int i) {
-    if (i >= nt) return kDead;
-    const int tile = first + kWarps * i;
-    const int pidx = a.tile_shift >= 0 ? tile >> a.tile_shift : tile / a.tiles_per_page;
-    const int page = table[pidx];
-    if ((unsigned)page < (unsigned)a.num_pages)
-      return (page * Hkv + g) * a.tiles_per_page + (tile - pidx * a.tiles_per_page) +
-             (tile * 16 < min_key || tile * 16 + 16 > seq_len ? kMasked : 0);
-    report(a.status, DOE_DEVICE_ERR_PAGE);
-    return kDead;
+  int at = 0, end = 0, b = 0, g = 0;  // what is left of the piece, its sequence and head
+  auto seq_size = [&](int s) { return sm_end[s] - (s ? sm_end[s - 1] : 0); };
+  auto seq_of = [&](int x, int lo) {  // the sequence that holds entry x, at least lo
+    int hi = a.num_seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sm_end[mid] > x) hi = mid;
+      else lo = mid + 1;
+    }
+    return lo;
   };
-#pragma unroll
-  for (int i = 0; i < kBlkRing - 32; i += 32) sm_blk[warp][i + lane] = i < nt + kStages ? block_number(i + lane) : kDead;
-  int ahead = nt > kBlkRing - 32 ? block_number(kBlkRing - 32 + lane) : kDead;
-  __syncwarp();
-
-  const uint32_t wbase = smem_addr(ring) + warp * kWarpBytes;
-  const uint8_t* k_lane = a.k_pool + 16 * lane;
-  const uint8_t* v_lane = a.v_pool + 16 * lane;
-  // lanes 0-7 copy the K scales, 8-15 the V scales
-  const uint8_t* s_lane = (lane < 8 ? k_lane : v_lane - 128) + kI4Codes;
-  const uint32_t lane_dst = wbase + 16 * lane;
-  const uint32_t s_dst = lane_dst + kI4Codes + (lane < 8 ? 0 : kI4Block - 128);
-  // Fills the slot at byte `slot` of the ring with block number blk, a dead one
-  // with zeros
-  auto issue = [&](int blk, uint32_t slot) {
-    const uint32_t size = blk == kDead ? 0u : 16u;
-    const size_t off = (size_t)(blk == kDead ? 0u : (uint32_t)blk & ~(uint32_t)kMasked) * kI4Block;
-    copy16(lane_dst + slot, k_lane + off, size);
-    copy16(lane_dst + slot + 512, k_lane + off + 512, size);
-    copy16(lane_dst + slot + kI4Block, v_lane + off, size);
-    copy16(lane_dst + slot + kI4Block + 512, v_lane + off + 512, size);
-    if (lane < 16) copy16(s_dst + slot, s_lane + off, size);
+  auto open_piece = [&]() {
+    const int piece = item / Hkv;
+    g = item - piece * Hkv;
+    at = piece * size;
+    end = min(total, at + size);
+    b = seq_of(at, b);
+    // an end inside a sequence's fixed cost leaves that sequence to the next piece
+    const int s = seq_of(end - 1, b), over = end - (sm_end[s] - seq_size(s));
+    if (over <= kRowCost) end -= over;
+  };
+  auto take = [&]() {  // the piece's next stretch
+    if (at >= sm_end[b]) ++b;
+    const int row_size = seq_size(b), row_at = sm_end[b] - row_size;
+    const Keys seq = keys_of(a, sm_len[b]);
+    const int tile_begin = max(0, at - row_at - kRowCost);
+    at = min(end, row_at + row_size);
+    const int tile_end = min(at - row_at - kRowCost, seq.tiles);
+    return Stretch{b, g, seq.seq_len, seq.min_key, seq.origin + tile_begin, max(0, tile_end - tile_begin), row_at,
+                   tile_begin == 0 && at == row_at + row_size};
   };
 
-  // first copies before the query work (and before griddepcontrol.wait when the
-  // caller vouches for the inputs); the block that receives the new row, the walk's
-  // last of the warp that appends it, waits for the append
-  const bool append_pending =
-      a.new_k != nullptr && seq_len > 0 && nt > 0 && first + kWarps * (nt - 1) == (seq_len - 1) >> 4;
-  const int early = min(kStages - kStep, append_pending ? nt - 1 : nt);
-  for (int k = 0; k < early; ++k) {
-    issue(sm_blk[warp][k], k * kSlot);
-    if (k % kStep == kStep - 1) copy_commit();
-  }
-  if (first_row) {
-    if (a.inputs_stable) pdl_wait();
-    pdl_trigger();
-  }
-  AppendRow app;
-  if (append_pending) app.load(a, b, g, seq_len - 1, table, lane);
+  Walker<CAP, 1> walker(a, sm_blk[warp], ring + warp * kWarpBytes, lane);
+  open_piece();
+  Stretch cur = take();
+  walker.start(cur);
+  if (a.inputs_stable) pdl_wait();
+  pdl_trigger();
+  int cut_row[2] = {-1, -1}, cut_at[2] = {0, 0};   // rows that the piece holds a part of
+  bool first = true;                               // the piece's first stretch
+  while (true) {
+    Sums sums;
+    walker.walk(cur, sums);
 
-  // ---- Q as the B operand: lane (r = head, t) holds dims 32 grp + 8 t + 0..7,
-  // word i of each run = dims (2 i, 2 i + 1) = the K word's nibbles i and i + 4
-  uint32_t qb[4][4];
-  float qinit[4][4];  // -8 sum_group q of heads 2 t, 2 t + 1 (times 2^-24), for both token rows
-  {
-    const __half* qrow = a.q + ((size_t)b * a.num_heads + (size_t)g * group + r) * kD;
-    const bool live = r < group;
-    uint4 qv[4];
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-      qv[n] = live ? *reinterpret_cast<const uint4*>(qrow + 32 * n + 8 * t) : make_uint4(0, 0, 0, 0);
-    if (a.freq_cis != nullptr && live && seq_len > 0) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        float rc[8], rsn[8];
-        rope_table<4>(a.freq_cis, a.rope_positions, kD / 2, (long long)seq_len - 1, 32 * n + 8 * t, a.status,
-                      tile_begin == 0 && g == 0 && lane == 0 && warp == 0, rc, rsn);
-        const uint4 lo = qv[n], hi = qv[n + 2];
-        rope_rotate<4>(reinterpret_cast<const uint32_t*>(&lo), reinterpret_cast<const uint32_t*>(&hi), true, rc, rsn,
-                       reinterpret_cast<uint32_t*>(&qv[n]));
-        rope_rotate<4>(reinterpret_cast<const uint32_t*>(&hi), reinterpret_cast<const uint32_t*>(&lo), false, rc, rsn,
-                       reinterpret_cast<uint32_t*>(&qv[n + 2]));
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      float qs = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w = word(qv[n], i) ^ (!CAP && a.scale < 0.0f ? 0x80008000u : 0u);
-        float mult = 1.0f;
-        if (i & 1) {  // meets codes read as n 2^-20; q 2^-4 loses bits only below |q| = 2^-10, 2^-21 absolute
-          w = hmul2(w, 0x2c002c00u);
-          mult = 16.0f;
-        }
-        qb[n][i] = w;
-        const float2 f = f2(w);
-        qs += mult * (f.x + f.y);
-      }
-      qs += __shfl_xor_sync(0xffffffffu, qs, 1);
-      qs += __shfl_xor_sync(0xffffffffu, qs, 2);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        qinit[n][j] = -8.0f / kTwo24 * __shfl_sync(0xffffffffu, qs, (2 * t + j) * 4);
-        qinit[n][2 + j] = qinit[n][j];
-        asm("" : "+f"(qinit[n][2 + j]));  // a quad of registers of its own: the MMA takes it without copies
-      }
-    }
-  }
-
-  // heads 2 t and 2 t + 1 of this lane's accumulator columns
-  float m_ref[2] = {kNone, kNone}, l_run[2] = {0.0f, 0.0f};
-  int v_exp = -3;                // every V scale seen is at most 2^v_exp (or infinite)
-  uint32_t v_lim = 0x30003000u;  // 2^v_exp as an f16 pair
-  float m_lim[2] = {kNone, kNone};  // x of a score 2^8 over its maximum
-  float acc[8][4], off[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-
-  if (append_pending) app.store(a, g, lane);
-  for (int k = early; k < kStages - kStep; ++k) {
-    issue(sm_blk[warp][k], k * kSlot);
-    if (k % kStep == kStep - 1) copy_commit();
-  }
-
-  // x is the softcapped score in the log2 domain (CAP) or the bare product, which
-  // c > 0 takes there: the sign of the scale is in Q, and a scale of 0 becomes
-  // tiny so that the -inf of a dead key stays -inf
-  uint32_t eight[4];  // A operand of the -8: rows 2 n, 2 n + 1 take group n
-#pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    eight[n] = (r >> 1) == n ? 0x00080008u : 0u;
-    asm("" : "+r"(eight[n]));
-  }
-  const float to_cap = a.scale * kTwo24 / a.softcap, cap_log2 = a.softcap * kLog2e;  // CAP only
-  const float c_log2 = CAP ? 1.0f : fmaxf(fabsf(a.scale) * (kLog2e * kTwo24), 1e-30f), inv_c = 1.0f / c_log2;
-  uint32_t slot = 0, refill = (kStages - kStep) * kSlot;  // byte offsets in the ring
-  for (int k = 0; k < nt; k += kStep) {
-    if ((k & 31) == 0 && k != 0) {
-      sm_blk[warp][(k + kBlkRing - 64 + lane) & (kBlkRing - 1)] = ahead;
-      ahead = block_number(k + kBlkRing - 32 + lane);
-    }
-    __syncwarp();  // also: the slots refilled here were read in the last step
-    int blk[kStep];
-#pragma unroll
-    for (int u = 0; u < kStep; ++u) {
-      blk[u] = sm_blk[warp][(k + u) & (kBlkRing - 1)];
-      issue(sm_blk[warp][(k + u + kStages - kStep) & (kBlkRing - 1)], refill + u * kSlot);
-    }
-    copy_commit();
-    copy_wait<kStages / kStep - 1>();
-    __syncwarp();
-    float x[kStep][4];
-    uint4 vw[kStep][2], vs[kStep][2];
-    uint32_t vmax = v_lim;  // scales are not negative, so they order as 16-bit integers
-#pragma unroll
-    for (int u = 0; u < kStep; ++u) {
-      const uint32_t kb = wbase + slot + u * kSlot, vb = kb + kI4Block;
-      uint4 kw[2];
-      uint2 ks[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        kw[h] = lds128(kb + 512 * h + 16 * lane);     // token r + 8 h
-        ks[h] = lds64(kb + kI4Codes + 64 * h + 8 * r);
-        vw[u][h] = lds128(vb + 512 * h + 16 * lane);  // tokens 2 t, 2 t + 1 (+ 8 h)
-        vs[u][h] = lds128(vb + kI4Codes + 64 * h + 16 * t);
-      }
-      // ---- S = K Q^T: rows token r / r + 8, columns heads 2 t, 2 t + 1 ---------
-      float s[4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const uint32_t w0 = word(kw[0], n), w1 = word(kw[1], n);
-        const uint32_t y0 = w0 >> 8, y1 = w1 >> 8;
-        float c[4];
-        mma_from(c, w0 & kLo, w1 & kLo, y0 & kLo, y1 & kLo, qb[n][0], qb[n][2], qinit[n][0], qinit[n][1], qinit[n][2],
-                 qinit[n][3]);
-        mma_16816(c, w0 & kHi, w1 & kHi, y0 & kHi, y1 & kHi, qb[n][1], qb[n][3]);
-        const float2 sa = f2(n < 2 ? ks[0].x : ks[0].y), sb = f2(n < 2 ? ks[1].x : ks[1].y);
-        const float s0 = (n & 1) ? sa.y : sa.x, s1 = (n & 1) ? sb.y : sb.x;
-        s[0] = n ? fmaf(s0, c[0], s[0]) : s0 * c[0];
-        s[1] = n ? fmaf(s0, c[1], s[1]) : s0 * c[1];
-        s[2] = n ? fmaf(s1, c[2], s[2]) : s1 * c[2];
-        s[3] = n ? fmaf(s1, c[3], s[3]) : s1 * c[3];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[u][i] = CAP ? cap_log2 * tanhf(s[i] * to_cap) : s[i];
-    }
-    refill = slot;
-    slot = slot == (kStages - kStep) * kSlot ? 0 : slot + kStep * kSlot;
-    // dead keys: what stands there (codes, scales) may be anything
-    if ((blk[0] | blk[kStep - 1]) < 0) {
-#pragma unroll
-      for (int u = 0; u < kStep; ++u) {
-        const int pos0 = (first + kWarps * (k + u)) << 4;
-        const int lo = min_key, hi = blk[u] == kDead ? 0 : seq_len;
-        if (pos0 + r < lo || pos0 + r >= hi) x[u][0] = x[u][1] = -INFINITY;
-        if (pos0 + r + 8 < lo || pos0 + r + 8 >= hi) x[u][2] = x[u][3] = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int key = pos0 + 2 * t + 8 * h;
-          const uint32_t keep = (key >= lo && key < hi ? 0x0000ffffu : 0u) |
-                                (key + 1 >= lo && key + 1 < hi ? 0xffff0000u : 0u);
-          vs[u][h].x &= keep; vs[u][h].y &= keep; vs[u][h].z &= keep; vs[u][h].w &= keep;
-        }
-      }
+    // the next stretch's first copies go out before this one's results
+    const Stretch done = cur;
+    const bool more = at < end;
+    if (more) {
+      cur = take();
+      walker.start(cur);
     }
 
-    // ---- the reference moves when a score or a V scale outgrows it -------------
-    float mx[2] = {fmaxf(x[0][0], x[0][2]), fmaxf(x[0][1], x[0][3])};
-#pragma unroll
-    for (int u = 0; u < kStep; ++u) {
-      if (u) {
-        mx[0] = fmaxf(mx[0], fmaxf(x[u][0], x[u][2]));
-        mx[1] = fmaxf(mx[1], fmaxf(x[u][1], x[u][3]));
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        vmax = __vimax3_u16x2(__vimax3_u16x2(vmax, vs[u][h].x, vs[u][h].y), vs[u][h].z, vs[u][h].w);
-    }
-    const bool grow = mx[0] > m_lim[0] || mx[1] > m_lim[1] || vmax != v_lim;
-    if (__any_sync(0xffffffffu, grow)) {
-      const float2 vf = f2(vmax);  // at least 2^v_exp
-      const float vm = warp_max(fmaxf(vf.x, vf.y));
-      int e = v_exp;
-      if (vm > f2(v_lim).x) e = min(15, (int)((__float_as_uint(vm) >> 23) & 255) - 126);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], o));
-        // reference = score maximum + exponent of the V scales - 4: p <= 2^15
-        // and s p <= 2^12 while a score may still outgrow the maximum by 2^8
-        const float base = m_ref[j] - (float)(v_exp - 4);
-        const float top = fmaxf(base, mx[j] * c_log2), m_new = top + (float)(e - 4);
-        const float corr = ex2(m_ref[j] - m_new);
-        m_ref[j] = m_new;
-        m_lim[j] = (top + 8.0f) * inv_c;
-        l_run[j] *= corr;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          acc[i][j] *= corr;
-          acc[i][2 + j] *= corr;
-        }
-        off[j] *= corr;
-      }
-      v_exp = e;
-      v_lim = (uint32_t)(e + 15) * 0x04000400u;
-    }
-
-#pragma unroll
-    for (int u = 0; u < kStep; ++u) {
-      float p[4];
-      p[0] = ex2(fmaf(x[u][0], c_log2, -m_ref[0]));
-      p[1] = ex2(fmaf(x[u][1], c_log2, -m_ref[1]));
-      p[2] = ex2(fmaf(x[u][2], c_log2, -m_ref[0]));
-      p[3] = ex2(fmaf(x[u][3], c_log2, -m_ref[1]));
-      l_run[0] += p[0] + p[2];
-      l_run[1] += p[1] + p[3];
-      const uint32_t p0 = transpose8x8(pack_half2(p[0], p[1]));  // head r, tokens 2 t, 2 t + 1
-      const uint32_t p1 = transpose8x8(pack_half2(p[2], p[3]));  // tokens + 8
-
-      // ---- O^T += V^T (s P)^T: m-block 2 n + j = dims 32 n + 4 row' + {2 j, 2 j + 1}
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const uint32_t b0 = hmul2(p0, word(vs[u][0], n)), b1 = hmul2(p1, word(vs[u][1], n));
-        const uint32_t w0 = word(vw[u][0], n), w1 = word(vw[u][1], n);
-        const uint32_t y0 = prmt(w0, 0u, 0x4341u), y1 = prmt(w1, 0u, 0x4341u);  // bytes 1 and 3
-        mma_16816(acc[2 * n], w0 & kLo, w0 & kBoth, w1 & kLo, w1 & kBoth, b0, b1);
-        mma_16816(acc[2 * n + 1], y0 & kLo, y0, y1 & kLo, y1, b0, b1);
-        mma_16816(off, eight[n], 0u, eight[n], 0u, b0, b1);
-      }
-    }
-  }
-
-  // ---- join the warps of this split (O staged in this warp's own ring) ---------
-  copy_wait<0>();
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) l_run[j] += __shfl_xor_sync(0xffffffffu, l_run[j], o);
-    if (r == 0) {
-      sm_m[warp][2 * t + j] = m_ref[j];
-      sm_l[warp][2 * t + j] = l_run[j];
-    }
-  }
-  float* my_o = reinterpret_cast<float*>(ring + warp * kWarpBytes);  // [8][128]
-#pragma unroll
-  for (int n = 0; n < 4; ++n)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float o8 = __shfl_sync(0xffffffffu, off[j], 8 * n + t);  // row 2 n
-      const float lo0 = acc[2 * n][j], lo1 = acc[2 * n + 1][j];
-      const float hi0 = (acc[2 * n][2 + j] - lo0) * 0.0625f, hi1 = (acc[2 * n + 1][2 + j] - lo1) * 0.0625f;
-      const float4 v = make_float4((lo0 - o8) * kTwo24, (hi0 - o8) * kTwo24, (lo1 - o8) * kTwo24, (hi1 - o8) * kTwo24);
-      *reinterpret_cast<float4*>(my_o + (2 * t + j) * kD + 32 * n + 4 * r) = v;
-    }
-  __syncthreads();
-
-  const int dim = threadIdx.x;  // 128 threads == head dim
-  const size_t out_row = ((size_t)b * a.num_heads + (size_t)g * group) * kD;
-  auto store = [&](int h, int d, float o, float l) {
-    const float v = l != 0.0f ? o / l : 0.0f;
-    if (a.out_bf16)
-      reinterpret_cast<__nv_bfloat16*>(a.out)[out_row + (size_t)h * kD + d] = __float2bfloat16_rn(v);
-    else
-      a.out[out_row + (size_t)h * kD + d] = v;
-  };
-  const bool whole = SHARES ? nparts == 1 : nparts == 0;
-  // where this CTA's partial row goes
-  const size_t slot_at = SHARES ? 2 * (size_t)blockIdx.x + (first_row ? 0 : 1) : row * a.max_parts + part;
-  float* cta_o = reinterpret_cast<float*>(ring);  // [8][128], over the first warp's
-  for (int h = 0; h < group; ++h) {
-    float M = kNone, O = 0.0f, L = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][h]);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2(sm_m[w][h] - M);
-      O += f * reinterpret_cast<const float*>(ring + w * kWarpBytes)[h * kD + dim];
-      L += f * sm_l[w][h];
-    }
-    if (whole) {
-      store(h, dim, O, L);
-    } else if (slices == 1) {
-      a.part_o[(slot_at * group + h) * kD + dim] = O;
-      if (dim == 0) {
-        a.part_ml[(slot_at * group + h) * 2] = M;
-        a.part_ml[(slot_at * group + h) * 2 + 1] = L;
-      }
+    const size_t row = (size_t)done.b * Hkv + done.g;
+    if (done.whole) {
+      walker.each(sums, [&](int j, int d, const float4& v) {
+        if (2 * t + j < group) store_out(a, row * group + 2 * t + j, d, v, sums.l[j]);
+      });
     } else {
-      cta_o[h * kD + dim] = O;  // read only by this thread before
-      if (dim == 0) {
-        cta_ml[h][0] = M;
-        cta_ml[h][1] = L;
+      const size_t part = 2 * (size_t)item + (first ? 0 : 1);
+      walker.each(sums, [&](int j, int d, const float4& v) {
+        if (2 * t + j < group) *reinterpret_cast<float4*>(a.part_o + (part * group + 2 * t + j) * kD + d) = v;
+      });
+      if (r == 0)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (2 * t + j < group)
+            *reinterpret_cast<float2*>(a.part_ml + (part * group + 2 * t + j) * 2) = make_float2(sums.m[j], sums.l[j]);
+      if (first) {
+        cut_row[0] = (int)row;
+        cut_at[0] = done.row_at;
+      } else {
+        cut_row[1] = (int)row;
+        cut_at[1] = done.row_at;
       }
     }
-  }
-  if (whole) {
-    if (SHARES) continue;
-    return;
+    first = false;
+    if (!more) break;
   }
 
-  // ---- the splits of a cluster: this CTA joins its slice of the dims ------------
-  int rank = 0;
-  const int width = kD / slices;
-  if (!SHARES && slices > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
-    rank = (int)cluster.block_rank();
-    cluster.sync();
-    for (int i = threadIdx.x; i < group * width; i += kWarps * 32) {
-      const int h = i / width, d = rank * width + i % width;
-      float M = kNone, O = 0.0f, L = 0.0f;
-      float m[8], o[8], l[8];
+  // ---- the last part of a row to finish stitches them, in key order ------------------
+  if (cut_row[0] < 0 && cut_row[1] < 0) return;
+  __syncwarp();
+  const int e = lane & 1;  // lanes 0 and 1 take a row each
+  const int my_row = cut_row[e], my_at = cut_at[e];
+  int c0 = 0, n = 0, last = 0;
+  if (my_row >= 0) {
+    c0 = (my_at + kRowCost) / size;
+    n = (my_at + seq_size(my_row / Hkv) - 1) / size - c0 + 1;
+    if (lane < 2) last = arrive_last(&a.counters[my_row], n);
+  }
+  __syncwarp();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    if (!__shfl_sync(0xffffffffu, last, i)) continue;
+    const int from0 = __shfl_sync(0xffffffffu, c0, i), parts = __shfl_sync(0xffffffffu, n, i);
+    const int row = cut_row[i];
+    // in its first piece, a row that another one precedes is the second part
+    const int second = from0 * size < cut_at[i] ? 1 : 0;
+    auto part_at = [&](int p, int h) {
+      return (2 * ((size_t)(from0 + p) * Hkv + g) + (p == 0 ? second : 0)) * group + h;
+    };
+    for (int h0 = 0; h0 < group; h0 += 4) {  // four heads together: one after another took 16 % more at 30 parts
+      float M[4], L[4];
+      float4 O[4];
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (c < slices) {
-          const float* ml = cluster.map_shared_rank(&cta_ml[h][0], c);
-          m[c] = ml[0];
-          l[c] = ml[1];
-          o[c] = cluster.map_shared_rank(cta_o, c)[h * kD + d];
-          M = fmaxf(M, m[c]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        M[j] = kNone;
+        L[j] = 0.0f;
+        O[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+      for (int p0 = 0; p0 < parts; p0 += 32) {  // lane p weighs part p0 + p
+        float weight[4];
+        float2 ml[4];
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (c < slices) {
-          const float f = ex2(m[c] - M);
-          O += f * o[c];
-          L += f * l[c];
+        for (int j = 0; j < 4; ++j)
+          ml[j] = p0 + lane < parts ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) +
+                                             part_at(p0 + lane, min(h0 + j, group - 1)))
+                                    : make_float2(kNone, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float top = fmaxf(M[j], warp_max(ml[j].x)), f = ex2(M[j] - top);
+          weight[j] = ex2(ml[j].x - top);
+          L[j] = L[j] * f + warp_sum(weight[j] * ml[j].y);
+          O[j] = make_float4(O[j].x * f, O[j].y * f, O[j].z * f, O[j].w * f);
+          M[j] = top;
         }
-      if (nparts == 1) {
-        store(h, d, O, L);
-      } else {
-        a.part_o[(slot_at * group + h) * kD + d] = O;
-        if (i % width == 0) {
-          float* ml = a.part_ml + ((slot_at * slices + rank) * group + h) * 2;
-          ml[0] = M;
-          ml[1] = L;
+        constexpr int kBatch = 6;  // parts whose loads are in flight together
+        const int some = min(32, parts - p0);
+        for (int q = 0; q < some; q += kBatch) {
+          float4 o[kBatch][4];
+#pragma unroll
+          for (int c = 0; c < kBatch; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              o[c][j] = __ldcg(reinterpret_cast<const float4*>(
+                  a.part_o + part_at(p0 + min(q + c, some - 1), min(h0 + j, group - 1)) * kD + 4 * lane));
+#pragma unroll
+          for (int c = 0; c < kBatch; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float w = __shfl_sync(0xffffffffu, weight[j], (q + c) & 31);
+              if (q + c < some)
+                O[j] = make_float4(O[j].x + w * o[c][j].x, O[j].y + w * o[c][j].y, O[j].z + w * o[c][j].z,
+                                   O[j].w + w * o[c][j].w);
+            }
         }
       }
-    }
-    cluster.sync();  // the others have read this CTA's partials
-    if (nparts == 1) return;
-  }
-  // ---- the last part of (b, g, slice) to finish stitches them, in order --------
-  int c0 = 0;       // SHARES: the CTA that holds the row's first block,
-  bool c0_second = false;  // as the second part that it writes
-  if (SHARES) {
-    const int size = sm_end[b] - (b ? sm_end[b - 1] : 0);
-    c0 = share.owner(row_at);
-    nparts = share.owner(row_at + size - 1) - c0 + 1;
-    c0_second = share.begin(c0) < row_at;
-  }
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    unsigned* counter = &a.counters[row * slices + rank];
-    sm_last = atomicAdd(counter, 1u) == (unsigned)(nparts - 1);
-    if (sm_last) *counter = 0u;  // ready for the next launch
-  }
-  __syncthreads();
-  if (sm_last) {
-    __threadfence();
-    for (int i = threadIdx.x; i < group * width; i += kWarps * 32) {
-      const int h = i / width, d = rank * width + i % width;
-      float M = kNone, O = 0.0f, L = 0.0f;
-      // a running reference, so that the loads of several parts are in flight
-      constexpr int kBatch = 8;
-      for (int p0 = 0; p0 < nparts; p0 += kBatch) {
-        float2 ml[kBatch];
-        float o[kBatch];
 #pragma unroll
-        for (int c = 0; c < kBatch; ++c) {
-          const int p = min(p0 + c, nparts - 1);
-          const size_t from =
-              SHARES ? 2 * (size_t)(c0 + p) + (p == 0 && c0_second ? 1 : 0) : row * a.max_parts + p;
-          ml[c] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + (from * slices + rank) * group + h);
-          o[c] = __ldcg(a.part_o + (from * group + h) * kD + d);
-        }
-        float m = M;
-#pragma unroll
-        for (int c = 0; c < kBatch; ++c) m = fmaxf(m, ml[c].x);
-        const float f0 = ex2(M - m);
-        O *= f0;
-        L *= f0;
-        M = m;
-#pragma unroll
-        for (int c = 0; c < kBatch; ++c)
-          if (p0 + c < nparts) {
-            const float f = ex2(ml[c].x - M);
-            O += f * o[c];
-            L += f * ml[c].y;
-          }
-      }
-      store(h, d, O, L);
+      for (int j = 0; j < 4; ++j)
+        if (h0 + j < group) store_out(a, (size_t)row * group + h0 + j, 4 * lane, O[j], L[j]);
     }
   }
-  if (!SHARES) return;
-  }  // rows of the share
 }
 
-template <bool CAP, bool SHARES>
-int launch_one(const Args& a, dim3 grid, unsigned slices, cudaStream_t st) {
-  static std::atomic<bool> attr[kMaxDevices];
-  const int rc = once_per_device(attr, [] {
-    return cuda_status(
-        cudaFuncSetAttribute(decode_kernel<CAP, SHARES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
-        "cudaFuncSetAttribute(paged_decode_int4)");
+template <typename Kernel>
+int launch_one(Kernel kernel, std::atomic<bool> (&attr)[kMaxDevices], const Args& a, dim3 grid, unsigned slices,
+               cudaStream_t st) {
+  const int rc = once_per_device(attr, [&] {
+    return cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
+                       "cudaFuncSetAttribute(paged_decode_int4)");
   });
   if (rc != DOE_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -807,46 +1005,60 @@ int launch_one(const Args& a, dim3 grid, unsigned slices, cudaStream_t st) {
   at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = slices > 1 ? 2 : 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, decode_kernel<CAP, SHARES>, a), "paged_decode_int4");
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, a), "paged_decode_int4");
+}
+
+template <bool CAP>
+int launch_cap(const Args& a, bool list, dim3 grid, unsigned slices, cudaStream_t st) {
+  static std::atomic<bool> attr[2][kMaxDevices];
+  return list ? launch_one(pieces_kernel<CAP>, attr[0], a, grid, slices, st)
+              : launch_one(splits_kernel<CAP>, attr[1], a, grid, slices, st);
 }
 
 // How a launch is cut, and the sizes that follow.
 struct Plan {
-  bool shares;                     // even shares of all rows' blocks over `grid` CTAs
-  uint64_t split_tiles, slices;    // else: blocks per split, splits per cluster
-  uint64_t max_parts, grid;        // parts per row, CTAs (per row when not shares)
-  uint64_t slots;                  // partial rows in the workspace
+  bool list;                     // pieces of one list; else splits
+  uint64_t split_tiles, slices;  // splits: blocks per split, splits per cluster
+  uint64_t max_parts, grid;      // splits: parts per row; CTAs (per row)
+  uint64_t slots;                // parts in the workspace (whatever the window, which its size query lacks)
 };
 
-// Even shares while a row is cut into a few parts at most, which its last CTA
-// stitches alone.  With fewer rows than that each row gets its own splits, so
-// many that there are about two CTAs per SM, joined in clusters.  A given
-// split_pages asks for splits of that length; they serve more than
-// kMaxStreamSeqs sequences too.
-Plan plan(uint64_t num_seqs, uint64_t kv_heads, uint64_t max_tiles, uint64_t tiles_per_page, uint64_t split_pages) {
+// `tiles`: the most blocks of a row that can be read (its block-table row, or the
+// window).  Short rows, enough of them to fill the SMs: one CTA each, nothing to
+// join.  Else the list, while a row is cut into about a dozen parts at most, which
+// one warp stitches.  With fewer rows each gets its own splits, as many as CTAs
+// are resident.  A given split_pages asks for splits of that length; they serve
+// more than kMaxListSeqs sequences too.
+Plan plan(uint64_t num_seqs, uint64_t kv_heads, uint64_t max_tiles, uint64_t tiles_per_page, uint64_t split_pages,
+          uint64_t window) {
   Plan p = {};
-  const uint64_t rows = num_seqs * kv_heads, ctas = (uint64_t)num_sms() * kCtasPerSm;
-  p.slices = 1;
-  if (split_pages == 0 && num_seqs <= kMaxStreamSeqs && rows * 16 >= ctas && rows * max_tiles <= 0x7fffffffull) {
-    p.shares = true;
-    p.grid = ctas * (getenv("I4M") ? atoi(getenv("I4M")) : 1);
-    p.max_parts = 2;
-    p.slots = 2 * p.grid;
-    return p;
-  }
+  const uint64_t rows = num_seqs * kv_heads, sms = (uint64_t)num_sms(), ctas = sms * kCtasPerSm;
+  const uint64_t tiles = window != 0 && window / 16 + 2 < max_tiles ? window / 16 + 2 : max_tiles;
   uint64_t t = split_pages * tiles_per_page;
-  if (t == 0) {
-    const uint64_t fill = (2 * (uint64_t)num_sms() + rows - 1) / rows;
-    t = (max_tiles + fill - 1) / fill;
-    if (t < 4) t = 4;
+  if (t == 0 && num_seqs <= kMaxListSeqs && rows * 14 >= ctas * kWarps && kv_heads <= ctas * kWarps &&
+      num_seqs * (max_tiles + kRowCost) <= 0x1fffffffull) {
+    p.slots = 2 * ctas * kWarps;
+    if (rows < sms || tiles > kShortRow) {
+      p.list = true;
+      p.slices = 1;
+      p.max_parts = 2;
+      p.grid = ctas;
+      return p;
+    }
+    t = tiles;
+  } else if (t == 0) {
+    const uint64_t fill = (2 * sms + rows - 1) / rows;
+    p.slots = rows * fill;
+    t = rows >= sms && tiles <= kShortRow ? tiles : (tiles + fill - 1) / fill;
+    if (t < 8) t = 8;
+  } else {
+    p.slots = rows * ((max_tiles + t - 1) / t);
   }
-  if (t > max_tiles) t = max_tiles;
-  p.split_tiles = t;
-  const uint64_t splits = (max_tiles + t - 1) / t;
+  p.split_tiles = t < tiles ? t : tiles;
+  const uint64_t splits = (tiles + p.split_tiles - 1) / p.split_tiles;
   p.slices = splits > 16 ? 8 : 1;
   p.max_parts = (splits + p.slices - 1) / p.slices;
   p.grid = p.max_parts * p.slices;
-  p.slots = rows * p.max_parts;
   return p;
 }
 
@@ -861,10 +1073,13 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   const uint32_t tpp = kv->page_size / 16;
   const uint64_t max_tiles = (uint64_t)kv->max_pages_per_seq * tpp;
   const uint64_t rows = (uint64_t)num_seqs * Hkv;
-  const Plan pl = plan(num_seqs ? num_seqs : 1, Hkv, max_tiles, tpp, split_pages);
+  const Plan pl = plan(num_seqs ? num_seqs : 1, Hkv, max_tiles, tpp, split_pages, opts ? opts->sliding_window : 0);
+  // The counters come first, in a region of one size for all but huge batches, so
+  // that decodes of any shapes can share a workspace whose counters stay zero.  A
+  // part has O and, for each of up to 8 slices, (m, l) per head.
+  const uint64_t ctr_bytes = (rows * 8 * sizeof(unsigned) + kCounterBytes - 1) / kCounterBytes * kCounterBytes;
   const uint64_t parts = pl.slots * group;
-  const uint64_t ctr_off = (parts * (kD + 2 * pl.slices) * sizeof(float) + 255) / 256 * 256;
-  const uint64_t ws = ctr_off + rows * pl.slices * sizeof(unsigned);
+  const uint64_t ws = ctr_bytes + parts * (kD + 2 * 8) * sizeof(float);
   if (ws_needed_out) {
     *ws_needed_out = ws;
     return DOE_OK;
@@ -884,9 +1099,9 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
                  "kv heads");
     return DOE_INVALID_ARGUMENT;
   }
-  for (const void* p : {(const void*)kv->k_pool, (const void*)kv->v_pool, q, (const void*)launch->workspace})
+  for (const void* p : {(const void*)kv->k_pool, (const void*)kv->v_pool, q, (const void*)launch->workspace, (const void*)out})
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) {
-      set_op_error("doe_paged_decode: pools, q and the workspace must be 16-byte aligned");
+      set_op_error("doe_paged_decode: pools, q, out and the workspace must be 16-byte aligned");
       return DOE_INVALID_ARGUMENT;
     }
   for (const void* p : {new_k, new_v})
@@ -903,9 +1118,9 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   a.new_k = static_cast<const __half*>(new_k);
   a.new_v = static_cast<const __half*>(new_v);
   a.out = out;
-  a.part_o = static_cast<float*>(launch->workspace);
+  a.counters = static_cast<unsigned*>(launch->workspace);
+  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(launch->workspace) + ctr_bytes);
   a.part_ml = a.part_o + parts * kD;
-  a.counters = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(launch->workspace) + ctr_off);
   a.status = launch->status;
   a.freq_cis = opts ? opts->freq_cis : nullptr;
   a.rope_positions = opts ? (int)opts->rope_positions : 0;
@@ -928,16 +1143,14 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   a.out_bf16 = (opts && (opts->flags & DOE_DECODE_OUT_BF16)) ? 1 : 0;
   a.inputs_stable = (opts && (opts->flags & DOE_DECODE_INPUTS_STABLE)) ? 1 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(launch->stream);
-  if (pl.max_parts > 1 && !(opts && (opts->flags & DOE_DECODE_COUNTERS_ZEROED))) {
+  if ((pl.list || pl.max_parts > 1) && !(opts && (opts->flags & DOE_DECODE_COUNTERS_ZEROED))) {
     const int rc =
         cuda_status(cudaMemsetAsync(a.counters, 0, rows * pl.slices * sizeof(unsigned), st), "cudaMemsetAsync(split counters)");
     if (rc != DOE_OK) return rc;
   }
-  const dim3 grid = pl.shares ? dim3((unsigned)pl.grid) : dim3((unsigned)pl.grid, Hkv, num_seqs);
-  const unsigned slices = (unsigned)pl.slices;
-  if (pl.shares)
-    return a.softcap > 0.0f ? launch_one<true, true>(a, grid, slices, st) : launch_one<false, true>(a, grid, slices, st);
-  return a.softcap > 0.0f ? launch_one<true, false>(a, grid, slices, st) : launch_one<false, false>(a, grid, slices, st);
+  const dim3 grid = pl.list ? dim3((unsigned)pl.grid) : dim3((unsigned)pl.grid, Hkv, num_seqs);
+  return a.softcap > 0.0f ? launch_cap<true>(a, pl.list, grid, (unsigned)pl.slices, st)
+                          : launch_cap<false>(a, pl.list, grid, (unsigned)pl.slices, st);
 }
 
 }  // namespace doe

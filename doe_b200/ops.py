@@ -115,7 +115,8 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     out_dtype torch.bfloat16 writes a bf16 output (DOE_DECODE_OUT_BF16).
     `ws`: a workspace kept for paged decodes alone, zeroed when created
     (decode_workspace); its split counters then need no clearing per call
-    (DOE_DECODE_COUNTERS_ZEROED).  inputs_stable: seq_lens, the block table and
+    (DOE_DECODE_COUNTERS_ZEROED).  int4 caches keep one per stream by
+    themselves.  inputs_stable: seq_lens, the block table and
     the pool rows (other than the appended ones) are final before the call is
     enqueued, so the first copies may start before the preceding kernel ends
     (DOE_DECODE_INPUTS_STABLE)."""
@@ -127,19 +128,21 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     out = torch.empty((B, H, D), dtype=out_dtype, device=q.device) if out is None else out
     _need(out, out_dtype, "out")
     flags = abi.DECODE_OUT_BF16 if out_dtype == torch.bfloat16 else 0
-    if ws is not None:
+    if ws is not None or cache.kv_dtype == "int4":
         flags |= abi.DECODE_COUNTERS_ZEROED
     if inputs_stable:
         flags |= abi.DECODE_INPUTS_STABLE
     kv = cache.struct()
     lib = abi.lib()
     need = lib.doe_paged_decode_workspace_bytes(C.byref(kv), B, H, split_pages)
-    if ws is None:
+    if ws is None and cache.kv_dtype != "int4":
         l = _launch(need, status, stream, q.device)
     else:
-        if ws.numel() < need:
-            raise ValueError(f"decode workspace of {need} bytes needed, {ws.numel()} given")
         s = stream if stream is not None else torch.cuda.current_stream(q.device)
+        if ws is None:
+            ws = _kept_workspace(need, q.device, s)
+        elif ws.numel() < need:
+            raise ValueError(f"decode workspace of {need} bytes needed, {ws.numel()} given")
         l = abi.Launch(s.cuda_stream, ws.data_ptr(), ws.numel(), status.data_ptr() if status is not None else None)
     nk = new_k.data_ptr() if new_k is not None else None
     nv = new_v.data_ptr() if new_v is not None else None
@@ -162,6 +165,21 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
             C.byref(kv), B, H, q.data_ptr(), seq_lens.data_ptr(), nk, nv, float(scale), out.data_ptr(),
             split_pages, freq_cis.data_ptr(), freq_cis.shape[0], C.byref(l)))
     return out
+
+
+_DECODE_WS: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _kept_workspace(nbytes: int, device, stream) -> torch.Tensor:
+    """The int4 decodes' own workspace of a stream: its counters stay zero from call to call, whatever
+    the shapes (they come first), so no call clears them."""
+    key = (device.index, stream.cuda_stream)
+    buf = _DECODE_WS.get(key)
+    if buf is None or buf.numel() < nbytes:
+        with torch.cuda.stream(stream):
+            buf = torch.zeros(max(nbytes, 1 << 22), dtype=torch.uint8, device=device)
+        _DECODE_WS[key] = buf
+    return buf
 
 
 def decode_workspace(cache: PagedKVCache, num_seqs: int, num_heads: int, split_pages: int = 0) -> torch.Tensor:

@@ -6,6 +6,8 @@
 //
 // Both are copies with a little arithmetic, bound by HBM: 512 bytes of f16 K
 // and V against 144 bytes of blocks per (token, kv head).
+#include <type_traits>
+
 #include "int4.cuh"
 
 namespace doe {
@@ -34,123 +36,128 @@ struct Int4AppendArgs {
   int n_tokens, num_kv_heads, rope_positions;
 };
 
-// One warp per (sequence, 16-token block, kv head); half-warp hw takes the
-// token pairs 2 j + hw, lane l16 the dims [8 l16, 8 l16 + 8): one K word per
-// token and two V words per pair.
+// One warp per (sequence, 16-token block, kv head, K or V).  Half-warp hw takes the
+// token pairs 2 j + hw, lane l16 the dims [8 l16, 8 l16 + 8): one K word per token
+// and two V words per pair; a group's maximum is four lanes'.  All 16 rows (4 KB)
+// are loaded before any is quantised.
+struct BlockWork {
+  int b, h, kv;
+  int pos0;             // the chunk's first position
+  long long first, end;  // the block's first position, the chunk's end
+  size_t block;         // byte offset in the pool
+  bool mapped;
+  __device__ __forceinline__ bool live(int tok) const { return first + tok >= pos0 && first + tok < end; }
+  __device__ __forceinline__ size_t row(int tok, int n_tokens, int heads) const {
+    return ((size_t)b * n_tokens + (size_t)(first + tok - pos0)) * heads + h;
+  }
+};
+// False: nothing of the chunk is there.  An unmapped block is reported.
+__device__ __forceinline__ bool find_block(BlockWork& w, const PageMap& map, const int32_t* positions, int n_tokens,
+                                           int heads, int wid, int32_t* status) {
+  w.kv = wid & 1;
+  w.h = (wid >> 1) % heads;
+  w.b = blockIdx.y;
+  w.pos0 = positions[w.b];
+  w.first = (long long)(w.pos0 & ~15) + 16ll * (wid / (2 * heads));
+  w.end = (long long)w.pos0 + n_tokens;
+  if (w.first >= w.end) return false;
+  const int page = w.pos0 < 0 ? -1 : map.page(w.b, w.first);
+  w.mapped = page >= 0;
+  if (!w.mapped && (threadIdx.x & 31) == 0) report(status, DOE_DEVICE_ERR_PAGE);
+  const int tile = (int)(w.first % map.page_size) / 16;
+  w.block = w.mapped ? (((size_t)page * heads + w.h) * (map.page_size / 16) + tile) * kI4Block : 0;
+  return true;
+}
+
+template <bool ROPE>
 __global__ void __launch_bounds__(256) int4_append_kernel(const Int4AppendArgs a, int warps_per_seq) {
   const int wid = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (wid >= warps_per_seq) return;
   const int hw = lane >> 4, l16 = lane & 15, t = l16 & 3, group = l16 >> 2;
-  const int Hkv = a.num_kv_heads, h = wid % Hkv, b = blockIdx.y;
-  const int pos0 = a.positions[b];
-  if (pos0 < 0) {
-    if (wid == 0 && lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
-    return;
-  }
-  const long long first = (long long)(pos0 & ~15) + 16ll * (wid / Hkv);  // the block's first position
-  const long long end = (long long)pos0 + a.n_tokens;
-  if (first >= end) return;
-  const int page = a.map.page(b, first);
-  if (page < 0) {
-    if (lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
-    return;
-  }
-  const int tiles = a.map.page_size / 16;
-  const int tile = (int)(first % a.map.page_size) / 16;
-  const size_t block = (((size_t)page * Hkv + h) * tiles + tile) * kI4Block;
-
-  for (int kv = 0; kv < 2; ++kv) {
-    const __half* src = kv ? a.new_v : a.new_k;
-    uint8_t* dst = (kv ? a.v_pool : a.k_pool) + block;
-    uint4 x[8];
+  BlockWork w;
+  if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid, a.status) || !w.mapped) return;
+  const __half* src = (w.kv ? a.new_v : a.new_k) + 8 * l16;
+  uint8_t* dst = (w.kv ? a.v_pool : a.k_pool) + w.block;
+  uint4 x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {  // token 2 (2 (i / 2) + hw) + i % 2 of the block
+  for (int i = 0; i < 8; ++i) {
+    const int tok = 4 * (i >> 1) + 2 * hw + (i & 1);
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (w.live(tok)) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + w.row(tok, a.n_tokens, a.num_kv_heads) * 128));
+  }
+  if (ROPE && w.kv == 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
       const int tok = 4 * (i >> 1) + 2 * hw + (i & 1);
-      const long long pos = first + tok;
-      const bool live = pos >= pos0 && pos < end;
-      x[i] = make_uint4(0, 0, 0, 0);
-      if (live)
-        x[i] = *reinterpret_cast<const uint4*>(
-            src + (((size_t)b * a.n_tokens + (size_t)(pos - pos0)) * Hkv + h) * 128 + 8 * l16);
-    }
-    if (kv == 0 && a.freq_cis != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int tok = 4 * (i >> 1) + 2 * hw + (i & 1);
-        const long long pos = first + tok;
-        const bool live = pos >= pos0 && pos < end;
-        uint4 p;
-        p.x = __shfl_xor_sync(0xffffffffu, x[i].x, 8);
-        p.y = __shfl_xor_sync(0xffffffffu, x[i].y, 8);
-        p.z = __shfl_xor_sync(0xffffffffu, x[i].z, 8);
-        p.w = __shfl_xor_sync(0xffffffffu, x[i].w, 8);
-        if (live) {
-          float c[8], sn[8];
-          rope_table<4>(a.freq_cis, a.rope_positions, 64, pos, 8 * (l16 & 7), a.status, l16 == 0, c, sn);
-          const uint4 mine = x[i];
-          rope_rotate<4>(reinterpret_cast<const uint32_t*>(&mine), reinterpret_cast<const uint32_t*>(&p), l16 < 8, c,
-                         sn, reinterpret_cast<uint32_t*>(&x[i]));
-        }
+      uint4 p;
+      p.x = __shfl_xor_sync(0xffffffffu, x[i].x, 8);
+      p.y = __shfl_xor_sync(0xffffffffu, x[i].y, 8);
+      p.z = __shfl_xor_sync(0xffffffffu, x[i].z, 8);
+      p.w = __shfl_xor_sync(0xffffffffu, x[i].w, 8);
+      if (w.live(tok)) {
+        float c[8], sn[8];
+        rope_table<4>(a.freq_cis, a.rope_positions, 64, w.first + tok, 8 * (l16 & 7), a.status, l16 == 0, c, sn);
+        const uint4 mine = x[i];
+        rope_rotate<4>(reinterpret_cast<const uint32_t*>(&mine), reinterpret_cast<const uint32_t*>(&p), l16 < 8, c, sn,
+                       reinterpret_cast<uint32_t*>(&x[i]));
       }
     }
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int pair = 2 * j + hw;
-      uint32_t code[2][8];
-      __half sh[2];
-      bool live[2];
+  for (int j = 0; j < 4; ++j) {
+    const int pair = 2 * j + hw;
+    uint2 c[2][4];  // codes of dims (2 i, 2 i + 1)
+    __half sh[2];
+    bool live[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      live[e] = w.live(2 * pair + e);
+      const __half2* hx = reinterpret_cast<const __half2*>(&x[2 * j + e]);
+      const __half2 m2 = __hmax2(__hmax2(__habs2(hx[0]), __habs2(hx[1])), __hmax2(__habs2(hx[2]), __habs2(hx[3])));
+      float amax = fmaxf(__low2float(m2), __high2float(m2));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      sh[e] = __float2half_rn(div7(amax));
+      const float s = __half2float(sh[e]), rs = inverse_of(s);
+      if (s >= 0x1p-14f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[e][i] = quantize_u4x2<false>(__half22float2(hx[i]), s, rs);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[e][i] = quantize_u4x2<true>(__half22float2(hx[i]), s, rs);
+      }
+    }
+    if (w.kv == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const long long pos = first + 2 * pair + e;
-        live[e] = pos >= pos0 && pos < end;
-        const __half2* hx = reinterpret_cast<const __half2*>(&x[2 * j + e]);
-        __half2 m2 = __hmax2(__hmax2(__habs2(hx[0]), __habs2(hx[1])), __hmax2(__habs2(hx[2]), __habs2(hx[3])));
-        float amax = fmaxf(__low2float(m2), __high2float(m2));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        sh[e] = __float2half_rn(div7(amax));
-        const float s = __half2float(sh[e]);
-        const float rs = s != 0.0f ? __frcp_rn(s) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = __half22float2(hx[i]);
-          code[e][2 * i] = s != 0.0f ? quantize_u4(f.x, s, rs) : 8u;
-          code[e][2 * i + 1] = s != 0.0f ? quantize_u4(f.y, s, rs) : 8u;
+        const int tok = 2 * pair + e;
+        const uint32_t even = pack_u4x4(c[e][0].x, c[e][1].x, c[e][2].x, c[e][3].x);
+        const uint32_t odd = pack_u4x4(c[e][0].y, c[e][1].y, c[e][2].y, c[e][3].y);
+        if (live[e]) {
+          *reinterpret_cast<uint32_t*>(dst + tok * 64 + t * 16 + group * 4) = prmt(even, odd, 0x5410u);
+          if (t == 0) *reinterpret_cast<__half*>(dst + kI4Codes + (tok * 4 + group) * 2) = sh[e];
         }
       }
-      if (kv == 0) {
+    } else {
+      // dims 8 l16 .. + 8 are g = 2 t (the first four) and g = 2 t + 1
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t w = 0;
+      for (int u = 0; u < 2; ++u) {
+        uint32_t half[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w |= (code[e][2 * i] | (code[e][2 * i + 1] << 16)) << (4 * i);
-          const int tok = 2 * pair + e;
-          if (live[e]) {
-            *reinterpret_cast<uint32_t*>(dst + tok * 64 + t * 16 + group * 4) = w;
-            if (t == 0) *reinterpret_cast<__half*>(dst + kI4Codes + (tok * 4 + group) * 2) = sh[e];
-          }
+        for (int e = 0; e < 2; ++e)
+          half[e] = pack_u4x4(c[e][2 * u].x, c[e][2 * u].y, c[e][2 * u + 1].x, c[e][2 * u + 1].y);
+        uint8_t* at = dst + (((pair >> 2) * 8 + 2 * t + u) * 4 + (pair & 3)) * 16 + group * 4;
+        if (live[0] && live[1]) {
+          *reinterpret_cast<uint32_t*>(at) = prmt(half[0], half[1], 0x5410u);
+        } else {
+          if (live[0]) *reinterpret_cast<uint16_t*>(at) = (uint16_t)half[0];
+          if (live[1]) *reinterpret_cast<uint16_t*>(at + 2) = (uint16_t)half[1];
         }
-      } else {
-        // dims 8 l16 .. + 8 are g = 2 t (the first four) and g = 2 t + 1
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t hw16[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            hw16[e] = code[e][4 * u] | (code[e][4 * u + 1] << 4) | (code[e][4 * u + 2] << 8) | (code[e][4 * u + 3] << 12);
-          uint8_t* at = dst + (((pair >> 2) * 8 + 2 * t + u) * 4 + (pair & 3)) * 16 + group * 4;
-          if (live[0] && live[1]) {
-            *reinterpret_cast<uint32_t*>(at) = hw16[0] | (hw16[1] << 16);
-          } else {
-            if (live[0]) *reinterpret_cast<uint16_t*>(at) = (uint16_t)hw16[0];
-            if (live[1]) *reinterpret_cast<uint16_t*>(at + 2) = (uint16_t)hw16[1];
-          }
-        }
-        if (t == 0) {
-          __half* at = reinterpret_cast<__half*>(dst + kI4Codes) + (pair * 4 + group) * 2;
-          if (live[0]) at[0] = sh[0];
-          if (live[1]) at[1] = sh[1];
-        }
+      }
+      if (t == 0) {
+        __half* at = reinterpret_cast<__half*>(dst + kI4Codes) + (pair * 4 + group) * 2;
+        if (live[0]) at[0] = sh[0];
+        if (live[1]) at[1] = sh[1];
       }
     }
   }
@@ -173,9 +180,13 @@ int launch_int4_append(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tok
   a.num_kv_heads = (int)kv->num_kv_heads;
   a.rope_positions = (int)rope_positions;
   // a chunk starting inside a block touches one block more
-  const uint64_t warps = (((uint64_t)n_tokens + 14) / 16 + 1) * kv->num_kv_heads;
+  const uint64_t warps = (((uint64_t)n_tokens + 14) / 16 + 1) * kv->num_kv_heads * 2;
   const dim3 grid((unsigned)((warps + 7) / 8), num_seqs);
-  int4_append_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(launch->stream)>>>(a, (int)warps);
+  cudaStream_t st = static_cast<cudaStream_t>(launch->stream);
+  if (freq_cis != nullptr)
+    int4_append_kernel<true><<<grid, 256, 0, st>>>(a, (int)warps);
+  else
+    int4_append_kernel<false><<<grid, 256, 0, st>>>(a, (int)warps);
   return cuda_status(cudaGetLastError(), "int4_append_kernel");
 }
 
@@ -210,66 +221,81 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
     reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(r)[i];
 }
 
-// The lane layout of int4_append_kernel, reversed: one warp per (sequence,
-// 16-token block, kv head).
+// (n - 8) * s of a code pair where the mask has left it, in f16: 1024 + n (or 1024 +
+// 16 n) and n - 8 are exact, so the product is rounded once, as from f32.
+__device__ __forceinline__ __half2 code_values(uint32_t w, int i, __half2 s) {
+  const uint32_t x = (i & 2) ? w >> 8 : w;
+  uint32_t m = (i & 1) ? (x & 0x00f000f0u) | 0x64006400u : (x & 0x000f000fu) | 0x64006400u;
+  __half2 v = *reinterpret_cast<__half2*>(&m);
+  v = (i & 1) ? __hfma2(v, __float2half2_rn(0.0625f), __float2half2_rn(-72.0f)) : __hadd2(v, __float2half2_rn(-1032.0f));
+  return __hmul2(v, s);
+}
+
+// The lane layout of int4_append_kernel, reversed.
 template <typename T>
 __global__ void __launch_bounds__(256) int4_read_kernel(const PagedReadArgs a, int warps_per_seq) {
   const int wid = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (wid >= warps_per_seq) return;
   const int hw = lane >> 4, l16 = lane & 15, t = l16 & 3, group = l16 >> 2;
-  const int Hkv = a.num_kv_heads, h = wid % Hkv, b = blockIdx.y;
-  const int pos0 = a.positions[b];
-  if (pos0 < 0) {
-    if (wid == 0 && lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
-    return;
-  }
-  const long long first = (long long)(pos0 & ~15) + 16ll * (wid / Hkv);
-  const long long end = (long long)pos0 + a.n_tokens;
-  if (first >= end) return;
-  const int page = a.map.page(b, first);
-  if (page < 0) {
-    if (lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
-    return;
-  }
-  const int tiles = a.map.page_size / 16;
-  const int tile = (int)(first % a.map.page_size) / 16;
-  const size_t block = (((size_t)page * Hkv + h) * tiles + tile) * kI4Block;
-  for (int kv = 0; kv < 2; ++kv) {
-    const uint8_t* src = a.pool[kv] + block;
-    T* dst = static_cast<T*>(a.out[kv]);
-    uint32_t w[8];
-    __half s[8];
+  BlockWork w;
+  if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid, a.status)) return;
+  const uint8_t* src = (w.kv ? a.pool[1] : a.pool[0]) + w.block;
+  T* dst = static_cast<T*>(w.kv ? a.out[1] : a.out[0]) + 8 * l16;
+  uint32_t code[4][2];
+  __half s[4][2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int pair = 2 * j + hw;
+  for (int j = 0; j < 4; ++j) {
+    const int pair = 2 * j + hw;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (kv == 0) {
-          const int tok = 2 * pair + e;
-          w[2 * j + e] = *reinterpret_cast<const uint32_t*>(src + tok * 64 + t * 16 + group * 4);
-          s[2 * j + e] = reinterpret_cast<const __half*>(src + kI4Codes)[tok * 4 + group];
-        } else {
-          w[2 * j + e] = *reinterpret_cast<const uint32_t*>(
-              src + (((pair >> 2) * 8 + 2 * t + e) * 4 + (pair & 3)) * 16 + group * 4);
-          s[2 * j + e] = reinterpret_cast<const __half*>(src + kI4Codes)[(pair * 4 + group) * 2 + e];
-        }
+    for (int e = 0; e < 2; ++e) {
+      const int tok = 2 * pair + e;
+      const int at = w.kv ? (((pair >> 2) * 8 + 2 * t + e) * 4 + (pair & 3)) * 16 + group * 4 : tok * 64 + t * 16 + group * 4;
+      const int sc = w.kv ? (pair * 4 + group) * 2 + e : tok * 4 + group;
+      // an unmapped block reads as zeros
+      code[j][e] = w.mapped ? *reinterpret_cast<const uint32_t*>(src + at) : 0u;
+      s[j][e] = w.mapped ? reinterpret_cast<const __half*>(src + kI4Codes)[sc] : __ushort_as_half(0);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    // values of tokens 2 pair and 2 pair + 1 as four (dim, dim + 1) pairs
+    __half2 v[2][4];
+    if constexpr (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value) {
+      if (w.kv == 0) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[e][i] = code_values(code[j][e], i, __half2half2(s[j][e]));
+      } else {
+        const __half2 s2 = __halves2half2(s[j][0], s[j][1]);
+#pragma unroll
+        for (int i = 0; i < 4; i += 2)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            // one dim of both tokens each
+            const __half2 a0 = code_values(code[j][u], i, s2), a1 = code_values(code[j][u], i + 1, s2);
+            v[0][2 * u + i / 2] = __lows2half2(a0, a1);
+            v[1][2 * u + i / 2] = __highs2half2(a0, a1);
+          }
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const long long pos = first + 2 * (2 * j + hw) + e;
-        if (pos < pos0 || pos >= end) continue;
-        const float sf = __half2float(s[2 * j + e]);
-        float v[8];
+    for (int e = 0; e < 2; ++e) {
+      const int tok = 2 * (2 * j + hw) + e;
+      if (!w.live(tok)) continue;
+      T* at = dst + w.row(tok, a.n_tokens, a.num_kv_heads) * 128;
+      if constexpr (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value) {
+        __stcs(reinterpret_cast<uint4*>(at), *reinterpret_cast<const uint4*>(v[e]));
+      } else {
+        const float sf = __half2float(s[j][e]);
+        float f[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint32_t n = kv == 0 ? (w[2 * j + e] >> (4 * (i >> 1) + 16 * (i & 1))) & 15u
-                                     : (w[2 * j + (i >> 2)] >> (16 * e + 4 * (i & 3))) & 15u;
-          v[i] = (float)((int)n - 8) * sf;
+          const uint32_t n = w.kv == 0 ? (code[j][e] >> (4 * (i >> 1) + 16 * (i & 1))) & 15u
+                                       : (code[j][i >> 2] >> (16 * e + 4 * (i & 3))) & 15u;
+          f[i] = (float)((int)n - 8) * sf;
         }
-        store8(dst + (((size_t)b * a.n_tokens + (size_t)(pos - pos0)) * Hkv + h) * 128 + 8 * l16, v);
+        store8(at, f);
       }
     }
   }
@@ -284,19 +310,18 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const PagedReadArgs a) 
   const int pos0 = a.positions[b];
   const long long pos = (long long)pos0 + tok;
   const int page = pos0 < 0 ? -1 : a.map.page(b, pos);
-  if (page < 0) {
-    if (lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
-    return;
-  }
+  if (page < 0 && lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
   const int in_page = (int)(pos % a.map.page_size);
   const int Hkv = a.num_kv_heads, D = a.head_dim, n = Hkv * D;
   const size_t row = ((size_t)page * a.map.page_size + in_page) * n;
   const size_t out = ((size_t)b * a.n_tokens + tok) * n;
+#pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
     T* dst = static_cast<T*>(a.out[kv]) + out;
     for (int i = lane * 8; i < n; i += 256) {
-      float v[8];
-      if (INT8) {
+      float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};  // of an unmapped page
+      if (page < 0) {
+      } else if (INT8) {
         const float s = __half2float(a.scale[kv][((size_t)page * Hkv + i / D) * a.map.page_size + in_page]);
         const uint2 w = *reinterpret_cast<const uint2*>(a.pool[kv] + row + i);
         const int8_t* c = reinterpret_cast<const int8_t*>(&w);
@@ -320,7 +345,7 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const PagedReadArgs a) 
 template <typename T>
 static int launch_read(const doe_paged_kv* kv, const PagedReadArgs& a, uint32_t num_seqs, cudaStream_t st) {
   if (kv->kv_dtype == DOE_KV_INT4) {
-    const uint64_t warps = (((uint64_t)a.n_tokens + 14) / 16 + 1) * kv->num_kv_heads;
+    const uint64_t warps = (((uint64_t)a.n_tokens + 14) / 16 + 1) * kv->num_kv_heads * 2;
     const dim3 grid((unsigned)((warps + 7) / 8), num_seqs);
     int4_read_kernel<T><<<grid, 256, 0, st>>>(a, (int)warps);
     return cuda_status(cudaGetLastError(), "int4_read_kernel");

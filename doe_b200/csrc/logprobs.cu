@@ -8,15 +8,24 @@
 //   top k by (value descending, index ascending); NaN orders as -inf
 //
 // One pass over the row: every element is loaded once, costs one exponential
-// and a comparison with a threshold.  Bound by HBM for f32 and near the SFU's
-// rate for 16-bit logits.  All sums are f32.
+// and a share of a maximum.  Bound by HBM for f32 and near the SFU's rate for
+// 16-bit logits.  All sums are f32.
+//
+// Loads go through a ring in shared memory (cp.async, every thread its own
+// vectors, no barrier): 4 CTAs of 24 KB in flight per SM, where two vectors per
+// thread in registers kept 24 KB and 0.54 of HBM.
 //
 // Top k without sorting the row: the maxima of 32 disjoint thread groups are 32
-// different elements, so their minimum is a value that at least 32 elements
-// reach.  Elements below it are never candidates; the others (about 32 ln 32 of
-// all those seen when it was taken) go into a shared buffer.  The threshold is
-// renewed at the 1st, 2nd, 4th, 8th, ... step.  A full buffer (sorted or tied
-// rows) is cut to its best k, whose last key then is the threshold.
+// different elements, so the k-th largest of them is a bound that at least k
+// elements reach.  It is taken at the first step; elements above it go into a
+// shared buffer.  After the 1st, 4th, 16th, ... step the buffer is cut to its
+// best k, whose last value is the new bound: later elements equal to it lose by
+// their index, so only larger ones matter, about k of them until the next cut.
+// Between cuts the warps run on without a barrier (one per step cost 40 of 155 us
+// at 1024 rows of 128256 bf16 logits).  A row that fills the buffer all the same
+// (rising ones) is gone over again with a cut whenever it is full.  Where fewer
+// than k elements lie above the first bound (rows that a mask or ties leave with
+// few values) the first ones that equal it are looked for in another pass.
 //
 // Few rows: a row is split over a cluster of up to 8 CTAs whose statistics and
 // best k meet in the first CTA through distributed shared memory, so the call
@@ -33,8 +42,8 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
-constexpr int kCap = 2048;    // candidate buffer (a power of two)
-constexpr int kUnroll = 4;    // 16-byte loads per thread and step
+constexpr int kCap = 1024;    // candidate buffer (a power of two)
+constexpr uint32_t kStages = 4;  // steps in the ring
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct Args {
@@ -66,40 +75,52 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 16 bytes of logits: N elements, two per step of each().
 template <typename T>
 struct Vec;
 template <>
 struct Vec<float> {
-  static constexpr int N = 4;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
-    x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y);
-    x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+  static constexpr int N = 4, kUnroll = 2;  // 16-byte loads per thread and step
+  static constexpr uint32_t kLow = 0xff800000u;  // -inf
+  static __device__ __forceinline__ float max(const uint4& v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  static __device__ __forceinline__ float2 pair(const uint4& v, int i) {
+    return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
+                  : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
   }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
 };
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) {
+  return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w));
+}
 template <>
 struct Vec<__half> {
-  static constexpr int N = 8;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
+  static constexpr int N = 8, kUnroll = 2;
+  static constexpr uint32_t kLow = 0xfc00fc00u;
+  static __device__ __forceinline__ float2 pair(const uint4& v, int i) {
+    const uint32_t w = word(v, i);
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+  static __device__ __forceinline__ float max(const uint4& v) {
     const __half2* h = reinterpret_cast<const __half2*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(h[i]);
-      x[2 * i] = f.x; x[2 * i + 1] = f.y;
-    }
+    const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(f.x, f.y);
   }
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
 };
 template <>
 struct Vec<__nv_bfloat16> {
-  static constexpr int N = 8;
-  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+  static constexpr int N = 8, kUnroll = 2;
+  static constexpr uint32_t kLow = 0xff80ff80u;
+  static __device__ __forceinline__ float2 pair(const uint4& v, int i) {
+    const uint32_t w = word(v, i);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ float max(const uint4& v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 };
@@ -129,11 +150,12 @@ __device__ __forceinline__ Stat merge(Stat a, Stat b) {
 struct Shared {
   unsigned long long buf[kCap];
   unsigned long long sel[kMaxTop];  // the CTA's best k, in order
-  unsigned long long thr_key;       // buffer cuts: only better keys matter
-  float wmin[kWarps];
+  float group_max[32];
   Stat stat[kWarps];
+  uint32_t hits[kWarps];
   Stat total;
   uint32_t count;
+  uint32_t full;  // candidates were lost
 };
 
 // Sorts buf[0, n) descending; n is padded to a power of two with zeros.
@@ -165,6 +187,7 @@ __device__ void select(Shared& sh, uint32_t n, uint32_t k) {
     if (threadIdx.x < n) {
       const unsigned long long mine = sh.buf[threadIdx.x];
       uint32_t rank = 0;
+#pragma unroll 8
       for (uint32_t i = 0; i < n; ++i) rank += sh.buf[i] > mine;
       if (rank < k) sh.sel[rank] = mine;
     }
@@ -175,138 +198,222 @@ __device__ void select(Shared& sh, uint32_t n, uint32_t k) {
   __syncthreads();
 }
 
-// A lower bound that at least 32 of the elements seen so far reach: the least
-// of 32 groups' maxima (8 threads each).  Every thread gets it.
-__device__ float group_bound(Shared& sh, float tmax) {
+// A lower bound that at least k of the elements seen so far reach: the k-th
+// largest of 32 groups' maxima (8 threads each).  Every thread gets it.
+__device__ float group_bound(Shared& sh, float tmax, uint32_t k) {
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, o));
-#pragma unroll
-  for (int o = 8; o < 32; o <<= 1) tmax = fminf(tmax, __shfl_xor_sync(0xffffffffu, tmax, o));
-  if ((threadIdx.x & 31) == 0) sh.wmin[threadIdx.x >> 5] = tmax;
+  if ((threadIdx.x & 7) == 0) sh.group_max[threadIdx.x >> 3] = tmax;
   __syncthreads();
-  float b = sh.wmin[0];
-#pragma unroll
-  for (int i = 1; i < kWarps; ++i) b = fminf(b, sh.wmin[i]);
+  const uint32_t lane = threadIdx.x & 31;
+  const float mine = sh.group_max[lane];
+  uint32_t rank = 0;
+#pragma unroll 8
+  for (uint32_t i = 0; i < 32; ++i) {
+    const float other = sh.group_max[i];
+    rank += other > mine || (other == mine && i < lane);
+  }
+  const uint32_t at = __ballot_sync(0xffffffffu, rank == k - 1);
+  const float bound = __shfl_sync(0xffffffffu, mine, __ffs(at) - 1);
   __syncthreads();
-  return b;
+  return bound;
+}
+
+// Drops the candidates that are not above `bound`; the others stay, in any order.
+// Synchronises before and after.
+__device__ void filter(Shared& sh, float bound) {
+  __syncthreads();
+  const uint32_t n = min(sh.count, (uint32_t)kCap);
+  unsigned long long mine[kCap / kThreads];
+#pragma unroll
+  for (int i = 0; i < kCap / kThreads; ++i) mine[i] = i * kThreads + threadIdx.x < n ? sh.buf[i * kThreads + threadIdx.x] : 0;
+  __syncthreads();
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kCap / kThreads; ++i)
+    if (mine[i] != 0 && value_of(mine[i]) > bound) sh.buf[atomicAdd(&sh.count, 1u)] = mine[i];
+  __syncthreads();
+}
+
+// Keeps the best k of n >= k candidates; the last of them is the new bound.
+__device__ void cut(Shared& sh, uint32_t n, uint32_t k, float& bound) {
+  select(sh, n, k);
+  if (threadIdx.x < k) sh.buf[threadIdx.x] = sh.sel[threadIdx.x];
+  if (threadIdx.x == 0) sh.count = k;
+  bound = fmaxf(bound, value_of(sh.sel[k - 1]));
+  __syncthreads();
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const Args a, uint32_t splits) {
+__global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uint32_t splits) {
   __shared__ Shared sh;
-  constexpr int N = Vec<T>::N;
+  __shared__ uint4 ring[kStages * Vec<T>::kUnroll * kThreads];  // every thread reads what it loaded
+  using V = Vec<T>;
+  constexpr int N = V::N, kUnroll = V::kUnroll;
   const uint32_t split = blockIdx.x, tid = threadIdx.x, k = a.top_k;
   const uint64_t row = blockIdx.y;
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
   // 16-byte vectors from the row's base rounded down; the first and the last
-  // may hold elements outside the row
+  // may hold elements outside the row, which count as -inf
   const uint32_t shift = (uint32_t)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const uint4* base = reinterpret_cast<const uint4*>(x - shift);
-  const uint64_t nvec = ((uint64_t)shift + a.vocab + N - 1) / N;
-  const uint64_t per = (nvec + splits - 1) / splits;
-  const uint64_t v0 = split * per, v1 = v0 + per < nvec ? v0 + per : nvec;
-  if (tid == 0) {
-    sh.count = 0;
-    sh.thr_key = 0;
-  }
+  const uint32_t nvec = (uint32_t)(((uint64_t)shift + a.vocab + N - 1) / N), per = (nvec + splits - 1) / splits;
+  const uint32_t v0 = min(nvec, split * per), v1 = min(nvec, v0 + per);
+  const uint32_t whole0 = shift ? 1 : 0, whole1 = (uint32_t)(((uint64_t)shift + a.vocab) / N);  // vectors within the row
+  if (tid == 0) sh.count = sh.full = 0;
   __syncthreads();
 
+  int32_t token = -1;
+  float given = -INFINITY;  // the given token's logit
+  if (split == 0 && tid == 0 && a.tokens != nullptr) {
+    token = a.tokens[row];
+    if ((uint32_t)token < a.vocab) given = V::one(x + token);
+  }
   Stat st = {-INFINITY, 0.0f, 0.0f};
   float tmax = -INFINITY, bound = -INFINITY;
   uint32_t step = 0;
-  for (uint64_t at = v0; at < v1; at += kThreads * kUnroll, ++step) {
-    uint4 raw[kUnroll];
-    float e[kUnroll][N];
-    uint32_t live = 0;  // bit u: the vector holds elements of the row
+  // This thread's elements above the bound go into the buffer, one reservation per
+  // warp.  Returns the threads whose elements did not all fit: none of theirs are
+  // taken, and their places stay empty.
+  auto push = [&](const uint4 (&raw)[kUnroll], uint32_t at, float bound, bool mine) {
+    uint32_t hits = 0;
+    if (mine) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const uint64_t v = at + (uint64_t)u * kThreads + tid;
-      if (v < v1 && (v > 0 || shift == 0) && (v + 1) * N <= (uint64_t)shift + a.vocab) {
-        raw[u] = ldg_stream(base + v);
-        live |= 1u << u;
-      }
-    }
+      for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const uint64_t v = at + (uint64_t)u * kThreads + tid;
-      if (live >> u & 1) {
-        Vec<T>::unpack(raw[u], e[u]);
-      } else if (v < v1) {  // an edge vector: elements outside the row count as absent (-inf)
-        live |= 1u << u;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint64_t j = v * N + i;
-          e[u][i] = j >= shift && j < (uint64_t)shift + a.vocab ? Vec<T>::one(x + (j - shift)) : -INFINITY;
+        for (int i = 0; i < N; i += 2) {
+          const float2 f = V::pair(raw[u], i / 2);
+          hits |= (f.x > bound ? 1u : 0u) << (u * N + i) | (f.y > bound ? 2u : 0u) << (u * N + i);
         }
-      }
     }
-    float vmax = -INFINITY;
+    const uint32_t some = __popc(hits);
+    uint32_t upto = some;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
+      if ((tid & 31) >= o) upto += up;
+    }
+    uint32_t pos = 0;
+    if ((tid & 31) == 31 && upto != 0) pos = atomicAdd(&sh.count, upto);
+    pos = __shfl_sync(0xffffffffu, pos, 31) + upto - some;
+    const bool lost = pos + some > kCap && some != 0;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (live >> u & 1)
+      if (hits >> (u * N) & ((1u << N) - 1))
 #pragma unroll
-        for (int i = 0; i < N; ++i) vmax = fmaxf(vmax, e[u][i]);
+        for (int i = 0; i < N; ++i)
+          if (hits >> (u * N + i) & 1) {
+            const float2 f = V::pair(raw[u], i / 2);
+            const uint64_t j = (uint64_t)(at + u * kThreads + tid) * N + i - shift;
+            if (pos < kCap) sh.buf[pos] = lost ? 0ull : key_of((i & 1) ? f.y : f.x, (uint32_t)j);
+            ++pos;
+          }
+    return lost;
+  };
+  // An edge vector, element by element: those outside the row are -inf.
+  auto edge = [&](uint32_t at, uint4 (&raw)[kUnroll]) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const uint32_t v = at + u * kThreads + tid;
+      if (v < v1 && (v < whole0 || v >= whole1)) {
+        T e[N];
+        uint4 low = make_uint4(V::kLow, V::kLow, V::kLow, V::kLow);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint64_t j = (uint64_t)v * N + i;
+          e[i] = j >= shift && j < (uint64_t)shift + a.vocab ? x[j - shift] : reinterpret_cast<const T*>(&low)[i];
+        }
+        memcpy(&raw[u], e, 16);
+      }
+    }
+  };
+  constexpr uint32_t kStep = kThreads * kUnroll;  // vectors
+  auto inside = [&](uint32_t v) { return v < v1 && v >= whole0 && v < whole1; };
+  auto load = [&](uint32_t at, uint32_t slot) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const uint32_t v = at + u * kThreads + tid;
+      if (inside(v))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(
+                         (uint32_t)__cvta_generic_to_shared(&ring[(slot * kUnroll + u) * kThreads + tid])),
+                     "l"(base + v)
+                     : "memory");
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  };
+#pragma unroll
+  for (uint32_t i = 0; i < kStages - 1; ++i) load(v0 + i * kStep, i);
+  for (uint32_t at = v0; at < v1; at += kStep, ++step) {
+    load(at + (kStages - 1) * kStep, (step + kStages - 1) % kStages);
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 1) : "memory");
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      raw[u] = make_uint4(V::kLow, V::kLow, V::kLow, V::kLow);
+      if (inside(at + u * kThreads + tid)) raw[u] = ring[((step % kStages) * kUnroll + u) * kThreads + tid];
+    }
+    if (at < whole0 || at + kStep > whole1) edge(at, raw);
+    float vmax = V::max(raw[0]);
+#pragma unroll
+    for (int u = 1; u < kUnroll; ++u) vmax = fmaxf(vmax, V::max(raw[u]));
     if (vmax > st.m) raise(st, vmax);
     const float neg_m = st.m == -INFINITY ? 0.0f : -st.m;
     float2 s2 = make_float2(st.s, 0.0f), w2 = make_float2(st.w, 0.0f);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (live >> u & 1)
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-          const float2 d = fmul2(fadd2(make_float2(e[u][i], e[u][i + 1]), make_float2(neg_m, neg_m)),
-                                 make_float2(kLog2e, kLog2e));
-          const float2 p = make_float2(ex2(d.x), ex2(d.y));
-          s2 = fadd2(s2, p);
-          // clamped: a masked element adds 0 to w, not 0 * inf
-          w2 = ffma2(p, make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f)), w2);
-        }
+      for (int i = 0; i < N / 2; ++i) {
+        const float2 d = fmul2(fadd2(V::pair(raw[u], i), make_float2(neg_m, neg_m)), make_float2(kLog2e, kLog2e));
+        const float2 p = make_float2(ex2(d.x), ex2(d.y));
+        s2 = fadd2(s2, p);
+        // clamped: a masked element adds 0 to w, not 0 * inf
+        w2 = ffma2(p, make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f)), w2);
+      }
     st.s = s2.x + s2.y;
     st.w = w2.x + w2.y;
     if (k == 0) continue;
     tmax = fmaxf(tmax, vmax);
-    if ((step & (step + 1)) == 0) bound = fmaxf(bound, group_bound(sh, tmax));
-    // candidates; retried after a cut when the buffer was full
-    unsigned long long pending = 0;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (live >> u & 1)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint64_t j = (at + (uint64_t)u * kThreads + tid) * N + i;
-          if (!(e[u][i] < bound) && j >= shift && j < (uint64_t)shift + a.vocab) pending |= 1ull << (u * N + i);
-        }
-    while (true) {
-      if (pending) {
-        const unsigned long long thr = sh.thr_key;
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (pending >> (u * N + i) & 1) {
-              const uint64_t j = (at + (uint64_t)u * kThreads + tid) * N + i - shift;
-              const unsigned long long key = key_of(e[u][i], (uint32_t)j);
-              if (key <= thr) {
-                pending &= ~(1ull << (u * N + i));
-              } else {
-                const uint32_t pos = atomicAdd(&sh.count, 1u);
-                if (pos < kCap) {
-                  sh.buf[pos] = key;
-                  pending &= ~(1ull << (u * N + i));
-                }
-              }
-            }
-      }
-      if (!__syncthreads_or(pending != 0)) break;
-      // full: keep the best k; the last of them is the new threshold
-      select(sh, kCap, k);
-      if (tid < k) sh.buf[tid] = sh.sel[tid];
-      if (tid == 0) {
-        sh.count = k;
-        sh.thr_key = sh.sel[k - 1];
-      }
-      bound = fmaxf(bound, value_of(sh.sel[k - 1]));
+    if (step == 0) bound = group_bound(sh, tmax, k);
+    if (__any_sync(0xffffffffu, vmax > bound) && push(raw, at, bound, true)) sh.full = 1;
+    if ((step & (step + 1)) == 0 && (step + 1 & 0x55555555u) != 0) {  // 1st, 4th, 16th, ... step
       __syncthreads();
+      const uint32_t n = sh.count;
+      const bool full = sh.full != 0;
+      __syncthreads();  // before the next candidates are counted
+      if (n > k && !full) cut(sh, n, k, bound);
+    }
+  }
+  __syncthreads();
+  if (sh.full) {
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    bound = tmax = -INFINITY;
+    for (uint32_t at = v0; at < v1; at += kStep) {
+      uint4 raw[kUnroll];
+      float vmax = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        raw[u] = make_uint4(V::kLow, V::kLow, V::kLow, V::kLow);
+        if (inside(at + u * kThreads + tid)) raw[u] = ldg_stream(base + at + u * kThreads + tid);
+      }
+      if (at < whole0 || at + kStep > whole1) edge(at, raw);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) vmax = fmaxf(vmax, V::max(raw[u]));
+      tmax = fmaxf(tmax, vmax);
+      if (at == v0) bound = group_bound(sh, tmax, k);
+      bool todo = true;
+      for (int round = 0;; ++round) {
+        if (__any_sync(0xffffffffu, todo && vmax > bound)) todo = push(raw, at, bound, todo);
+        else todo = false;
+        if (!__syncthreads_or(todo)) break;
+        if (round == 0) {  // a new bound
+          bound = fmaxf(bound, group_bound(sh, tmax, k));
+          filter(sh, bound);
+        } else {  // full again: the best k so far are the bound
+          cut(sh, kCap, k, bound);
+        }
+      }
     }
   }
 
@@ -318,31 +425,43 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Args a, uint32
     st = merge(st, b);
   }
   if ((tid & 31) == 0) sh.stat[tid >> 5] = st;
+  if (k != 0) {
+    __syncthreads();
+    uint32_t n = sh.count;
+    select(sh, n, k);
+    if (n < k) {
+      // the rest are the first elements that equal the bound (a NaN equals -inf)
+      const uint64_t j1 = min((uint64_t)a.vocab, max((uint64_t)v1 * N, (uint64_t)shift) - shift);
+      for (uint64_t j0 = max((uint64_t)v0 * N, (uint64_t)shift) - shift; j0 < j1 && n < k; j0 += kThreads) {
+        const uint64_t j = j0 + tid;
+        float v = 0.0f;
+        bool equal = false;
+        if (j < j1) {
+          v = V::one(x + j);
+          equal = bound == -INFINITY ? !(v > bound) : v == bound;
+        }
+        const uint32_t mask = __ballot_sync(0xffffffffu, equal);
+        if ((tid & 31) == 0) sh.hits[tid >> 5] = __popc(mask);
+        __syncthreads();
+        uint32_t pos = n + __popc(mask & ((1u << (tid & 31)) - 1));
+        for (uint32_t w = 0; w < kWarps; ++w) {
+          if (w < tid >> 5) pos += sh.hits[w];
+          n += sh.hits[w];
+        }
+        if (equal && pos < k) sh.sel[pos] = key_of(v, (uint32_t)j);
+        __syncthreads();
+      }
+    }
+  }
   __syncthreads();
   if (tid == 0) {
     Stat t = sh.stat[0];
     for (int i = 1; i < kWarps; ++i) t = merge(t, sh.stat[i]);
     sh.total = t;
   }
-  if (k != 0) {
-    // drop what the last bound excludes, then order the rest
-    bound = fmaxf(bound, group_bound(sh, tmax));
-    const uint32_t n = sh.count;
-    unsigned long long mine[kCap / kThreads];
-#pragma unroll
-    for (int i = 0; i < kCap / kThreads; ++i) mine[i] = i * kThreads + tid < n ? sh.buf[i * kThreads + tid] : 0;
-    __syncthreads();
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kCap / kThreads; ++i)
-      if (mine[i] != 0 && !(value_of(mine[i]) < bound)) sh.buf[atomicAdd(&sh.count, 1u)] = mine[i];
-    __syncthreads();
-    select(sh, sh.count, k);
-  }
   if (splits > 1) {
     cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
+    cluster.sync();  // every CTA's total and sel
     if (split == 0) {
       Stat t = sh.total;
       for (uint32_t i = 1; i < splits; ++i) t = merge(t, *cluster.map_shared_rank(&sh.total, i));
@@ -367,13 +486,8 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Args a, uint32
   const float ls = logf(t.s);
   if (tid == 0) {
     if (a.logprob != nullptr) {
-      const int32_t token = a.tokens[row];
-      float v = -INFINITY;
-      if ((uint32_t)token < a.vocab)
-        v = none ? -INFINITY : Vec<T>::one(x + token) - t.m - ls;
-      else
-        report(a.status, DOE_DEVICE_ERR_POSITION);
-      a.logprob[row] = v;
+      if ((uint32_t)token >= a.vocab) report(a.status, DOE_DEVICE_ERR_POSITION);
+      a.logprob[row] = none || (uint32_t)token >= a.vocab ? -INFINITY : given - t.m - ls;
     }
     if (a.entropy != nullptr) a.entropy[row] = none ? 0.0f : ls - t.w / t.s * kLn2;
   }
@@ -386,11 +500,12 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Args a, uint32
 
 template <typename T>
 int launch(const Args& a, uint64_t rows, cudaStream_t st) {
-  // A row is split while the CTAs would leave SMs idle and every split still
-  // has two steps' work.
+  // A row is split while there are at most 3 CTAs per SM (4 are resident; a split costs
+  // its own cuts: 64 rows of 128257 bf16 logits in 4 splits 21 us, in 8 25) and every split
+  // still has two steps' work.
   uint32_t splits = 1;
-  const uint64_t step = (uint64_t)kThreads * kUnroll * Vec<T>::N;
-  while (splits < 8 && rows * splits < 2ull * num_sms() && a.vocab > splits * step) splits *= 2;
+  const uint64_t step = (uint64_t)kThreads * Vec<T>::kUnroll * Vec<T>::N;
+  while (splits < 8 && rows * splits * 2 <= 3ull * num_sms() && a.vocab > splits * step) splits *= 2;
   for (uint64_t r0 = 0; r0 < rows; r0 += 65535) {
     Args b = a;
     const uint64_t n = rows - r0 < 65535 ? rows - r0 : 65535;

@@ -69,7 +69,7 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 
 // The int4 chunk kernels' own limits.
 int check_int4_chunk(const doe_paged_kv* kv, const char* fn, uint32_t n_tokens, const void* a, const void* b) {
-  if (n_tokens > 0x40000000u || ((uint64_t)n_tokens / 16 + 2) * kv->num_kv_heads > 0x7fffffffull)
+  if (n_tokens > 0x40000000u || ((uint64_t)n_tokens / 16 + 2) * kv->num_kv_heads > 0x3fffffffull)
     return invalid("%s: too many tokens (%u) for one launch", fn, n_tokens);
   if ((uint64_t)kv->page_size > 0x40000000u || kv->max_pages_per_seq > 0x7fffffffu || kv->num_pages > 0x7fffffffu)
     return invalid("%s: page_size, num_pages and max_pages_per_seq are limited to 31 bits", fn);

@@ -204,23 +204,17 @@ struct AppendRow {
       for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       const __half sh = __float2half_rn(div7(amax));
       const float s = __half2float(sh);
-      const float rs = s != 0.0f ? __frcp_rn(s) : 0.0f;
-      uint32_t c[4] = {8u, 8u, 8u, 8u};
-      if (s != 0.0f) {
-        c[0] = quantize_u4(x01.x, s, rs);
-        c[1] = quantize_u4(x01.y, s, rs);
-        c[2] = quantize_u4(x23.x, s, rs);
-        c[3] = quantize_u4(x23.y, s, rs);
-      }
+      const float rs = inverse_of(s);
+      const uint2 c01 = quantize_u4x2(x01, s, rs), c23 = quantize_u4x2(x23, s, rs);
       uint8_t* dst = (kv ? a.v_pool : a.k_pool) + block;
       if (kv == 0) {
         // even lanes hold dims 0..3 of the word's 8, odd lanes dims 4..7
-        uint32_t w = (c[0] | (c[1] << 16) | (c[2] << 4) | (c[3] << 20)) << (8 * (lane & 1));
+        uint32_t w = ((c01.x & 15u) | (c01.y & 15u) << 16 | (c23.x & 15u) << 4 | (c23.y & 15u) << 20) << (8 * (lane & 1));
         w |= __shfl_xor_sync(0xffffffffu, w, 1);
         if ((lane & 1) == 0) *reinterpret_cast<uint32_t*>(dst + tok * 64 + ((lane & 7) >> 1) * 16 + group * 4) = w;
         if ((lane & 7) == 0) *reinterpret_cast<__half*>(dst + kI4Codes + (tok * 4 + group) * 2) = sh;
       } else {
-        const uint32_t w = c[0] | (c[1] << 4) | (c[2] << 8) | (c[3] << 12);
+        const uint32_t w = pack_u4x4(c01.x, c01.y, c23.x, c23.y);
         *reinterpret_cast<uint16_t*>(dst + (((tok >> 3) * 8 + (lane & 7)) * 4 + ((tok >> 1) & 3)) * 16 + group * 4 +
                                      2 * (tok & 1)) = (uint16_t)w;
         if ((lane & 7) == 0)

@@ -29,10 +29,18 @@ def workspace(nbytes: int, device=None) -> torch.Tensor:
     return buf
 
 
+def _stream_handle(stream, device) -> int:
+    """The cudaStream_t of `stream`, or of the device's current stream (without building a
+    torch.cuda.Stream, which costs more than the rest of a wrapper)."""
+    if stream is not None:
+        return stream.cuda_stream
+    index = device.index if isinstance(device, torch.device) else None
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
 def _launch(ws_bytes: int = 0, status: torch.Tensor | None = None, stream=None, device=None) -> abi.Launch:
-    s = stream if stream is not None else torch.cuda.current_stream(device)
     ws = workspace(ws_bytes, device) if ws_bytes else None
-    return abi.Launch(s.cuda_stream, ws.data_ptr() if ws is not None else None,
+    return abi.Launch(_stream_handle(stream, device), ws.data_ptr() if ws is not None else None,
                       ws.numel() if ws is not None else 0,
                       status.data_ptr() if status is not None else None)
 
@@ -138,12 +146,12 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     if ws is None and cache.kv_dtype != "int4":
         l = _launch(need, status, stream, q.device)
     else:
-        s = stream if stream is not None else torch.cuda.current_stream(q.device)
+        s = _stream_handle(stream, q.device)
         if ws is None:
-            ws = _kept_workspace(need, q.device, s)
+            ws = _kept_workspace(need, q.device, s, stream)
         elif ws.numel() < need:
             raise ValueError(f"decode workspace of {need} bytes needed, {ws.numel()} given")
-        l = abi.Launch(s.cuda_stream, ws.data_ptr(), ws.numel(), status.data_ptr() if status is not None else None)
+        l = abi.Launch(s, ws.data_ptr(), ws.numel(), status.data_ptr() if status is not None else None)
     nk = new_k.data_ptr() if new_k is not None else None
     nv = new_v.data_ptr() if new_v is not None else None
     if sliding_window or softcap or flags:
@@ -167,18 +175,21 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     return out
 
 
-_DECODE_WS: dict[tuple[int, int], torch.Tensor] = {}
+_DECODE_WS: dict[tuple[int, int], list[torch.Tensor]] = {}
 
 
-def _kept_workspace(nbytes: int, device, stream) -> torch.Tensor:
+def _kept_workspace(nbytes: int, device, handle: int, stream) -> torch.Tensor:
     """The int4 decodes' own workspace of a stream: its counters stay zero from call to call, whatever
-    the shapes (they come first), so no call clears them."""
-    key = (device.index, stream.cuda_stream)
-    buf = _DECODE_WS.get(key)
-    if buf is None or buf.numel() < nbytes:
-        with torch.cuda.stream(stream):
-            buf = torch.zeros(max(nbytes, 1 << 22), dtype=torch.uint8, device=device)
-        _DECODE_WS[key] = buf
+    the shapes (they come first), so no call clears them.  Outgrown ones are kept, for the CUDA graphs
+    that may hold them; a capture that needs a larger one gets its own."""
+    kept = _DECODE_WS.setdefault((device.index, handle), [])
+    if kept and kept[-1].numel() >= nbytes:
+        return kept[-1]
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    with torch.cuda.stream(stream):  # None: the current stream, which `handle` is then
+        buf = torch.zeros(max(nbytes, 1 << 22, 2 * kept[-1].numel() if kept else 0), dtype=torch.uint8, device=device)
+    kept.append(buf)
     return buf
 
 
@@ -232,14 +243,15 @@ def paged_read(cache: PagedKVCache, positions, n_tokens: int, dtype=torch.float1
     """kv_read as values: tokens positions[b] .. + n_tokens of every sequence b (block-table
     row b) -> (k, v) [B, n_tokens, Hkv, D] of dtype (f16, bf16 or f32), for any cache type.
 
-    Rows on unmapped pages are left as they were (zeros without `out`)."""
+    Rows on unmapped pages are zeros (and set DOE_DEVICE_ERR_PAGE in `status`)."""
     _need(positions, torch.int32, "positions")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be float16, bfloat16 or float32")
     B = _rows_of(cache, positions.numel())
     shape = (B, int(n_tokens), cache.num_kv_heads, cache.head_dim)
     if out is None:
-        k, v = torch.zeros((2,) + shape, dtype=dtype, device=positions.device)
+        k = torch.empty(shape, dtype=dtype, device=positions.device)
+        v = torch.empty(shape, dtype=dtype, device=positions.device)
     else:
         k, v = out
         for t, n in ((k, "out k"), (v, "out v")):
@@ -294,15 +306,16 @@ def token_logprobs(logits, tokens=None, top_k: int = 0, status=None, stream=None
         if tokens.numel() != rows:
             raise ValueError(f"{rows} rows of logits, {tokens.numel()} tokens")
     dev = logits.device
-    f = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev) if tokens is not None else None
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
     ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
     top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
     l = _launch(0, status, stream, dev)
     abi.check("doe_token_logprobs", abi.lib().doe_token_logprobs(
         logits.data_ptr(), _DTYPES[logits.dtype], rows, vocab, max(logits.stride(0), vocab),
-        tokens.data_ptr() if tokens is not None else None, top_k, f[0].data_ptr() if tokens is not None else None,
-        f[1].data_ptr(), ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None, C.byref(l)))
-    return TokenLogprobs(f[0] if tokens is not None else None, f[1], ids, top)
+        tokens.data_ptr() if tokens is not None else None, top_k, logprob.data_ptr() if tokens is not None else None,
+        entropy.data_ptr(), ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None, C.byref(l)))
+    return TokenLogprobs(logprob, entropy, ids, top)
 
 
 def kv_write_dense(k_proj, v_proj, k_cache, v_cache, positions, status=None, stream=None):

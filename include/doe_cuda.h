@@ -410,8 +410,8 @@ int doe_paged_gather(const doe_paged_kv* kv, uint32_t seq, uint32_t start,
  * n_tokens, Hkv, D] of `dtype` (DOE_DTYPE_*, one rounding of code * scale; f16
  * pools are converted).  The rows a prefill over a cached prefix reads, or an
  * export; any pool type (doe_paged_gather copies codes and does not take int4
- * pools).  Rows on unmapped pages set DOE_DEVICE_ERR_PAGE and are left as they
- * were.  head_dim a multiple of 8; pools and outputs 16-byte aligned.       */
+ * pools).  Rows on unmapped pages set DOE_DEVICE_ERR_PAGE and are zeros.
+ * head_dim a multiple of 8; pools and outputs 16-byte aligned.       */
 int doe_paged_read(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tokens,
                    const int32_t* positions, void* k_out, void* v_out, uint32_t dtype,
                    const doe_launch* launch);

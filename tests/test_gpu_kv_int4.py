@@ -282,7 +282,7 @@ def test_append_every_scale_and_code():
     assert np.array_equal(cache.v_pool.cpu().numpy(), vp)
 
 
-def test_append_and_read_leave_unmapped_rows():
+def test_append_skips_and_read_zeroes_unmapped_rows():
     g = np.random.default_rng(6)
     table = np.array([[0, -1], [1, 2], [3, 3]], np.int32)
     cache = PagedKVCache(num_pages=3, page_size=16, num_kv_heads=2, head_dim=128, block_table=table, kv_dtype="int4")
@@ -300,9 +300,13 @@ def test_append_and_read_leave_unmapped_rows():
     assert int(status.item()) == DOE_DEVICE_ERR_PAGE
     got = out[0].cpu().numpy()
     want = kv_int4.values(*kv_int4.quantize(k))
-    assert np.array_equal(got[0, :12], want[0, :12].astype(np.float32)) and (got[0, 12:] == 9).all()
-    assert np.array_equal(got[1, :2], want[1, :2].astype(np.float32)) and (got[1, 2:] == 9).all()
-    assert (got[2] == 9).all()
+    assert np.array_equal(got[0, :12], want[0, :12].astype(np.float32)) and (got[0, 12:] == 0).all()
+    assert np.array_equal(got[1, :2], want[1, :2].astype(np.float32)) and (got[1, 2:] == 0).all()
+    assert (got[2] == 0).all()
+    old = PagedKVCache(num_pages=1, page_size=16, num_kv_heads=1, head_dim=128, block_table=np.array([[0, -1]]))
+    old.k_pool.fill_(2.0)
+    got = ops.paged_read(old, _t(np.array([10], np.int32)), 12, status=status)[0]
+    assert (got[0, :6] == 2).all() and (got[0, 6:] == 0).all()
 
 
 def test_append_rope_beyond_the_table_reports():

@@ -23,10 +23,10 @@ struct PageRegions {
 };
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // 16-byte loads in flight per thread
+constexpr int kUnroll = 8;  // 16-byte loads in flight per thread (4: 188 us for 8000 f16 pages, 8: 180)
 constexpr uint32_t kPiece = kThreads * kUnroll * 16;
 
-// One CTA per (16 KB piece of a page, pair).
+// One CTA per (32 KB piece of a page, pair).
 template <int N>
 __global__ void __launch_bounds__(kThreads)
     copy_pages_kernel(const __grid_constant__ PagePairs<N> pairs, const PageRegions r) {
@@ -41,9 +41,10 @@ __global__ void __launch_bounds__(kThreads)
     region = piece / r.chunks[0];
     piece %= r.chunks[0];
   }
-  const uint64_t bytes = r.page_bytes[region >> 1];
-  const uint4* src = reinterpret_cast<const uint4*>(r.base[region] + (uint64_t)from * bytes);
-  uint4* dst = reinterpret_cast<uint4*>(r.base[region] + (uint64_t)to * bytes);
+  const uint64_t bytes = region < 2 ? r.page_bytes[0] : r.page_bytes[1];
+  uint8_t* base = region == 0 ? r.base[0] : region == 1 ? r.base[1] : region == 2 ? r.base[2] : r.base[3];
+  const uint4* src = reinterpret_cast<const uint4*>(base + (uint64_t)from * bytes);
+  uint4* dst = reinterpret_cast<uint4*>(base + (uint64_t)to * bytes);
   const uint64_t n = bytes / 16, i0 = (uint64_t)piece * (kPiece / 16) + threadIdx.x;
   uint4 v[kUnroll];
 #pragma unroll

@@ -20,7 +20,8 @@ operators") and the tensor-parallel AllReduce to NCCL:
 
 Precision: weights and GEMM inputs bf16 with f32 accumulation; the residual
 stream f32; q/k/v and the KV cache f16 (every bf16-derived value is exact or
-better in f16 at these magnitudes); attention in f32.
+better in f16 at these magnitudes) unless DecoderConfig.kv_dtype asks for an
+int8 or int4 cache; attention in f32.
 
 Tensor parallelism (Megatron-style, by KV head): rank r of N holds query heads
 [r H/N, (r+1) H/N), KV heads [r Hkv/N, ...), the matching o_proj columns, FFN
@@ -56,6 +57,7 @@ class DecoderConfig:
     ctx: int = 4096          # cached tokens per sequence before the step
     page_size: int = 16
     weight_std: float = 0.02
+    kv_dtype: str = "f16"    # of the caches the decoder makes: "f16", "int8" or "int4"
 
     def check(self, world: int) -> None:
         if self.heads * self.head_dim != self.hidden:
@@ -78,8 +80,9 @@ class DecoderConfig:
         return 2 * (per + 2 * E) * self.layers
 
     def kv_read_bytes(self) -> int:
-        """f16 K and V bytes one step reads (ctx + 1 tokens per sequence, all layers)."""
-        return self.batch * (self.ctx + 1) * self.kv_heads * self.head_dim * 2 * 2 * self.layers
+        """K and V bytes one step reads (ctx + 1 tokens per sequence, all layers)."""
+        row = {"f16": 2 * self.head_dim, "int8": self.head_dim + 2, "int4": 72}[self.kv_dtype]
+        return self.batch * (self.ctx + 1) * self.kv_heads * row * 2 * self.layers
 
 
 def rope_table(positions: int, head_dim: int, theta: float) -> np.ndarray:
@@ -175,7 +178,7 @@ class Decoder:
             caches = []
             for l in range(cfg.layers):
                 c = PagedKVCache(num_pages=int(table.size), page_size=cfg.page_size, num_kv_heads=self.kvh,
-                                 head_dim=D, block_table=table, device=dev)
+                                 head_dim=D, block_table=table, kv_dtype=cfg.kv_dtype, device=dev)
                 fill_pools(c, seed * 1000 + 100 * l + rank)
                 caches.append(c)
         self.caches = caches

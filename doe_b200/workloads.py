@@ -91,6 +91,8 @@ class PagedWorkload:
     def kv_bytes_per_token(self) -> int:
         if self.kv_dtype == "f16":
             return 2 * self.num_kv_heads * self.head_dim * 2
+        if self.kv_dtype == "int4":
+            return 2 * self.num_kv_heads * 72  # 128 codes of 4 bits + 4 f16 scales, K and V
         return 2 * self.num_kv_heads * (self.head_dim + 2)  # int8 + f16 scale, K and V
 
     def step_bytes(self) -> dict:
@@ -204,7 +206,8 @@ def small_paged(seed: int, lens, num_heads=32, num_kv_heads=8, head_dim=128, pag
 def fill_pools(cache, seed: int, std: float = 1.0, chunk_rows: int = 1 << 18) -> None:
     """Fill a PagedKVCache's pools with seeded N(0, std) values on its device.
 
-    f16 pools hold the values; int8 pools hold their quantisation under the
+    f16 pools hold the values; int4 pools hold what doe_paged_append makes of
+    them; int8 pools hold their quantisation under the
     int8 KV definition (scale = f16(absmax / 127) per token and kv head,
     q = clamp(rint(x / scale), -127, 127)), computed with IEEE division and
     round-half-even on the device."""
@@ -214,6 +217,20 @@ def fill_pools(cache, seed: int, std: float = 1.0, chunk_rows: int = 1 << 18) ->
     gen.manual_seed(seed)
     rows = cache.k_pool.shape[0]
     Hkv, D, P = cache.num_kv_heads, cache.head_dim, cache.page_size
+    if cache.kv_dtype == "int4":
+        from . import ops
+        from .kv import PagedKVCache
+
+        step = max(1, min(65535, chunk_rows // P))
+        for p0 in range(0, cache.num_pages, step):
+            n = min(step, cache.num_pages - p0)
+            k, v = ((torch.randn((n, P, Hkv, D), generator=gen, device=cache.k_pool.device) * std).half()
+                    for _ in range(2))
+            pages = torch.arange(p0, p0 + n, dtype=torch.int32, device=cache.k_pool.device)[:, None].contiguous()
+            part = PagedKVCache.from_pools(cache.k_pool, cache.v_pool, page_size=P, num_kv_heads=Hkv, head_dim=D,
+                                           block_table=pages, kv_dtype="int4")
+            ops.paged_append(part, k, v, torch.zeros(n, dtype=torch.int32, device=cache.k_pool.device))
+        return
     for pool, scale in ((cache.k_pool, cache.k_scale), (cache.v_pool, cache.v_scale)):
         for r0 in range(0, rows, chunk_rows):
             r1 = min(rows, r0 + chunk_rows)

@@ -235,6 +235,30 @@ def test_decode_long_sequence_splits_and_far_pages():
         assert bool(((out - ref).abs() <= 2.0 ** -10 * 1.1 * a + 1e-4).all())
 
 
+@pytest.mark.parametrize("batch", [1, 32])
+def test_decode_long_flat_softmax_keeps_its_precision(batch):
+    """Tens of thousands of about equal weights: O is a hundred times smaller than the sums of codes
+    it comes from.  The two f16 roundings leave a relative error (2-norm) of 2^-12 each at most; 5e-4
+    leaves as much again for the f32 sums."""
+    n = 20000
+    pages = -(-n // 16)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(batch, 1)  # one text, shared
+    cache = PagedKVCache(num_pages=pages, page_size=16, num_kv_heads=8, head_dim=128, block_table=np.zeros((1, 1)),
+                         kv_dtype="int4")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    k, v = (torch.randn((1, n, 8, 128), generator=g, device="cuda").half() for _ in range(2))
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache.block_table, cache.max_pages_per_seq = table, pages
+    ops.paged_append(cache, k, v, zero)
+    q = torch.randn((batch, 32, 128), generator=g, device="cuda").half()
+    out = ops.paged_decode(cache, q, torch.full((batch,), n, dtype=torch.int32, device="cuda"), 128 ** -0.5).double()
+    k, v = (x[0].double() for x in ops.paged_read(cache, zero, n, dtype=torch.float32))
+    x = torch.einsum("bgud,tgd->bgut", q.double().view(batch, 8, 4, 128), k) / 128 ** 0.5
+    ref = torch.einsum("bgut,tgd->bgud", torch.softmax(x, -1), v).reshape(batch, 32, 128)
+    assert float((out - ref).norm() / ref.norm()) < 5e-4
+
+
 @pytest.mark.parametrize("rope", [False, True])
 @pytest.mark.parametrize("Hkv,page,T", [(1, 16, 1), (2, 16, 2), (8, 16, 15), (2, 32, 16), (1, 48, 17), (4, 16, 50), (3, 64, 33)])
 def test_append_is_exact(Hkv, page, T, rope):

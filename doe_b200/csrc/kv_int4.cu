@@ -42,14 +42,12 @@ struct Int4AppendArgs {
 // are loaded before any is quantised.
 struct BlockWork {
   int b, h, kv;
-  int pos0;             // the chunk's first position
-  long long first, end;  // the block's first position, the chunk's end
-  size_t block;         // byte offset in the pool
+  long long first;   // the block's first position
+  int lo, hi;        // its tokens in the chunk: [lo, hi) of 16
+  long long row0;    // row of token 0 in [B, T, Hkv] (of lo > 0: before the chunk's)
+  size_t block;      // byte offset in the pool
   bool mapped;
-  __device__ __forceinline__ bool live(int tok) const { return first + tok >= pos0 && first + tok < end; }
-  __device__ __forceinline__ size_t row(int tok, int n_tokens, int heads) const {
-    return ((size_t)b * n_tokens + (size_t)(first + tok - pos0)) * heads + h;
-  }
+  __device__ __forceinline__ bool whole() const { return lo == 0 && hi == 16; }
 };
 // False: nothing of the chunk is there.  An unmapped block is reported.
 __device__ __forceinline__ bool find_block(BlockWork& w, const PageMap& map, const int32_t* positions, int n_tokens,
@@ -57,11 +55,14 @@ __device__ __forceinline__ bool find_block(BlockWork& w, const PageMap& map, con
   w.kv = wid & 1;
   w.h = (wid >> 1) % heads;
   w.b = blockIdx.y;
-  w.pos0 = positions[w.b];
-  w.first = (long long)(w.pos0 & ~15) + 16ll * (wid / (2 * heads));
-  w.end = (long long)w.pos0 + n_tokens;
-  if (w.first >= w.end) return false;
-  const int page = w.pos0 < 0 ? -1 : map.page(w.b, w.first);
+  const int pos0 = positions[w.b];
+  w.first = (long long)(pos0 & ~15) + 16ll * (wid / (2 * heads));
+  const long long end = (long long)pos0 + n_tokens;
+  if (w.first >= end) return false;
+  w.lo = (int)max(0ll, pos0 - w.first);
+  w.hi = (int)min(16ll, end - w.first);
+  w.row0 = ((long long)w.b * n_tokens + (w.first - pos0)) * heads + w.h;
+  const int page = pos0 < 0 ? -1 : map.page(w.b, w.first);
   w.mapped = page >= 0;
   if (!w.mapped && (threadIdx.x & 31) == 0) report(status, DOE_DEVICE_ERR_PAGE);
   const int tile = (int)(w.first % map.page_size) / 16;
@@ -69,21 +70,20 @@ __device__ __forceinline__ bool find_block(BlockWork& w, const PageMap& map, con
   return true;
 }
 
-template <bool ROPE>
-__global__ void __launch_bounds__(256) int4_append_kernel(const Int4AppendArgs a, int warps_per_seq) {
-  const int wid = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (wid >= warps_per_seq) return;
-  const int hw = lane >> 4, l16 = lane & 15, t = l16 & 3, group = l16 >> 2;
-  BlockWork w;
-  if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid, a.status) || !w.mapped) return;
-  const __half* src = (w.kv ? a.new_v : a.new_k) + 8 * l16;
+// WHOLE: all 16 tokens are in the chunk.
+template <bool ROPE, bool WHOLE>
+__device__ __forceinline__ void append_block(const Int4AppendArgs& a, const BlockWork& w) {
+  const int lane = threadIdx.x & 31, hw = lane >> 4, l16 = lane & 15, t = l16 & 3, group = l16 >> 2;
+  const __half* src = (w.kv ? a.new_v : a.new_k) + w.row0 * 128 + 8 * l16;
   uint8_t* dst = (w.kv ? a.v_pool : a.k_pool) + w.block;
+  const int stride = a.num_kv_heads * 128;  // of a token
+  auto live = [&](int tok) { return WHOLE || (tok >= w.lo && tok < w.hi); };
   uint4 x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int tok = 4 * (i >> 1) + 2 * hw + (i & 1);
     x[i] = make_uint4(0, 0, 0, 0);
-    if (w.live(tok)) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + w.row(tok, a.n_tokens, a.num_kv_heads) * 128));
+    if (live(tok)) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + (long long)tok * stride));
   }
   if (ROPE && w.kv == 0) {
 #pragma unroll
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(256) int4_append_kernel(const Int4AppendArgs a
       p.y = __shfl_xor_sync(0xffffffffu, x[i].y, 8);
       p.z = __shfl_xor_sync(0xffffffffu, x[i].z, 8);
       p.w = __shfl_xor_sync(0xffffffffu, x[i].w, 8);
-      if (w.live(tok)) {
+      if (live(tok)) {
         float c[8], sn[8];
         rope_table<4>(a.freq_cis, a.rope_positions, 64, w.first + tok, 8 * (l16 & 7), a.status, l16 == 0, c, sn);
         const uint4 mine = x[i];
@@ -103,64 +103,95 @@ __global__ void __launch_bounds__(256) int4_append_kernel(const Int4AppendArgs a
       }
     }
   }
+  // scales of all rows first; the codes' two forms (see quantize_u4x2) then differ
+  // once per warp
+  float s[8], rs[8];
+  __half sh[8];
+  bool normal = true;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int pair = 2 * j + hw;
-    uint2 c[2][4];  // codes of dims (2 i, 2 i + 1)
-    __half sh[2];
-    bool live[2];
+  for (int i = 0; i < 8; ++i) {
+    const __half2* hx = reinterpret_cast<const __half2*>(&x[i]);
+    __half2 m2 = __hmax2(__hmax2(__habs2(hx[0]), __habs2(hx[1])), __hmax2(__habs2(hx[2]), __habs2(hx[3])));
+    uint32_t m = *reinterpret_cast<uint32_t*>(&m2), o = __shfl_xor_sync(0xffffffffu, m, 1);
+    m2 = __hmax2(m2, *reinterpret_cast<__half2*>(&o));
+    m = *reinterpret_cast<uint32_t*>(&m2);
+    o = __shfl_xor_sync(0xffffffffu, m, 2);
+    m2 = __hmax2(m2, *reinterpret_cast<__half2*>(&o));
+    sh[i] = __float2half_rn(div7(fmaxf(__low2float(m2), __high2float(m2))));
+    s[i] = __half2float(sh[i]);
+    rs[i] = inverse_of(s[i]);
+    normal &= s[i] >= 0x1p-14f;
+  }
+  normal = __all_sync(0xffffffffu, normal);
+  auto codes = [&](auto clamp, int i, uint2 (&c)[4]) {
+    const __half2* hx = reinterpret_cast<const __half2*>(&x[i]);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      live[e] = w.live(2 * pair + e);
-      const __half2* hx = reinterpret_cast<const __half2*>(&x[2 * j + e]);
-      const __half2 m2 = __hmax2(__hmax2(__habs2(hx[0]), __habs2(hx[1])), __hmax2(__habs2(hx[2]), __habs2(hx[3])));
-      float amax = fmaxf(__low2float(m2), __high2float(m2));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      sh[e] = __float2half_rn(div7(amax));
-      const float s = __half2float(sh[e]), rs = inverse_of(s);
-      if (s >= 0x1p-14f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[e][i] = quantize_u4x2<false>(__half22float2(hx[i]), s, rs);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[e][i] = quantize_u4x2<true>(__half22float2(hx[i]), s, rs);
-      }
-    }
+    for (int d = 0; d < 4; ++d) c[d] = quantize_u4x2<decltype(clamp)::value>(__half22float2(hx[d]), s[i], rs[i]);
+  };
+  auto write = [&](auto clamp) {
     if (w.kv == 0) {
+      uint8_t* at = dst + hw * 128 + t * 16 + group * 4;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int tok = 2 * pair + e;
-        const uint32_t even = pack_u4x4(c[e][0].x, c[e][1].x, c[e][2].x, c[e][3].x);
-        const uint32_t odd = pack_u4x4(c[e][0].y, c[e][1].y, c[e][2].y, c[e][3].y);
-        if (live[e]) {
-          *reinterpret_cast<uint32_t*>(dst + tok * 64 + t * 16 + group * 4) = prmt(even, odd, 0x5410u);
-          if (t == 0) *reinterpret_cast<__half*>(dst + kI4Codes + (tok * 4 + group) * 2) = sh[e];
+      for (int i = 0; i < 8; ++i) {
+        const int tok = 4 * (i >> 1) + (i & 1);  // + 2 hw
+        uint2 c[4];
+        codes(clamp, i, c);
+        const uint32_t even = pack_u4x4(c[0].x, c[1].x, c[2].x, c[3].x);
+        const uint32_t odd = pack_u4x4(c[0].y, c[1].y, c[2].y, c[3].y);
+        if (live(tok + 2 * hw)) {
+          *reinterpret_cast<uint32_t*>(at + tok * 64) = prmt(even, odd, 0x5410u);
+          if (t == 0) reinterpret_cast<__half*>(dst + kI4Codes)[(tok + 2 * hw) * 4 + group] = sh[i];
         }
       }
-    } else {
-      // dims 8 l16 .. + 8 are g = 2 t (the first four) and g = 2 t + 1
+      return;
+    }
+    // dims 8 l16 .. + 8 are g = 2 t (the first four) and g = 2 t + 1
+    uint8_t* at = dst + t * 128 + hw * 16 + group * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // pair 2 j + hw
+      uint2 c[2][4];
+      codes(clamp, 2 * j, c[0]);
+      codes(clamp, 2 * j + 1, c[1]);
+      const bool live0 = live(4 * j + 2 * hw), live1 = live(4 * j + 2 * hw + 1);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t half[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           half[e] = pack_u4x4(c[e][2 * u].x, c[e][2 * u].y, c[e][2 * u + 1].x, c[e][2 * u + 1].y);
-        uint8_t* at = dst + (((pair >> 2) * 8 + 2 * t + u) * 4 + (pair & 3)) * 16 + group * 4;
-        if (live[0] && live[1]) {
-          *reinterpret_cast<uint32_t*>(at) = prmt(half[0], half[1], 0x5410u);
+        uint8_t* to = at + (j >> 1) * 512 + (j & 1) * 32 + u * 64;
+        if (WHOLE || (live0 && live1)) {
+          *reinterpret_cast<uint32_t*>(to) = prmt(half[0], half[1], 0x5410u);
         } else {
-          if (live[0]) *reinterpret_cast<uint16_t*>(at) = (uint16_t)half[0];
-          if (live[1]) *reinterpret_cast<uint16_t*>(at + 2) = (uint16_t)half[1];
+          if (live0) *reinterpret_cast<uint16_t*>(to) = (uint16_t)half[0];
+          if (live1) *reinterpret_cast<uint16_t*>(to + 2) = (uint16_t)half[1];
         }
       }
       if (t == 0) {
-        __half* at = reinterpret_cast<__half*>(dst + kI4Codes) + (pair * 4 + group) * 2;
-        if (live[0]) at[0] = sh[0];
-        if (live[1]) at[1] = sh[1];
+        __half* to = reinterpret_cast<__half*>(dst + kI4Codes) + ((2 * j + hw) * 4 + group) * 2;
+        if (WHOLE) {
+          *reinterpret_cast<__half2*>(to) = __halves2half2(sh[2 * j], sh[2 * j + 1]);
+        } else {
+          if (live0) to[0] = sh[2 * j];
+          if (live1) to[1] = sh[2 * j + 1];
+        }
       }
     }
-  }
+  };
+  if (normal) write(std::false_type());
+  else write(std::true_type());
+}
+
+template <bool ROPE>
+__global__ void __launch_bounds__(256) int4_append_kernel(const Int4AppendArgs a, int warps_per_seq) {
+  pdl_wait();
+  pdl_trigger();
+  const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (wid >= warps_per_seq) return;
+  BlockWork w;
+  if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid, a.status) || !w.mapped) return;
+  if (w.whole()) append_block<ROPE, true>(a, w);
+  else append_block<ROPE, false>(a, w);
 }
 
 int launch_int4_append(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tokens, const void* new_k,
@@ -183,11 +214,9 @@ int launch_int4_append(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tok
   const uint64_t warps = (((uint64_t)n_tokens + 14) / 16 + 1) * kv->num_kv_heads * 2;
   const dim3 grid((unsigned)((warps + 7) / 8), num_seqs);
   cudaStream_t st = static_cast<cudaStream_t>(launch->stream);
-  if (freq_cis != nullptr)
-    int4_append_kernel<true><<<grid, 256, 0, st>>>(a, (int)warps);
-  else
-    int4_append_kernel<false><<<grid, 256, 0, st>>>(a, (int)warps);
-  return cuda_status(cudaGetLastError(), "int4_append_kernel");
+  return cuda_status(launch_pdl(freq_cis != nullptr ? int4_append_kernel<true> : int4_append_kernel<false>, grid,
+                                dim3(256), 0, st, a, (int)warps),
+                     "int4_append_kernel");
 }
 
 // ---- read: rows [positions[b], + T) of every sequence as values ---------------
@@ -231,63 +260,67 @@ __device__ __forceinline__ __half2 code_values(uint32_t w, int i, __half2 s) {
   return __hmul2(v, s);
 }
 
-// The lane layout of int4_append_kernel, reversed.
-template <typename T>
-__global__ void __launch_bounds__(256) int4_read_kernel(const PagedReadArgs a, int warps_per_seq) {
-  const int wid = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (wid >= warps_per_seq) return;
-  const int hw = lane >> 4, l16 = lane & 15, t = l16 & 3, group = l16 >> 2;
-  BlockWork w;
-  if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid, a.status)) return;
+// The lane layout of append_block, reversed.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void read_block(const PagedReadArgs& a, const BlockWork& w) {
+  const int lane = threadIdx.x & 31, hw = lane >> 4, l16 = lane & 15, t = l16 & 3, group = l16 >> 2;
   const uint8_t* src = (w.kv ? a.pool[1] : a.pool[0]) + w.block;
-  T* dst = static_cast<T*>(w.kv ? a.out[1] : a.out[0]) + 8 * l16;
+  T* dst = static_cast<T*>(w.kv ? a.out[1] : a.out[0]) + w.row0 * 128 + 8 * l16;
+  const int stride = a.num_kv_heads * 128;  // of a token
+  auto live = [&](int tok) { return WHOLE || (tok >= w.lo && tok < w.hi); };
+  // words and scales of tokens 4 j + 2 hw and the next (V: of their pair)
   uint32_t code[4][2];
-  __half s[4][2];
+  __half2 s[4];
+  const uint8_t* at = src + group * 4 + (w.kv ? t * 128 + hw * 16 : hw * 128 + t * 16);
+  const __half* sc = reinterpret_cast<const __half*>(src + kI4Codes) + (w.kv ? hw * 8 + group * 2 : hw * 8 + group);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int pair = 2 * j + hw;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int tok = 2 * pair + e;
-      const int at = w.kv ? (((pair >> 2) * 8 + 2 * t + e) * 4 + (pair & 3)) * 16 + group * 4 : tok * 64 + t * 16 + group * 4;
-      const int sc = w.kv ? (pair * 4 + group) * 2 + e : tok * 4 + group;
-      // an unmapped block reads as zeros
-      code[j][e] = w.mapped ? *reinterpret_cast<const uint32_t*>(src + at) : 0u;
-      s[j][e] = w.mapped ? reinterpret_cast<const __half*>(src + kI4Codes)[sc] : __ushort_as_half(0);
+    if (!w.mapped) {  // reads as zeros
+      code[j][0] = code[j][1] = 0u;
+      s[j] = __float2half2_rn(0.0f);
+    } else if (w.kv) {
+      const uint8_t* v = at + (j >> 1) * 512 + (j & 1) * 32;
+      code[j][0] = *reinterpret_cast<const uint32_t*>(v);
+      code[j][1] = *reinterpret_cast<const uint32_t*>(v + 64);
+      s[j] = *reinterpret_cast<const __half2*>(sc + j * 16);
+    } else {
+      code[j][0] = *reinterpret_cast<const uint32_t*>(at + j * 256);
+      code[j][1] = *reinterpret_cast<const uint32_t*>(at + j * 256 + 64);
+      s[j] = __halves2half2(sc[j * 16], sc[j * 16 + 4]);
     }
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    // values of tokens 2 pair and 2 pair + 1 as four (dim, dim + 1) pairs
-    __half2 v[2][4];
-    if constexpr (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value) {
+    const int tok = 4 * j + 2 * hw;
+    T* to = dst + (long long)tok * stride;
+    if constexpr (std::is_same<T, __half>::value) {
+      // both tokens' values as four (dim, dim + 1) pairs
+      __half2 v[2][4];
       if (w.kv == 0) {
+        const __half2 s0 = __low2half2(s[j]), s1 = __high2half2(s[j]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[e][i] = code_values(code[j][e], i, __half2half2(s[j][e]));
+        for (int i = 0; i < 4; ++i) {
+          v[0][i] = code_values(code[j][0], i, s0);
+          v[1][i] = code_values(code[j][1], i, s1);
+        }
       } else {
-        const __half2 s2 = __halves2half2(s[j][0], s[j][1]);
 #pragma unroll
         for (int i = 0; i < 4; i += 2)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            // one dim of both tokens each
-            const __half2 a0 = code_values(code[j][u], i, s2), a1 = code_values(code[j][u], i + 1, s2);
+          for (int u = 0; u < 2; ++u) {  // one dim of both tokens each
+            const __half2 a0 = code_values(code[j][u], i, s[j]), a1 = code_values(code[j][u], i + 1, s[j]);
             v[0][2 * u + i / 2] = __lows2half2(a0, a1);
             v[1][2 * u + i / 2] = __highs2half2(a0, a1);
           }
       }
-    }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int tok = 2 * (2 * j + hw) + e;
-      if (!w.live(tok)) continue;
-      T* at = dst + w.row(tok, a.n_tokens, a.num_kv_heads) * 128;
-      if constexpr (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value) {
-        __stcs(reinterpret_cast<uint4*>(at), *reinterpret_cast<const uint4*>(v[e]));
-      } else {
-        const float sf = __half2float(s[j][e]);
+      for (int e = 0; e < 2; ++e)
+        if (live(tok + e)) __stcs(reinterpret_cast<uint4*>(to + e * stride), *reinterpret_cast<const uint4*>(v[e]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (!live(tok + e)) continue;
+        const float sf = e ? __high2float(s[j]) : __low2float(s[j]);
         float f[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -295,10 +328,22 @@ __global__ void __launch_bounds__(256) int4_read_kernel(const PagedReadArgs a, i
                                        : (code[j][i >> 2] >> (16 * e + 4 * (i & 3))) & 15u;
           f[i] = (float)((int)n - 8) * sf;
         }
-        store8(at, f);
+        store8(to + e * stride, f);
       }
     }
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) int4_read_kernel(const PagedReadArgs a, int warps_per_seq) {
+  pdl_wait();
+  pdl_trigger();
+  const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (wid >= warps_per_seq) return;
+  BlockWork w;
+  if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid, a.status)) return;
+  if (w.whole()) read_block<T, true>(a, w);
+  else read_block<T, false>(a, w);
 }
 
 // f16 and int8 rows: one warp per (sequence, token), lanes over Hkv * D in
@@ -347,8 +392,7 @@ static int launch_read(const doe_paged_kv* kv, const PagedReadArgs& a, uint32_t 
   if (kv->kv_dtype == DOE_KV_INT4) {
     const uint64_t warps = (((uint64_t)a.n_tokens + 14) / 16 + 1) * kv->num_kv_heads * 2;
     const dim3 grid((unsigned)((warps + 7) / 8), num_seqs);
-    int4_read_kernel<T><<<grid, 256, 0, st>>>(a, (int)warps);
-    return cuda_status(cudaGetLastError(), "int4_read_kernel");
+    return cuda_status(launch_pdl(int4_read_kernel<T>, grid, dim3(256), 0, st, a, (int)warps), "int4_read_kernel");
   }
   const dim3 grid(((uint32_t)a.n_tokens + 7) / 8, num_seqs);
   if (kv->kv_dtype == DOE_KV_INT8)

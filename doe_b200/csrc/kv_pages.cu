@@ -30,6 +30,8 @@ constexpr uint32_t kPiece = kThreads * kUnroll * 16;
 template <int N>
 __global__ void __launch_bounds__(kThreads)
     copy_pages_kernel(const __grid_constant__ PagePairs<N> pairs, const PageRegions r) {
+  pdl_wait();
+  pdl_trigger();
   const uint32_t pair = blockIdx.y;
   const int32_t from = pairs.page[2 * pair], to = pairs.page[2 * pair + 1];
   uint32_t piece = blockIdx.x, region = 0;
@@ -60,8 +62,7 @@ static int launch_some(const int32_t* pairs, uint32_t n, const PageRegions& r, c
   PagePairs<N> p;
   for (uint32_t i = 0; i < 2 * n; ++i) p.page[i] = pairs[i];
   const dim3 grid(2 * (r.chunks[0] + r.chunks[1]), n);
-  copy_pages_kernel<N><<<grid, kThreads, 0, st>>>(p, r);
-  return cuda_status(cudaGetLastError(), "copy_pages_kernel");
+  return cuda_status(launch_pdl(copy_pages_kernel<N>, grid, dim3(kThreads), 0, st, p, r), "copy_pages_kernel");
 }
 
 int launch_copy_pages(const doe_paged_kv* kv, const int32_t* pairs, uint32_t n, const doe_launch* launch) {

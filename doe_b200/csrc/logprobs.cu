@@ -251,6 +251,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   __shared__ uint4 ring[kStages * Vec<T>::kUnroll * kThreads];  // every thread reads what it loaded
   using V = Vec<T>;
   constexpr int N = V::N, kUnroll = V::kUnroll;
+  pdl_wait();
+  pdl_trigger();
   const uint32_t split = blockIdx.x, tid = threadIdx.x, k = a.top_k;
   const uint64_t row = blockIdx.y;
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
@@ -521,13 +523,15 @@ int launch(const Args& a, uint64_t rows, cudaStream_t st) {
     cfg.gridDim = dim3(splits, (unsigned)n);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = splits;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = splits > 1 ? 2 : 1;
     const int rc = cuda_status(cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, b, splits), "logprobs_kernel");
     if (rc != DOE_OK) return rc;
   }

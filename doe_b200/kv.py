@@ -96,7 +96,7 @@ class KvPool:
         return out
 
 
-_KV_DTYPES = {"f16": abi.DOE_KV_F16, "int8": abi.DOE_KV_INT8, "int4": abi.DOE_KV_INT4}
+KV_DTYPES = {"f16": abi.DOE_KV_F16, "int8": abi.DOE_KV_INT8, "int4": abi.DOE_KV_INT4}
 
 
 class PagedKVCache:
@@ -106,7 +106,7 @@ class PagedKVCache:
                  block_table, kv_dtype: str = "f16", device="cuda"):
         import torch
 
-        if kv_dtype not in _KV_DTYPES:
+        if kv_dtype not in KV_DTYPES:
             raise ValueError("kv_dtype must be 'f16', 'int8' or 'int4'")
         if kv_dtype == "int4" and (head_dim != 128 or page_size % 16):
             raise ValueError("int4 pools need head_dim 128 and a page_size that is a multiple of 16")
@@ -134,7 +134,7 @@ class PagedKVCache:
         """A cache over pools (and int8 scales) that the caller holds, in the layouts above, and a
         block table on the pools' device ([sequences, pages] int32, used as it is)."""
         self = cls.__new__(cls)
-        if kv_dtype not in _KV_DTYPES:
+        if kv_dtype not in KV_DTYPES:
             raise ValueError("kv_dtype must be 'f16', 'int8' or 'int4'")
         if kv_dtype == "int4" and (head_dim != 128 or page_size % 16):
             raise ValueError("int4 pools need head_dim 128 and a page_size that is a multiple of 16")
@@ -174,7 +174,7 @@ class PagedKVCache:
             self.k_pool.data_ptr(), self.v_pool.data_ptr(),
             self.k_scale.data_ptr() if self.k_scale is not None else None,
             self.v_scale.data_ptr() if self.v_scale is not None else None,
-            _KV_DTYPES[self.kv_dtype],
+            KV_DTYPES[self.kv_dtype],
             self.num_pages, self.page_size, self.num_kv_heads, self.head_dim,
             self.max_pages_per_seq, self.block_table.data_ptr())
 

@@ -7,13 +7,14 @@ status.  Nothing here computes on the host.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 from typing import NamedTuple
 
 import numpy as np
 import torch
 
 from . import _abi as abi
-from .kv import PagedKVCache
+from .kv import KV_DTYPES, PagedKVCache
 
 _WS: dict[int, torch.Tensor] = {}
 
@@ -109,6 +110,13 @@ def stitch(partials, out=None, stream=None):
     return out
 
 
+@lru_cache(maxsize=256)
+def _decode_need(B, H, split_pages, kv_dtype, num_pages, page_size, kv_heads, head_dim, max_pages, device) -> int:
+    """doe_paged_decode_workspace_bytes, which depends on these sizes (and the device's SM count) alone."""
+    kv = abi.PagedKV(1, 1, 1, 1, KV_DTYPES[kv_dtype], num_pages, page_size, kv_heads, head_dim, max_pages, 1)
+    return int(abi.lib().doe_paged_decode_workspace_bytes(C.byref(kv), B, H, split_pages))
+
+
 def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new_v=None, out=None,
                  split_pages: int = 0, status=None, stream=None, freq_cis=None, sliding_window: int = 0,
                  softcap: float = 0.0, out_dtype=torch.float32, ws=None, inputs_stable: bool = False):
@@ -142,7 +150,8 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
         flags |= abi.DECODE_INPUTS_STABLE
     kv = cache.struct()
     lib = abi.lib()
-    need = lib.doe_paged_decode_workspace_bytes(C.byref(kv), B, H, split_pages)
+    need = _decode_need(B, H, split_pages, cache.kv_dtype, cache.num_pages, cache.page_size, cache.num_kv_heads,
+                        cache.head_dim, cache.max_pages_per_seq, q.device.index)
     if ws is None and cache.kv_dtype != "int4":
         l = _launch(need, status, stream, q.device)
     else:

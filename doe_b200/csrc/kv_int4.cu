@@ -111,13 +111,13 @@ __device__ __forceinline__ void append_block(const Int4AppendArgs& a, const Bloc
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const __half2* hx = reinterpret_cast<const __half2*>(&x[i]);
-    __half2 m2 = __hmax2(__hmax2(__habs2(hx[0]), __habs2(hx[1])), __hmax2(__habs2(hx[2]), __habs2(hx[3])));
+    __half2 m2 = __hmax2_nan(__hmax2_nan(__habs2(hx[0]), __habs2(hx[1])), __hmax2_nan(__habs2(hx[2]), __habs2(hx[3])));
     uint32_t m = *reinterpret_cast<uint32_t*>(&m2), o = __shfl_xor_sync(0xffffffffu, m, 1);
-    m2 = __hmax2(m2, *reinterpret_cast<__half2*>(&o));
+    m2 = __hmax2_nan(m2, *reinterpret_cast<__half2*>(&o));
     m = *reinterpret_cast<uint32_t*>(&m2);
     o = __shfl_xor_sync(0xffffffffu, m, 2);
-    m2 = __hmax2(m2, *reinterpret_cast<__half2*>(&o));
-    sh[i] = __float2half_rn(div7(fmaxf(__low2float(m2), __high2float(m2))));
+    m2 = __hmax2_nan(m2, *reinterpret_cast<__half2*>(&o));
+    sh[i] = __float2half_rn(div7(__half2float(__hmax_nan(__low2half(m2), __high2half(m2)))));
     s[i] = __half2float(sh[i]);
     rs[i] = inverse_of(s[i]);
     normal &= s[i] >= 0x1p-14f;

@@ -156,10 +156,6 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 __device__ __forceinline__ float2 f2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 
 // The new token's row of kv head g, written by one warp: load() right after
@@ -199,9 +195,9 @@ struct AppendRow {
                        rc, rsn, reinterpret_cast<uint32_t*>(&v));
       }
       const float2 x01 = f2(v.x), x23 = f2(v.y);
-      float amax = fmaxf(fmaxf(fabsf(x01.x), fabsf(x01.y)), fmaxf(fabsf(x23.x), fabsf(x23.y)));
+      float amax = max_nan(max_nan(fabsf(x01.x), fabsf(x01.y)), max_nan(fabsf(x23.x), fabsf(x23.y)));
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      for (int o = 4; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       const __half sh = __float2half_rn(div7(amax));
       const float s = __half2float(sh);
       const float rs = inverse_of(s);

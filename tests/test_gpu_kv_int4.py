@@ -379,3 +379,52 @@ def test_refusals():
     with pytest.raises(ValueError):
         PagedKVCache.from_pools(cache.k_pool, cache.v_pool, page_size=16, num_kv_heads=1, head_dim=128,
                                 block_table=cache.block_table.cpu(), kv_dtype="int4")
+
+
+def test_non_finite_rows_stay_non_finite():
+    """A NaN anywhere in a group makes the group's scale NaN, so it reads back as NaN; an infinity
+    reads back as infinities and NaNs.  The other groups, heads and tokens keep their values, and a
+    decode sees the NaNs exactly where the row is attended."""
+    g = np.random.default_rng(9)
+    n, Hkv = 70, 2
+    table, pages = _table(g, [n], 16)
+    k, v = _rows(g, (1, n, Hkv, 128)), _rows(g, (1, n, Hkv, 128))
+    clean = [kv_int4.values(*kv_int4.quantize(x)).astype(np.float32) for x in (k, v)]
+    k[0, 3, 0, 40] = np.nan
+    v[0, 5, 1, 127] = np.nan
+    v[0, 2, 1, 0] = -np.inf
+    k[0, 6, 1, 64] = np.inf
+    cache = PagedKVCache(num_pages=pages, page_size=16, num_kv_heads=Hkv, head_dim=128, block_table=table,
+                         kv_dtype="int4")
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.paged_append(cache, _t(k), _t(v), zero)
+    for dt in (torch.float32, torch.float16):
+        rk, rv = (x.float().cpu().numpy() for x in ops.paged_read(cache, zero, n, dtype=dt))
+        assert np.isnan(rk[0, 3, 0, 32:64]).all() and np.isnan(rv[0, 5, 1, 96:]).all()
+        assert not np.isfinite(rv[0, 2, 1, :32]).any() and not np.isfinite(rk[0, 6, 1, 64:96]).any()
+        for r, w in zip((rk, rv), clean):
+            bad = ~np.isfinite(r)
+            w = torch.from_numpy(w).to(dt).float().numpy()
+            assert bad.sum() == 64 and np.array_equal(r[~bad], w[~bad])
+    q = _t(_rows(g, (1, 8, 128)))
+    length = torch.full((1,), n, dtype=torch.int32, device="cuda")
+    out = ops.paged_decode(cache, q, length, 0.1)[0].cpu().numpy()
+    assert np.isnan(out[:4]).all() and not np.isfinite(out[4:, 96:]).any()
+    # past the window
+    out = ops.paged_decode(cache, q, length, 0.1, sliding_window=n - 7)[0].cpu().numpy()
+    ref, a = kv_int4.attend(q[0].cpu().numpy(), clean[0][0], clean[1][0], 0.1, n - 7)
+    assert (np.abs(out - ref) <= 2.0 ** -10 * (1 + 2.0 ** -4) * a + 2e-5 * np.abs(clean[1]).max()).all()
+
+
+def test_decode_appends_non_finite_rows_as_such():
+    c = Case(31, [20, 33], 2, 4)
+    cache = c.cache()
+    nk, nv = _rows(c.g, (2, 2, 128)), _rows(c.g, (2, 2, 128))
+    nk[0, 1, 33] = np.nan
+    nv[1, 0, 70] = np.nan
+    out = _decode(c, cache, new_k=_t(nk), new_v=_t(nv))
+    assert np.isnan(out[0, 4:]).all() and np.isfinite(out[0, :4]).all()
+    assert np.isnan(out[1, :4, 64:96]).all() and np.isfinite(out[1, 4:]).all()
+    k, v = (x.cpu().numpy() for x in ops.paged_read(cache, _t(c.lens - 1), 1, dtype=torch.float32))
+    assert np.isnan(k[0, 0, 1, 32:64]).all() and np.isnan(k).sum() == 32
+    assert np.isnan(v[1, 0, 0, 64:96]).all() and np.isnan(v).sum() == 32

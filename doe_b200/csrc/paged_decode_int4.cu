@@ -62,6 +62,8 @@ constexpr int kCtasPerSm = 3;                  // resident: 168 registers a thre
 constexpr int kRowCost = 4;                    // a sequence's fixed cost in the list, in blocks
 constexpr int kMinPiece = 8;                   // entries; more than kRowCost, so that no piece is empty
 constexpr uint64_t kShortRow = 128;            // blocks that one CTA walks alone when there are rows enough
+constexpr uint64_t kLoneRow = 32;              // the same, when there are few rows
+constexpr uint64_t kMinSplit = 16;             // blocks
 constexpr uint64_t kCounterBytes = 1 << 16;    // of the workspace's head, for 2048 rows' counters
 constexpr uint32_t kMaxListSeqs = 1024;        // sequences whose lengths a CTA adds up
 constexpr int kSlot = 2 * kI4Block;            // K block, V block
@@ -636,12 +638,12 @@ __device__ __forceinline__ bool arrive_last(unsigned* counter, int n) {
 
 // A running sum of parts (m, l, o): eight are loaded together, then added in order.
 struct Joined {
+  static constexpr int kBatch = 8;
   float m = kNone, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   // at(p, m l, o): the loads of part p < n
   template <typename F>
   __device__ __forceinline__ void add(int n, F&& at) {
-    constexpr int kBatch = 8;
     for (int p0 = 0; p0 < n; p0 += kBatch) {
       float2 ml[kBatch];
       float4 po[kBatch];
@@ -664,6 +666,42 @@ struct Joined {
     }
   }
 };
+
+// The last part of a (row, slice of the dims) to finish stitches them, in key order.
+// T threads take every T-th part of four dims of a head each, so that one round
+// of loads reaches all parts (one thread each: 3 of them in turn for 24 parts).
+__device__ __forceinline__ void stitch_parts(const Args& a, size_t row, int rank, int slices, int nparts, int* last) {
+  __syncthreads();
+  if (threadIdx.x == 0) *last = arrive_last(&a.counters[row * slices + rank], nparts);
+  __syncthreads();
+  if (!*last) return;
+  const int quads = kD / 4 / slices, items = a.group * quads;
+  int T = 1;
+  while (T * Joined::kBatch < nparts && 2 * T * items <= kWarps * 32) T *= 2;  // at most 32: 4 items at least
+  const int sub = threadIdx.x & (T - 1);
+  for (int i0 = 0; i0 < items; i0 += kWarps * 32 / T) {
+    const int i = i0 + threadIdx.x / T, at = min(i, items - 1);
+    const int h = at / quads, d = (rank * quads + at % quads) * 4;
+    Joined sum;
+    sum.add(sub < nparts ? (nparts - sub + T - 1) / T : 0, [&](int p, float2& ml, float4& o) {
+      const size_t from = row * a.max_parts + sub + p * T;
+      ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + (from * slices + rank) * a.group + h);
+      o = __ldcg(reinterpret_cast<const float4*>(a.part_o + (from * a.group + h) * kD + d));
+    });
+    for (int x = 1; x < T; x <<= 1) {
+      const float top = fmaxf(sum.m, __shfl_xor_sync(0xffffffffu, sum.m, x)), f = ex2(sum.m - top);
+      sum.m = top;
+      sum.l *= f;
+      sum.o = make_float4(sum.o.x * f, sum.o.y * f, sum.o.z * f, sum.o.w * f);
+      sum.l += __shfl_xor_sync(0xffffffffu, sum.l, x);
+      sum.o.x += __shfl_xor_sync(0xffffffffu, sum.o.x, x);
+      sum.o.y += __shfl_xor_sync(0xffffffffu, sum.o.y, x);
+      sum.o.z += __shfl_xor_sync(0xffffffffu, sum.o.z, x);
+      sum.o.w += __shfl_xor_sync(0xffffffffu, sum.o.w, x);
+    }
+    if (sub == 0 && i < items) store_out(a, row * a.group + h, d, sum.o, sum.l);
+  }
+}
 
 // ---- few rows: one CTA per split --------------------------------------------------
 template <bool CAP>
@@ -764,24 +802,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) splits_kernel(const A
               make_float2(sum.m, sum.l);
       }
     }
-    cluster.sync();  // the others have read this CTA's part
+    cluster.sync();  // this CTA has read the others' parts
   }
-  if (nparts == 1) return;
-  // ---- the last part of a (row, slice) to finish stitches them, in key order ---------
-  __syncthreads();
-  if (threadIdx.x == 0) sm_last = arrive_last(&a.counters[row * slices + rank], nparts);
-  __syncthreads();
-  if (!sm_last) return;
-  for (int i = threadIdx.x; i < group * quads; i += kWarps * 32) {
-    const int h = i / quads, d = (rank * quads + i % quads) * 4;
-    Joined sum;
-    sum.add(nparts, [&](int p, float2& ml, float4& o) {
-      const size_t from = row * a.max_parts + p;
-      ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + (from * slices + rank) * group + h);
-      o = __ldcg(reinterpret_cast<const float4*>(a.part_o + (from * group + h) * kD + d));
-    });
-    store_out(a, row * group + h, d, sum.o, sum.l);
-  }
+  if (nparts > 1) stitch_parts(a, row, rank, slices, nparts, &sm_last);
 }
 
 // ---- many rows: pieces of one list, a warp each -------------------------------------
@@ -1051,10 +1074,10 @@ Plan plan(uint64_t num_seqs, uint64_t kv_heads, uint64_t max_tiles, uint64_t til
     }
     t = tiles;
   } else if (t == 0) {
-    const uint64_t fill = (2 * sms + rows - 1) / rows;
+    const uint64_t fill = (sms * 5 / 2 + rows - 1) / rows;
     p.slots = rows * fill;
-    t = rows >= sms && tiles <= kShortRow ? tiles : (tiles + fill - 1) / fill;
-    if (t < 8) t = 8;
+    t = tiles <= (rows >= sms ? kShortRow : kLoneRow) ? tiles : (tiles + fill - 1) / fill;
+    if (t < kMinSplit) t = kMinSplit;
   } else {
     p.slots = rows * ((max_tiles + t - 1) / t);
   }

@@ -90,6 +90,19 @@ struct Vec<float> {
                   : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
   }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
+  // A bit per element above `bound`, and the element (of the thread's N kUnroll) of a bit.
+  static __device__ __forceinline__ uint32_t above(const uint4 (&raw)[kUnroll], float bound) {
+    uint32_t hits = 0;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float2 f = pair(raw[u], i / 2);
+        hits |= (f.x > bound ? 1u << (u * N + i) : 0u) | (f.y > bound ? 2u << (u * N + i) : 0u);
+      }
+    return hits;
+  }
+  static __device__ __forceinline__ uint32_t element(uint32_t bit) { return bit; }
 };
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
   return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w));
@@ -108,6 +121,18 @@ struct Vec<__half> {
     return fmaxf(f.x, f.y);
   }
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+  // `bound` is an element's value, so the conversion is exact; bits 0-15 are the words' low halves
+  static __device__ __forceinline__ uint32_t above(const uint4 (&raw)[kUnroll], float bound) {
+    const __half2 b = __float2half2_rn(bound);
+    uint32_t hits = 0;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        hits |= __hgt2_mask(reinterpret_cast<const __half2*>(&raw[u])[i], b) & (0x00010001u << (4 * u + i));
+    return hits;
+  }
+  static __device__ __forceinline__ uint32_t element(uint32_t bit) { return 2 * (bit & 15) + (bit >> 4); }
 };
 template <>
 struct Vec<__nv_bfloat16> {
@@ -123,6 +148,18 @@ struct Vec<__nv_bfloat16> {
     return fmaxf(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  // `bound` is an element's value, so the conversion is exact; bits 0-15 are the words' low halves
+  static __device__ __forceinline__ uint32_t above(const uint4 (&raw)[kUnroll], float bound) {
+    const __nv_bfloat162 b = __float2bfloat162_rn(bound);
+    uint32_t hits = 0;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        hits |= __hgt2_mask(reinterpret_cast<const __nv_bfloat162*>(&raw[u])[i], b) & (0x00010001u << (4 * u + i));
+    return hits;
+  }
+  static __device__ __forceinline__ uint32_t element(uint32_t bit) { return 2 * (bit & 15) + (bit >> 4); }
 };
 
 // Running (m, s, w), w in log2 units; m = -inf: nothing but -inf seen.
@@ -275,46 +312,22 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   Stat st = {-INFINITY, 0.0f, 0.0f};
   float tmax = -INFINITY, bound = -INFINITY;
   uint32_t step = 0;
-  // This thread's elements above the bound go into the buffer, one reservation per
-  // warp.  Returns the threads whose elements did not all fit: none of theirs are
-  // taken, and their places stay empty.
-  auto push = [&](const uint4 (&raw)[kUnroll], uint32_t at, float bound, bool mine) {
-    uint32_t hits = 0;
-    if (mine) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-          const float2 f = V::pair(raw[u], i / 2);
-          hits |= (f.x > bound ? 1u : 0u) << (u * N + i) | (f.y > bound ? 2u : 0u) << (u * N + i);
-        }
+  // This thread's elements above the bound (there are some) go into the buffer.  Their
+  // values are read back from the ring's slot, where a run-time index costs nothing.
+  // True: they did not all fit; none are taken, and their places stay empty.
+  auto push = [&](const uint4 (&raw)[kUnroll], uint32_t at, uint32_t slot, float bound) {
+    uint32_t hits = V::above(raw, bound), pos = atomicAdd(&sh.count, __popc(hits));
+    const bool lost = pos + __popc(hits) > kCap;
+    for (; hits != 0; hits &= hits - 1, ++pos) {
+      const uint32_t e = V::element(__ffs(hits) - 1), u = e / N, i = e % N;
+      const float v = V::one(reinterpret_cast<const T*>(&ring[(slot * kUnroll + u) * kThreads + tid]) + i);
+      const uint64_t j = (uint64_t)(at + u * kThreads + tid) * N + i - shift;
+      if (pos < kCap) sh.buf[pos] = lost ? 0ull : key_of(v, (uint32_t)j);
     }
-    const uint32_t some = __popc(hits);
-    uint32_t upto = some;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
-      if ((tid & 31) >= o) upto += up;
-    }
-    uint32_t pos = 0;
-    if ((tid & 31) == 31 && upto != 0) pos = atomicAdd(&sh.count, upto);
-    pos = __shfl_sync(0xffffffffu, pos, 31) + upto - some;
-    const bool lost = pos + some > kCap && some != 0;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (hits >> (u * N) & ((1u << N) - 1))
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (hits >> (u * N + i) & 1) {
-            const float2 f = V::pair(raw[u], i / 2);
-            const uint64_t j = (uint64_t)(at + u * kThreads + tid) * N + i - shift;
-            if (pos < kCap) sh.buf[pos] = lost ? 0ull : key_of((i & 1) ? f.y : f.x, (uint32_t)j);
-            ++pos;
-          }
     return lost;
   };
   // An edge vector, element by element: those outside the row are -inf.
-  auto edge = [&](uint32_t at, uint4 (&raw)[kUnroll]) {
+  auto edge = [&](uint32_t at, uint32_t slot, uint4 (&raw)[kUnroll]) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const uint32_t v = at + u * kThreads + tid;
@@ -327,6 +340,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
           e[i] = j >= shift && j < (uint64_t)shift + a.vocab ? x[j - shift] : reinterpret_cast<const T*>(&low)[i];
         }
         memcpy(&raw[u], e, 16);
+        ring[(slot * kUnroll + u) * kThreads + tid] = raw[u];
       }
     }
   };
@@ -350,12 +364,13 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
     load(at + (kStages - 1) * kStep, (step + kStages - 1) % kStages);
     asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 1) : "memory");
     uint4 raw[kUnroll];
+    const uint32_t slot = step % kStages;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       raw[u] = make_uint4(V::kLow, V::kLow, V::kLow, V::kLow);
-      if (inside(at + u * kThreads + tid)) raw[u] = ring[((step % kStages) * kUnroll + u) * kThreads + tid];
+      if (inside(at + u * kThreads + tid)) raw[u] = ring[(slot * kUnroll + u) * kThreads + tid];
     }
-    if (at < whole0 || at + kStep > whole1) edge(at, raw);
+    if (at < whole0 || at + kStep > whole1) edge(at, slot, raw);
     float vmax = V::max(raw[0]);
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u) vmax = fmaxf(vmax, V::max(raw[u]));
@@ -377,8 +392,9 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
     if (k == 0) continue;
     tmax = fmaxf(tmax, vmax);
     if (step == 0) bound = group_bound(sh, tmax, k);
-    if (__any_sync(0xffffffffu, vmax > bound) && push(raw, at, bound, true)) sh.full = 1;
-    if ((step & (step + 1)) == 0 && (step + 1 & 0x55555555u) != 0) {  // 1st, 4th, 16th, ... step
+    if (vmax > bound && push(raw, at, slot, bound)) sh.full = 1;
+    // 1st, 4th, 16th, ... step, but not the last
+    if ((step & (step + 1)) == 0 && (step + 1 & 0x55555555u) != 0 && at + kStep < v1) {
       __syncthreads();
       const uint32_t n = sh.count;
       const bool full = sh.full != 0;
@@ -398,16 +414,16 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
       for (int u = 0; u < kUnroll; ++u) {
         raw[u] = make_uint4(V::kLow, V::kLow, V::kLow, V::kLow);
         if (inside(at + u * kThreads + tid)) raw[u] = ldg_stream(base + at + u * kThreads + tid);
+        ring[u * kThreads + tid] = raw[u];
       }
-      if (at < whole0 || at + kStep > whole1) edge(at, raw);
+      if (at < whole0 || at + kStep > whole1) edge(at, 0, raw);
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) vmax = fmaxf(vmax, V::max(raw[u]));
       tmax = fmaxf(tmax, vmax);
       if (at == v0) bound = group_bound(sh, tmax, k);
       bool todo = true;
       for (int round = 0;; ++round) {
-        if (__any_sync(0xffffffffu, todo && vmax > bound)) todo = push(raw, at, bound, todo);
-        else todo = false;
+        todo = todo && vmax > bound && push(raw, at, 0, bound);
         if (!__syncthreads_or(todo)) break;
         if (round == 0) {  // a new bound
           bound = fmaxf(bound, group_bound(sh, tmax, k));

@@ -36,13 +36,6 @@ __device__ __forceinline__ float div7(float amax) {
   const float q0 = amax * kInv7;
   return fmaf(fmaf(-q0, 7.0f, amax), kInv7, q0);
 }
-// The larger of two, NaN if either is: a NaN makes its group's scale NaN, so the
-// group reads back as NaN.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 // About 1 / s, and 0 for 0 (so that a row of zeros gets the code of 0).
 __device__ __forceinline__ float inverse_of(float s) {
   float r;

@@ -104,7 +104,7 @@ __device__ __forceinline__ void append_block(const Int4AppendArgs& a, const Bloc
     }
   }
   // scales of all rows first; the codes' two forms (see quantize_u4x2) then differ
-  // once per warp
+  // once per warp.  A NaN makes its group's scale NaN, so the group reads back as NaN
   float s[8], rs[8];
   __half sh[8];
   bool normal = true;

@@ -75,7 +75,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 16 bytes of logits: N elements, two per step of each().
+// 16 bytes of logits: N elements.  Floor: what elements are raised to, see lowest().
 template <typename T>
 struct Vec;
 template <>
@@ -90,6 +90,12 @@ struct Vec<float> {
                   : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
   }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
+  using Floor = float;
+  static __device__ __forceinline__ Floor floor_of(float v) { return v; }
+  static __device__ __forceinline__ float2 pair_over(const uint4& v, int i, Floor f) {
+    const float2 x = pair(v, i);
+    return make_float2(max_nan(x.x, f), max_nan(x.y, f));
+  }
   // A bit per element above `bound`, and the element (of the thread's N kUnroll) of a bit.
   static __device__ __forceinline__ uint32_t above(const uint4 (&raw)[kUnroll], float bound) {
     uint32_t hits = 0;
@@ -121,6 +127,13 @@ struct Vec<__half> {
     return fmaxf(f.x, f.y);
   }
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+  using Floor = __half2;
+  static __device__ __forceinline__ Floor floor_of(float v) { return __half2half2(__float2half_rd(v)); }
+  static __device__ __forceinline__ float2 pair_over(const uint4& v, int i, Floor f) {
+    const uint32_t w = word(v, i);
+    const __half2 x = __hmax2_nan(*reinterpret_cast<const __half2*>(&w), f);
+    return __half22float2(x);
+  }
   // `bound` is an element's value, so the conversion is exact; bits 0-15 are the words' low halves
   static __device__ __forceinline__ uint32_t above(const uint4 (&raw)[kUnroll], float bound) {
     const __half2 b = __float2half2_rn(bound);
@@ -148,6 +161,13 @@ struct Vec<__nv_bfloat16> {
     return fmaxf(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  using Floor = __nv_bfloat162;
+  static __device__ __forceinline__ Floor floor_of(float v) { return __bfloat162bfloat162(__float2bfloat16_rd(v)); }
+  static __device__ __forceinline__ float2 pair_over(const uint4& v, int i, Floor f) {
+    const uint32_t w = word(v, i);
+    const __nv_bfloat162 x = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w), f);
+    return pair(make_uint4(*reinterpret_cast<const uint32_t*>(&x), 0, 0, 0), 0);
+  }
   // `bound` is an element's value, so the conversion is exact; bits 0-15 are the words' low halves
   static __device__ __forceinline__ uint32_t above(const uint4 (&raw)[kUnroll], float bound) {
     const __nv_bfloat162 b = __float2bfloat162_rn(bound);
@@ -162,26 +182,40 @@ struct Vec<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t element(uint32_t bit) { return 2 * (bit & 15) + (bit >> 4); }
 };
 
-// Running (m, s, w), w in log2 units; m = -inf: nothing but -inf seen.
+// Running sums over elements x of d = (x - m) log2(e) + excess(m): s = sum 2^d and
+// w = sum d 2^d.  m = -inf: nothing but -inf (and NaN, which s counts) seen.
 struct Stat {
   float m, s, w;
 };
+// Up to this |m| the exponent is one fma, x log2(e) - R with R = m log2(e) rounded;
+// its difference from (x - m) log2(e) is known.  Beyond, and for the type's lowest
+// value, whose product overflows, x - m is taken first.
+constexpr float kFused = 6e4f;  // lowest() is then above f16's lowest value, and excess() below 2^-8
+__device__ __forceinline__ float excess(float m) { return fabsf(m) < kFused ? fmaf(m, kLog2e, -(m * kLog2e)) : 0.0f; }
+// Elements below add nothing to sums over m; raised to this they add 0 d, not 0 * inf.
+// Far enough below m in any of the types.
+__device__ __forceinline__ float lowest(float m) { return m - fmaxf(150.0f, fabsf(m) * 0x1p-6f); }
 __device__ __forceinline__ void raise(Stat& a, float m) {
   if (a.m == -INFINITY) {  // a.s counts only NaN so far
     a.w = a.s;
   } else {
-    const float d = fmaxf((a.m - m) * kLog2e, -200.0f), c = ex2(d);  // 2^-200 is 0
+    const float d = fmaxf(fmaf(a.m - m, kLog2e, excess(m) - excess(a.m)), -200.0f), c = ex2(d);  // 2^-200 is 0
     a.w = c * fmaf(d, a.s, a.w);
     a.s *= c;
   }
   a.m = m;
 }
-__device__ __forceinline__ Stat merge(Stat a, Stat b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s, a.w + b.w};
+// Largest value of the warp's lanes.
+__device__ __forceinline__ float redux_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;\n" : "=f"(r) : "f"(v));
+  return r;
+}
+// The sum of all lanes' (a lane without one has {-inf, 0, 0}), on every lane.
+__device__ __forceinline__ Stat warp_merge(Stat a) {
+  const float m = redux_max(a.m);
   if (a.m != m) raise(a, m);
-  if (b.m != m) raise(b, m);
-  return {m, a.s + b.s, a.w + b.w};
+  return {m, warp_sum(a.s), warp_sum(a.w)};
 }
 
 struct Shared {
@@ -309,7 +343,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
     token = a.tokens[row];
     if ((uint32_t)token < a.vocab) given = V::one(x + token);
   }
-  Stat st = {-INFINITY, 0.0f, 0.0f};
+  Stat st = {-INFINITY, 0.0f, 0.0f};  // m is the warp's
+  typename V::Floor floor = V::floor_of(0.0f);
   float tmax = -INFINITY, bound = -INFINITY;
   uint32_t step = 0;
   // This thread's elements above the bound (there are some) go into the buffer.  Their
@@ -374,19 +409,34 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
     float vmax = V::max(raw[0]);
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u) vmax = fmaxf(vmax, V::max(raw[u]));
-    if (vmax > st.m) raise(st, vmax);
-    const float neg_m = st.m == -INFINITY ? 0.0f : -st.m;
+    if (__any_sync(0xffffffffu, vmax > st.m)) {  // one m for the warp
+      raise(st, redux_max(fmaxf(vmax, st.m)));
+      floor = V::floor_of(lowest(st.m));
+    }
     float2 s2 = make_float2(st.s, 0.0f), w2 = make_float2(st.w, 0.0f);
+    if (fabsf(st.m) < kFused) {
+      const float2 minus_r = make_float2(-(st.m * kLog2e), -(st.m * kLog2e));
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+      for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        const float2 d = fmul2(fadd2(V::pair(raw[u], i), make_float2(neg_m, neg_m)), make_float2(kLog2e, kLog2e));
-        const float2 p = make_float2(ex2(d.x), ex2(d.y));
-        s2 = fadd2(s2, p);
-        // clamped: a masked element adds 0 to w, not 0 * inf
-        w2 = ffma2(p, make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f)), w2);
-      }
+        for (int i = 0; i < N / 2; ++i) {
+          const float2 d = ffma2(V::pair_over(raw[u], i, floor), make_float2(kLog2e, kLog2e), minus_r);
+          const float2 p = make_float2(ex2(d.x), ex2(d.y));
+          s2 = fadd2(s2, p);
+          w2 = ffma2(p, d, w2);
+        }
+    } else {
+      const float neg_m = st.m == -INFINITY ? 0.0f : -st.m;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          const float2 d = fmul2(fadd2(V::pair(raw[u], i), make_float2(neg_m, neg_m)), make_float2(kLog2e, kLog2e));
+          const float2 p = make_float2(ex2(d.x), ex2(d.y));
+          s2 = fadd2(s2, p);
+          w2 = ffma2(p, make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f)), w2);
+        }
+    }
     st.s = s2.x + s2.y;
     st.w = w2.x + w2.y;
     if (k == 0) continue;
@@ -436,15 +486,16 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   }
 
   // ---- the CTA's statistics and best k -------------------------------------
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Stat b = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                    __shfl_xor_sync(0xffffffffu, st.w, o)};
-    st = merge(st, b);
-  }
+  st.s = warp_sum(st.s);
+  st.w = warp_sum(st.w);
   if ((tid & 31) == 0) sh.stat[tid >> 5] = st;
+  __syncthreads();
+  if (tid >= kThreads - 32) {  // the warp that select() needs least
+    const uint32_t lane = tid & 31;
+    st = warp_merge(lane < kWarps ? sh.stat[lane] : Stat{-INFINITY, 0.0f, 0.0f});
+    if (lane == 0) sh.total = st;
+  }
   if (k != 0) {
-    __syncthreads();
     uint32_t n = sh.count;
     select(sh, n, k);
     if (n < k) {
@@ -471,25 +522,18 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
       }
     }
   }
-  __syncthreads();
-  if (tid == 0) {
-    Stat t = sh.stat[0];
-    for (int i = 1; i < kWarps; ++i) t = merge(t, sh.stat[i]);
-    sh.total = t;
-  }
   if (splits > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();  // every CTA's total and sel
     if (split == 0) {
-      Stat t = sh.total;
-      for (uint32_t i = 1; i < splits; ++i) t = merge(t, *cluster.map_shared_rank(&sh.total, i));
       unsigned long long key = 0;
       if (k != 0 && tid < splits * k) key = cluster.map_shared_rank(sh.sel, tid / k)[tid % k];
-      __syncthreads();
-      if (tid == 0) {
-        sh.total = t;
-        sh.count = 0;
+      if (tid >= kThreads - 32) {
+        const uint32_t lane = tid & 31;
+        st = warp_merge(lane < splits ? *cluster.map_shared_rank(&sh.total, lane) : Stat{-INFINITY, 0.0f, 0.0f});
+        if (lane == 0) sh.total = st;
       }
+      if (tid == 0) sh.count = 0;
       __syncthreads();
       if (key != 0) sh.buf[atomicAdd(&sh.count, 1u)] = key;
       __syncthreads();
@@ -501,13 +545,13 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   __syncthreads();
   const Stat t = sh.total;
   const bool none = t.s == 0.0f;  // every element is -inf
-  const float ls = logf(t.s);
+  const float log2s = log2f(t.s), ls = (log2s - excess(t.m)) * kLn2;
   if (tid == 0) {
     if (a.logprob != nullptr) {
       if ((uint32_t)token >= a.vocab) report(a.status, DOE_DEVICE_ERR_POSITION);
       a.logprob[row] = none || (uint32_t)token >= a.vocab ? -INFINITY : given - t.m - ls;
     }
-    if (a.entropy != nullptr) a.entropy[row] = none ? 0.0f : ls - t.w / t.s * kLn2;
+    if (a.entropy != nullptr) a.entropy[row] = none ? 0.0f : (log2s - t.w / t.s) * kLn2;
   }
   if (tid < k) {
     const unsigned long long key = sh.sel[tid];

@@ -175,3 +175,17 @@ def test_refusals():
         ops.token_logprobs(x, torch.zeros(2, dtype=torch.int32, device="cuda"))
     with pytest.raises(RuntimeError):
         ops.token_logprobs(x, top_k=33)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_maxima_on_both_sides_of_the_exponents_two_forms(dtype, sign):
+    """Largest logits just below and above 60000 in different parts of a row, some masked."""
+    g = np.random.default_rng(4)
+    x = g.standard_normal((4, 70001)) * 3 + sign * 59999.0
+    x[1] += 3.0
+    x[2, ::3] = -np.inf
+    x[3, 5:] = -np.inf
+    x = torch.from_numpy(x.astype(np.float32)).to(DTYPES[dtype]).cuda()
+    assert torch.isfinite(x[0]).all()
+    _check(x, [0, 1, 4, 3], 7)

@@ -221,7 +221,8 @@ __device__ __forceinline__ Stat warp_merge(Stat a) {
 struct Shared {
   unsigned long long buf[kCap];
   unsigned long long sel[kMaxTop];  // the CTA's best k, in order
-  float group_max[32];
+  alignas(16) float group_max[32];
+  float bound;
   Stat stat[kWarps];
   uint32_t hits[kWarps];
   Stat total;
@@ -252,8 +253,7 @@ __device__ void sort_keys(Shared& sh, uint32_t n) {
 
 // The best k of buf[0, n) into sel, in order (zeros when n < k).  Ends synchronised.
 __device__ void select(Shared& sh, uint32_t n, uint32_t k) {
-  if (threadIdx.x < kMaxTop) sh.sel[threadIdx.x] = 0;
-  __syncthreads();
+  if (threadIdx.x >= n && threadIdx.x < k) sh.sel[threadIdx.x] = 0;
   if (n <= kThreads) {  // keys differ, so a key's rank is the number of larger ones
     if (threadIdx.x < n) {
       const unsigned long long mine = sh.buf[threadIdx.x];
@@ -274,20 +274,24 @@ __device__ void select(Shared& sh, uint32_t n, uint32_t k) {
 __device__ float group_bound(Shared& sh, float tmax, uint32_t k) {
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, o));
-  if ((threadIdx.x & 7) == 0) sh.group_max[threadIdx.x >> 3] = tmax;
+  const uint32_t tid = threadIdx.x;
+  if ((tid & 7) == 0) sh.group_max[tid >> 3] = tmax;
   __syncthreads();
-  const uint32_t lane = threadIdx.x & 31;
-  const float mine = sh.group_max[lane];
-  uint32_t rank = 0;
-#pragma unroll 8
-  for (uint32_t i = 0; i < 32; ++i) {
-    const float other = sh.group_max[i];
-    rank += other > mine || (other == mine && i < lane);
+  if (tid < 32) {
+    const float mine = sh.group_max[tid];
+    uint32_t rank = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 32; i += 4) {
+      const float4 other = *reinterpret_cast<const float4*>(&sh.group_max[i]);
+      rank += other.x > mine || (other.x == mine && i < tid);
+      rank += other.y > mine || (other.y == mine && i + 1 < tid);
+      rank += other.z > mine || (other.z == mine && i + 2 < tid);
+      rank += other.w > mine || (other.w == mine && i + 3 < tid);
+    }
+    if (rank == k - 1) sh.bound = mine;
   }
-  const uint32_t at = __ballot_sync(0xffffffffu, rank == k - 1);
-  const float bound = __shfl_sync(0xffffffffu, mine, __ffs(at) - 1);
   __syncthreads();
-  return bound;
+  return sh.bound;
 }
 
 // Drops the candidates that are not above `bound`; the others stay, in any order.
@@ -335,7 +339,6 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   const uint32_t v0 = min(nvec, split * per), v1 = min(nvec, v0 + per);
   const uint32_t whole0 = shift ? 1 : 0, whole1 = (uint32_t)(((uint64_t)shift + a.vocab) / N);  // vectors within the row
   if (tid == 0) sh.count = sh.full = 0;
-  __syncthreads();
 
   int32_t token = -1;
   float given = -INFINITY;  // the given token's logit
@@ -356,8 +359,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
     for (; hits != 0; hits &= hits - 1, ++pos) {
       const uint32_t e = V::element(__ffs(hits) - 1), u = e / N, i = e % N;
       const float v = V::one(reinterpret_cast<const T*>(&ring[(slot * kUnroll + u) * kThreads + tid]) + i);
-      const uint64_t j = (uint64_t)(at + u * kThreads + tid) * N + i - shift;
-      if (pos < kCap) sh.buf[pos] = lost ? 0ull : key_of(v, (uint32_t)j);
+      if (pos < kCap) sh.buf[pos] = lost ? 0ull : key_of(v, (at + u * kThreads + tid) * N + i - shift);
     }
     return lost;
   };
@@ -381,11 +383,14 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   };
   constexpr uint32_t kStep = kThreads * kUnroll;  // vectors
   auto inside = [&](uint32_t v) { return v < v1 && v >= whole0 && v < whole1; };
+  const uint32_t end = min(v1, whole1);
+  auto all_inside = [&](uint32_t at) { return at >= whole0 && at + kStep <= end; };
   auto load = [&](uint32_t at, uint32_t slot) {
+    const bool all = all_inside(at);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const uint32_t v = at + u * kThreads + tid;
-      if (inside(v))
+      if (all || inside(v))
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(
                          (uint32_t)__cvta_generic_to_shared(&ring[(slot * kUnroll + u) * kThreads + tid])),
                      "l"(base + v)
@@ -401,11 +406,13 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
     uint4 raw[kUnroll];
     const uint32_t slot = step % kStages;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      raw[u] = make_uint4(V::kLow, V::kLow, V::kLow, V::kLow);
-      if (inside(at + u * kThreads + tid)) raw[u] = ring[(slot * kUnroll + u) * kThreads + tid];
+    for (int u = 0; u < kUnroll; ++u) raw[u] = ring[(slot * kUnroll + u) * kThreads + tid];
+    if (!all_inside(at)) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (!inside(at + u * kThreads + tid)) raw[u] = make_uint4(V::kLow, V::kLow, V::kLow, V::kLow);
+      edge(at, slot, raw);
     }
-    if (at < whole0 || at + kStep > whole1) edge(at, slot, raw);
     float vmax = V::max(raw[0]);
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u) vmax = fmaxf(vmax, V::max(raw[u]));
@@ -447,13 +454,15 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
     if ((step & (step + 1)) == 0 && (step + 1 & 0x55555555u) != 0 && at + kStep < v1) {
       __syncthreads();
       const uint32_t n = sh.count;
-      const bool full = sh.full != 0;
-      __syncthreads();  // before the next candidates are counted
-      if (n > k && !full) cut(sh, n, k, bound);
+      if (n > k && sh.full == 0) cut(sh, n, k, bound);
+      else __syncthreads();  // before the next candidates are counted
     }
   }
+  st.s = warp_sum(st.s);
+  st.w = warp_sum(st.w);
+  if ((tid & 31) == 0) sh.stat[tid >> 5] = st;
   __syncthreads();
-  if (sh.full) {
+  if (k != 0 && sh.full) {
     __syncthreads();
     if (tid == 0) sh.count = 0;
     bound = tmax = -INFINITY;
@@ -486,10 +495,6 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   }
 
   // ---- the CTA's statistics and best k -------------------------------------
-  st.s = warp_sum(st.s);
-  st.w = warp_sum(st.w);
-  if ((tid & 31) == 0) sh.stat[tid >> 5] = st;
-  __syncthreads();
   if (tid >= kThreads - 32) {  // the warp that select() needs least
     const uint32_t lane = tid & 31;
     st = warp_merge(lane < kWarps ? sh.stat[lane] : Stat{-INFINITY, 0.0f, 0.0f});
@@ -541,8 +546,9 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
     }
     cluster.sync();
     if (split != 0) return;
+  } else if (k == 0) {
+    __syncthreads();  // select() ends with one
   }
-  __syncthreads();
   const Stat t = sh.total;
   const bool none = t.s == 0.0f;  // every element is -inf
   const float log2s = log2f(t.s), ls = (log2s - excess(t.m)) * kLn2;

@@ -42,6 +42,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
+constexpr int kMaxSplits = 8;
 constexpr int kCap = 1024;    // candidate buffer (a power of two)
 constexpr uint32_t kStages = 4;  // steps in the ring
 constexpr float kLn2 = 0.6931471805599453f;
@@ -219,52 +220,56 @@ __device__ __forceinline__ Stat warp_merge(Stat a) {
 }
 
 struct Shared {
-  unsigned long long buf[kCap];
+  alignas(16) unsigned long long buf[kCap];
+  alignas(16) unsigned long long joined[kMaxSplits * kMaxTop];  // first CTA of a cluster: all CTAs' best k
   unsigned long long sel[kMaxTop];  // the CTA's best k, in order
   alignas(16) float group_max[32];
   float bound;
   Stat stat[kWarps];
   uint32_t hits[kWarps];
-  Stat total;
+  Stat totals[kMaxSplits];  // first CTA of a cluster: of all CTAs
   uint32_t count;
   uint32_t full;  // candidates were lost
 };
 
 // Sorts buf[0, n) descending; n is padded to a power of two with zeros.
-__device__ void sort_keys(Shared& sh, uint32_t n) {
+__device__ void sort_keys(unsigned long long* buf, uint32_t n) {
   uint32_t p = 2;
   while (p < n) p <<= 1;
-  for (uint32_t i = n + threadIdx.x; i < p; i += kThreads) sh.buf[i] = 0;
+  for (uint32_t i = n + threadIdx.x; i < p; i += kThreads) buf[i] = 0;
   __syncthreads();
   for (uint32_t size = 2; size <= p; size <<= 1)
     for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
       for (uint32_t i = threadIdx.x; i < p / 2; i += kThreads) {
         const uint32_t lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
         const bool down = (lo & size) == 0;
-        const unsigned long long x = sh.buf[lo], y = sh.buf[hi];
+        const unsigned long long x = buf[lo], y = buf[hi];
         if ((x < y) == down) {
-          sh.buf[lo] = y;
-          sh.buf[hi] = x;
+          buf[lo] = y;
+          buf[hi] = x;
         }
       }
       __syncthreads();
     }
 }
 
-// The best k of buf[0, n) into sel, in order (zeros when n < k).  Ends synchronised.
-__device__ void select(Shared& sh, uint32_t n, uint32_t k) {
+// The best k of buf[0, n), all different, into sel, in order (zeros when n < k).  buf
+// has room for n rounded up to a power of two.  Ends synchronised.
+__device__ void select(Shared& sh, unsigned long long* buf, uint32_t n, uint32_t k) {
   if (threadIdx.x >= n && threadIdx.x < k) sh.sel[threadIdx.x] = 0;
-  if (n <= kThreads) {  // keys differ, so a key's rank is the number of larger ones
+  if (n <= kThreads) {  // a key's rank is the number of larger ones
     if (threadIdx.x < n) {
-      const unsigned long long mine = sh.buf[threadIdx.x];
+      const unsigned long long mine = buf[threadIdx.x];
       uint32_t rank = 0;
+      const ulonglong2* two = reinterpret_cast<const ulonglong2*>(buf);
 #pragma unroll 8
-      for (uint32_t i = 0; i < n; ++i) rank += sh.buf[i] > mine;
+      for (uint32_t i = 0; i < n / 2; ++i) rank += (two[i].x > mine) + (two[i].y > mine);
+      if (n & 1) rank += buf[n - 1] > mine;
       if (rank < k) sh.sel[rank] = mine;
     }
   } else {
-    sort_keys(sh, n);
-    if (threadIdx.x < k) sh.sel[threadIdx.x] = sh.buf[threadIdx.x];
+    sort_keys(buf, n);
+    if (threadIdx.x < k) sh.sel[threadIdx.x] = buf[threadIdx.x];
   }
   __syncthreads();
 }
@@ -274,24 +279,20 @@ __device__ void select(Shared& sh, uint32_t n, uint32_t k) {
 __device__ float group_bound(Shared& sh, float tmax, uint32_t k) {
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, o));
-  const uint32_t tid = threadIdx.x;
-  if ((tid & 7) == 0) sh.group_max[tid >> 3] = tmax;
+  if ((threadIdx.x & 7) == 0) sh.group_max[threadIdx.x >> 3] = tmax;
   __syncthreads();
-  if (tid < 32) {
-    const float mine = sh.group_max[tid];
-    uint32_t rank = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < 32; i += 4) {
-      const float4 other = *reinterpret_cast<const float4*>(&sh.group_max[i]);
-      rank += other.x > mine || (other.x == mine && i < tid);
-      rank += other.y > mine || (other.y == mine && i + 1 < tid);
-      rank += other.z > mine || (other.z == mine && i + 2 < tid);
-      rank += other.w > mine || (other.w == mine && i + 3 < tid);
-    }
-    if (rank == k - 1) sh.bound = mine;
+  const uint32_t lane = threadIdx.x & 31;
+  const float mine = sh.group_max[lane];
+  uint32_t rank = 0;
+#pragma unroll 8
+  for (uint32_t i = 0; i < 32; ++i) {
+    const float other = sh.group_max[i];
+    rank += other > mine || (other == mine && i < lane);
   }
+  const uint32_t at = __ballot_sync(0xffffffffu, rank == k - 1);
+  const float bound = __shfl_sync(0xffffffffu, mine, __ffs(at) - 1);
   __syncthreads();
-  return sh.bound;
+  return bound;
 }
 
 // Drops the candidates that are not above `bound`; the others stay, in any order.
@@ -313,7 +314,7 @@ __device__ void filter(Shared& sh, float bound) {
 
 // Keeps the best k of n >= k candidates; the last of them is the new bound.
 __device__ void cut(Shared& sh, uint32_t n, uint32_t k, float& bound) {
-  select(sh, n, k);
+  select(sh, sh.buf, n, k);
   if (threadIdx.x < k) sh.buf[threadIdx.x] = sh.sel[threadIdx.x];
   if (threadIdx.x == 0) sh.count = k;
   bound = fmaxf(bound, value_of(sh.sel[k - 1]));
@@ -339,13 +340,6 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   const uint32_t v0 = min(nvec, split * per), v1 = min(nvec, v0 + per);
   const uint32_t whole0 = shift ? 1 : 0, whole1 = (uint32_t)(((uint64_t)shift + a.vocab) / N);  // vectors within the row
   if (tid == 0) sh.count = sh.full = 0;
-
-  int32_t token = -1;
-  float given = -INFINITY;  // the given token's logit
-  if (split == 0 && tid == 0 && a.tokens != nullptr) {
-    token = a.tokens[row];
-    if ((uint32_t)token < a.vocab) given = V::one(x + token);
-  }
   Stat st = {-INFINITY, 0.0f, 0.0f};  // m is the warp's
   typename V::Floor floor = V::floor_of(0.0f);
   float tmax = -INFINITY, bound = -INFINITY;
@@ -400,6 +394,13 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   };
 #pragma unroll
   for (uint32_t i = 0; i < kStages - 1; ++i) load(v0 + i * kStep, i);
+  if (splits > 1) cg::this_cluster().barrier_arrive();
+  int32_t token = -1;
+  float given = -INFINITY;  // the given token's logit
+  if (split == 0 && tid == 0 && a.tokens != nullptr) {
+    token = a.tokens[row];
+    if ((uint32_t)token < a.vocab) given = V::one(x + token);
+  }
   for (uint32_t at = v0; at < v1; at += kStep, ++step) {
     load(at + (kStages - 1) * kStep, (step + kStages - 1) % kStages);
     asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 1) : "memory");
@@ -498,11 +499,11 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   if (tid >= kThreads - 32) {  // the warp that select() needs least
     const uint32_t lane = tid & 31;
     st = warp_merge(lane < kWarps ? sh.stat[lane] : Stat{-INFINITY, 0.0f, 0.0f});
-    if (lane == 0) sh.total = st;
+    if (lane == 0) sh.totals[0] = st;
   }
   if (k != 0) {
     uint32_t n = sh.count;
-    select(sh, n, k);
+    select(sh, sh.buf, n, k);
     if (n < k) {
       // the rest are the first elements that equal the bound (a NaN equals -inf)
       const uint64_t j1 = min((uint64_t)a.vocab, max((uint64_t)v1 * N, (uint64_t)shift) - shift);
@@ -528,28 +529,27 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
     }
   }
   if (splits > 1) {
+    // every CTA writes into the first one's shared memory, which none of them reads after
+    // it has gone
     cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();  // every CTA's total and sel
-    if (split == 0) {
-      unsigned long long key = 0;
-      if (k != 0 && tid < splits * k) key = cluster.map_shared_rank(sh.sel, tid / k)[tid % k];
-      if (tid >= kThreads - 32) {
-        const uint32_t lane = tid & 31;
-        st = warp_merge(lane < splits ? *cluster.map_shared_rank(&sh.total, lane) : Stat{-INFINITY, 0.0f, 0.0f});
-        if (lane == 0) sh.total = st;
-      }
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
-      if (key != 0) sh.buf[atomicAdd(&sh.count, 1u)] = key;
-      __syncthreads();
-      if (k != 0) select(sh, sh.count, k);
-    }
+    Shared* first = cluster.map_shared_rank(&sh, 0);
+    if (k == 0) __syncthreads();  // totals[0]; select() ends with one
+    const Stat mine = sh.totals[0];
+    cluster.barrier_wait();  // the first CTA runs, and has not yet reached the next sync
+    // entries without an element differ too; their upper half is 0
+    if (tid < k) first->joined[split * k + tid] = sh.sel[tid] != 0 ? sh.sel[tid] : split * k + tid + 1;
+    if (tid == 0 && split != 0) first->totals[split] = mine;
     cluster.sync();
     if (split != 0) return;
-  } else if (k == 0) {
-    __syncthreads();  // select() ends with one
+    if (tid >= kThreads - 32) {
+      const uint32_t lane = tid & 31;
+      st = warp_merge(lane < splits ? sh.totals[lane] : Stat{-INFINITY, 0.0f, 0.0f});
+      if (lane == 0) sh.totals[0] = st;
+    }
+    if (k != 0) select(sh, sh.joined, splits * k, k);
   }
-  const Stat t = sh.total;
+  if (k == 0) __syncthreads();
+  const Stat t = sh.totals[0];
   const bool none = t.s == 0.0f;  // every element is -inf
   const float log2s = log2f(t.s), ls = (log2s - excess(t.m)) * kLn2;
   if (tid == 0) {
@@ -561,8 +561,9 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
   }
   if (tid < k) {
     const unsigned long long key = sh.sel[tid];
-    a.top_ids[row * k + tid] = key != 0 ? (int32_t)(0xffffffffu - (uint32_t)key) : -1;
-    a.top_logprobs[row * k + tid] = key == 0 || none ? -INFINITY : value_of(key) - t.m - ls;
+    const bool some = key >> 32 != 0;
+    a.top_ids[row * k + tid] = some ? (int32_t)(0xffffffffu - (uint32_t)key) : -1;
+    a.top_logprobs[row * k + tid] = !some || none ? -INFINITY : value_of(key) - t.m - ls;
   }
 }
 
@@ -573,7 +574,7 @@ int launch(const Args& a, uint64_t rows, cudaStream_t st) {
   // still has two steps' work.
   uint32_t splits = 1;
   const uint64_t step = (uint64_t)kThreads * Vec<T>::kUnroll * Vec<T>::N;
-  while (splits < 8 && rows * splits * 2 <= 3ull * num_sms() && a.vocab > splits * step) splits *= 2;
+  while (splits < (uint32_t)kMaxSplits && rows * splits * 2 <= 3ull * num_sms() && a.vocab > splits * step) splits *= 2;
   for (uint64_t r0 = 0; r0 < rows; r0 += 65535) {
     Args b = a;
     const uint64_t n = rows - r0 < 65535 ? rows - r0 : 65535;

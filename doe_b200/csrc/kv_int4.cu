@@ -16,10 +16,12 @@ namespace doe {
 struct PageMap {
   const int32_t* block_table;
   int page_size, num_pages, max_pages;
-  __device__ __forceinline__ int page(int b, long long pos) const {
+  __device__ __forceinline__ int entry(int b, long long pos) const {
     const long long pidx = pos / page_size;
-    if (pos < 0 || pidx >= max_pages) return -1;
-    const int p = block_table[(size_t)b * max_pages + pidx];
+    return pos < 0 || pidx >= max_pages ? -1 : block_table[(size_t)b * max_pages + pidx];
+  }
+  __device__ __forceinline__ int page(int b, long long pos) const {
+    const int p = entry(b, pos);
     return (unsigned)p < (unsigned)num_pages ? p : -1;
   }
 };
@@ -45,13 +47,12 @@ struct BlockWork {
   long long first;   // the block's first position
   int lo, hi;        // its tokens in the chunk: [lo, hi) of 16
   long long row0;    // row of token 0 in [B, T, Hkv] (of lo > 0: before the chunk's)
-  size_t block;      // byte offset in the pool
-  bool mapped;
+  int entry, tile;   // of the block table, not yet looked at; the block within its page
   __device__ __forceinline__ bool whole() const { return lo == 0 && hi == 16; }
 };
-// False: nothing of the chunk is there.  An unmapped block is reported.
+// False: nothing of the chunk is there.
 __device__ __forceinline__ bool find_block(BlockWork& w, const PageMap& map, const int32_t* positions, int n_tokens,
-                                           int heads, int wid, int32_t* status) {
+                                           int heads, int wid) {
   w.kv = wid & 1;
   w.h = (wid >> 1) % heads;
   w.b = blockIdx.y;
@@ -62,12 +63,16 @@ __device__ __forceinline__ bool find_block(BlockWork& w, const PageMap& map, con
   w.lo = (int)max(0ll, pos0 - w.first);
   w.hi = (int)min(16ll, end - w.first);
   w.row0 = ((long long)w.b * n_tokens + (w.first - pos0)) * heads + w.h;
-  const int page = pos0 < 0 ? -1 : map.page(w.b, w.first);
-  w.mapped = page >= 0;
-  if (!w.mapped && (threadIdx.x & 31) == 0) report(status, DOE_DEVICE_ERR_PAGE);
-  const int tile = (int)(w.first % map.page_size) / 16;
-  w.block = w.mapped ? (((size_t)page * heads + w.h) * (map.page_size / 16) + tile) * kI4Block : 0;
+  w.entry = pos0 < 0 ? -1 : map.entry(w.b, w.first);
+  w.tile = (int)(w.first % map.page_size) / 16;
   return true;
+}
+// The block's byte offset in the pool.  False, and reported: it is not mapped.
+__device__ __forceinline__ bool mapped(const BlockWork& w, const PageMap& map, int heads, int32_t* status, size_t& block) {
+  block = (((size_t)(unsigned)w.entry * heads + w.h) * (map.page_size / 16) + w.tile) * kI4Block;
+  if ((unsigned)w.entry < (unsigned)map.num_pages) return true;
+  if ((threadIdx.x & 31) == 0) report(status, DOE_DEVICE_ERR_PAGE);
+  return false;
 }
 
 // WHOLE: all 16 tokens are in the chunk.
@@ -75,7 +80,6 @@ template <bool ROPE, bool WHOLE>
 __device__ __forceinline__ void append_block(const Int4AppendArgs& a, const BlockWork& w) {
   const int lane = threadIdx.x & 31, hw = lane >> 4, l16 = lane & 15, t = l16 & 3, group = l16 >> 2;
   const __half* src = (w.kv ? a.new_v : a.new_k) + w.row0 * 128 + 8 * l16;
-  uint8_t* dst = (w.kv ? a.v_pool : a.k_pool) + w.block;
   const int stride = a.num_kv_heads * 128;  // of a token
   auto live = [&](int tok) { return WHOLE || (tok >= w.lo && tok < w.hi); };
   uint4 x[8];
@@ -85,6 +89,9 @@ __device__ __forceinline__ void append_block(const Int4AppendArgs& a, const Bloc
     x[i] = make_uint4(0, 0, 0, 0);
     if (live(tok)) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + (long long)tok * stride));
   }
+  size_t block;  // the rows are on their way while the page is looked up
+  if (!mapped(w, a.map, a.num_kv_heads, a.status, block)) return;
+  uint8_t* dst = (w.kv ? a.v_pool : a.k_pool) + block;
   if (ROPE && w.kv == 0) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -189,7 +196,7 @@ __global__ void __launch_bounds__(256) int4_append_kernel(const Int4AppendArgs a
   const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (wid >= warps_per_seq) return;
   BlockWork w;
-  if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid, a.status) || !w.mapped) return;
+  if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid)) return;
   if (w.whole()) append_block<ROPE, true>(a, w);
   else append_block<ROPE, false>(a, w);
 }
@@ -264,7 +271,9 @@ __device__ __forceinline__ __half2 code_values(uint32_t w, int i, __half2 s) {
 template <typename T, bool WHOLE>
 __device__ __forceinline__ void read_block(const PagedReadArgs& a, const BlockWork& w) {
   const int lane = threadIdx.x & 31, hw = lane >> 4, l16 = lane & 15, t = l16 & 3, group = l16 >> 2;
-  const uint8_t* src = (w.kv ? a.pool[1] : a.pool[0]) + w.block;
+  size_t block;
+  const bool some = mapped(w, a.map, a.num_kv_heads, a.status, block);
+  const uint8_t* src = (w.kv ? a.pool[1] : a.pool[0]) + (some ? block : 0);
   T* dst = static_cast<T*>(w.kv ? a.out[1] : a.out[0]) + w.row0 * 128 + 8 * l16;
   const int stride = a.num_kv_heads * 128;  // of a token
   auto live = [&](int tok) { return WHOLE || (tok >= w.lo && tok < w.hi); };
@@ -275,7 +284,7 @@ __device__ __forceinline__ void read_block(const PagedReadArgs& a, const BlockWo
   const __half* sc = reinterpret_cast<const __half*>(src + kI4Codes) + (w.kv ? hw * 8 + group * 2 : hw * 8 + group);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (!w.mapped) {  // reads as zeros
+    if (!some) {  // reads as zeros
       code[j][0] = code[j][1] = 0u;
       s[j] = __float2half2_rn(0.0f);
     } else if (w.kv) {
@@ -341,7 +350,7 @@ __global__ void __launch_bounds__(256) int4_read_kernel(const PagedReadArgs a, i
   const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (wid >= warps_per_seq) return;
   BlockWork w;
-  if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid, a.status)) return;
+  if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid)) return;
   if (w.whole()) read_block<T, true>(a, w);
   else read_block<T, false>(a, w);
 }

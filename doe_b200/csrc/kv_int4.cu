@@ -38,6 +38,11 @@ struct Int4AppendArgs {
   int n_tokens, num_kv_heads, rope_positions;
 };
 
+// Of a CTA: warps share nothing, and at the append's 90 registers CTAs of 4 leave 20
+// of them resident on an SM where CTAs of 8 leave 16 (32 x 512 tokens written and
+// read: 35.5 us against 39.1; 2 warps 35.4, but 7.6 against 7.1 for 32 x 1 tokens).
+constexpr int kWarps = 4;
+
 // One warp per (sequence, 16-token block, kv head, K or V).  Half-warp hw takes the
 // token pairs 2 j + hw, lane l16 the dims [8 l16, 8 l16 + 8): one K word per token
 // and two V words per pair; a group's maximum is four lanes'.  All 16 rows (4 KB)
@@ -190,10 +195,10 @@ __device__ __forceinline__ void append_block(const Int4AppendArgs& a, const Bloc
 }
 
 template <bool ROPE>
-__global__ void __launch_bounds__(256) int4_append_kernel(const Int4AppendArgs a, int warps_per_seq) {
+__global__ void __launch_bounds__(kWarps * 32) int4_append_kernel(const Int4AppendArgs a, int warps_per_seq) {
   pdl_wait();
   pdl_trigger();
-  const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int wid = blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (wid >= warps_per_seq) return;
   BlockWork w;
   if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid)) return;
@@ -219,10 +224,10 @@ int launch_int4_append(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tok
   a.rope_positions = (int)rope_positions;
   // a chunk starting inside a block touches one block more
   const uint64_t warps = (((uint64_t)n_tokens + 14) / 16 + 1) * kv->num_kv_heads * 2;
-  const dim3 grid((unsigned)((warps + 7) / 8), num_seqs);
+  const dim3 grid((unsigned)((warps + kWarps - 1) / kWarps), num_seqs);
   cudaStream_t st = static_cast<cudaStream_t>(launch->stream);
   return cuda_status(launch_pdl(freq_cis != nullptr ? int4_append_kernel<true> : int4_append_kernel<false>, grid,
-                                dim3(256), 0, st, a, (int)warps),
+                                dim3(kWarps * 32), 0, st, a, (int)warps),
                      "int4_append_kernel");
 }
 
@@ -344,10 +349,10 @@ __device__ __forceinline__ void read_block(const PagedReadArgs& a, const BlockWo
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) int4_read_kernel(const PagedReadArgs a, int warps_per_seq) {
+__global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const PagedReadArgs a, int warps_per_seq) {
   pdl_wait();
   pdl_trigger();
-  const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int wid = blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (wid >= warps_per_seq) return;
   BlockWork w;
   if (!find_block(w, a.map, a.positions, a.n_tokens, a.num_kv_heads, wid)) return;
@@ -400,8 +405,8 @@ template <typename T>
 static int launch_read(const doe_paged_kv* kv, const PagedReadArgs& a, uint32_t num_seqs, cudaStream_t st) {
   if (kv->kv_dtype == DOE_KV_INT4) {
     const uint64_t warps = (((uint64_t)a.n_tokens + 14) / 16 + 1) * kv->num_kv_heads * 2;
-    const dim3 grid((unsigned)((warps + 7) / 8), num_seqs);
-    return cuda_status(launch_pdl(int4_read_kernel<T>, grid, dim3(256), 0, st, a, (int)warps), "int4_read_kernel");
+    const dim3 grid((unsigned)((warps + kWarps - 1) / kWarps), num_seqs);
+    return cuda_status(launch_pdl(int4_read_kernel<T>, grid, dim3(kWarps * 32), 0, st, a, (int)warps), "int4_read_kernel");
   }
   const dim3 grid(((uint32_t)a.n_tokens + 7) / 8, num_seqs);
   if (kv->kv_dtype == DOE_KV_INT8)

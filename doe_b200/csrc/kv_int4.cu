@@ -12,17 +12,13 @@
 
 namespace doe {
 
-// Page of token `pos` of sequence row b, or -1.
+// Positions are below 2^32 (an int32 and an int32's count), so index arithmetic has 32 bits.
 struct PageMap {
   const int32_t* block_table;
-  int page_size, num_pages, max_pages;
-  __device__ __forceinline__ int entry(int b, long long pos) const {
-    const long long pidx = pos / page_size;
-    return pos < 0 || pidx >= max_pages ? -1 : block_table[(size_t)b * max_pages + pidx];
-  }
-  __device__ __forceinline__ int page(int b, long long pos) const {
-    const int p = entry(b, pos);
-    return (unsigned)p < (unsigned)num_pages ? p : -1;
+  uint32_t page_size, num_pages, max_pages;
+  // Entry `pidx` of sequence row b, or -1 past the row.
+  __device__ __forceinline__ int entry(int b, uint32_t pidx) const {
+    return pidx >= max_pages ? -1 : block_table[(size_t)b * max_pages + pidx];
   }
 };
 
@@ -58,24 +54,26 @@ struct BlockWork {
 // False: nothing of the chunk is there.
 __device__ __forceinline__ bool find_block(BlockWork& w, const PageMap& map, const int32_t* positions, int n_tokens,
                                            int heads, int wid) {
+  const int pair = wid >> 1, nth = pair / heads;
   w.kv = wid & 1;
-  w.h = (wid >> 1) % heads;
+  w.h = pair - nth * heads;
   w.b = blockIdx.y;
   const int pos0 = positions[w.b];
-  w.first = (long long)(pos0 & ~15) + 16ll * (wid / (2 * heads));
+  w.first = (long long)(pos0 & ~15) + 16ll * nth;
   const long long end = (long long)pos0 + n_tokens;
   if (w.first >= end) return false;
   w.lo = (int)max(0ll, pos0 - w.first);
   w.hi = (int)min(16ll, end - w.first);
   w.row0 = ((long long)w.b * n_tokens + (w.first - pos0)) * heads + w.h;
-  w.entry = pos0 < 0 ? -1 : map.entry(w.b, w.first);
-  w.tile = (int)(w.first % map.page_size) / 16;
+  const uint32_t tile = (uint32_t)w.first / 16, per = map.page_size / 16, pidx = tile / per;
+  w.entry = pos0 < 0 ? -1 : map.entry(w.b, pidx);
+  w.tile = (int)(tile - pidx * per);
   return true;
 }
 // The block's byte offset in the pool.  False, and reported: it is not mapped.
 __device__ __forceinline__ bool mapped(const BlockWork& w, const PageMap& map, int heads, int32_t* status, size_t& block) {
   block = (((size_t)(unsigned)w.entry * heads + w.h) * (map.page_size / 16) + w.tile) * kI4Block;
-  if ((unsigned)w.entry < (unsigned)map.num_pages) return true;
+  if ((uint32_t)w.entry < map.num_pages) return true;
   if ((threadIdx.x & 31) == 0) report(status, DOE_DEVICE_ERR_PAGE);
   return false;
 }
@@ -218,7 +216,7 @@ int launch_int4_append(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_tok
   a.positions = positions;
   a.status = launch->status;
   a.freq_cis = freq_cis;
-  a.map = {kv->block_table, (int)kv->page_size, (int)kv->num_pages, (int)kv->max_pages_per_seq};
+  a.map = {kv->block_table, kv->page_size, kv->num_pages, kv->max_pages_per_seq};
   a.n_tokens = (int)n_tokens;
   a.num_kv_heads = (int)kv->num_kv_heads;
   a.rope_positions = (int)rope_positions;
@@ -367,10 +365,13 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const PagedReadArgs a) 
   const int tok = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, b = blockIdx.y;
   if (tok >= a.n_tokens) return;
   const int pos0 = a.positions[b];
-  const long long pos = (long long)pos0 + tok;
-  const int page = pos0 < 0 ? -1 : a.map.page(b, pos);
-  if (page < 0 && lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
-  const int in_page = (int)(pos % a.map.page_size);
+  const uint32_t pos = (uint32_t)pos0 + tok, pidx = pos / a.map.page_size;
+  int page = pos0 < 0 ? -1 : a.map.entry(b, pidx);
+  if ((uint32_t)page >= a.map.num_pages) {
+    page = -1;
+    if (lane == 0) report(a.status, DOE_DEVICE_ERR_PAGE);
+  }
+  const int in_page = (int)(pos - pidx * a.map.page_size);
   const int Hkv = a.num_kv_heads, D = a.head_dim, n = Hkv * D;
   const size_t row = ((size_t)page * a.map.page_size + in_page) * n;
   const size_t out = ((size_t)b * a.n_tokens + tok) * n;
@@ -428,7 +429,7 @@ int launch_paged_read(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t n_toke
   a.out[1] = v_out;
   a.positions = positions;
   a.status = launch->status;
-  a.map = {kv->block_table, (int)kv->page_size, (int)kv->num_pages, (int)kv->max_pages_per_seq};
+  a.map = {kv->block_table, kv->page_size, kv->num_pages, kv->max_pages_per_seq};
   a.n_tokens = (int)n_tokens;
   a.num_kv_heads = (int)kv->num_kv_heads;
   a.head_dim = (int)kv->head_dim;

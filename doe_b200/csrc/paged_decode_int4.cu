@@ -102,6 +102,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // A block's 16-byte copies of one lane (two of K codes, two of V codes, one of
 // scales where `scales`), or none of them.
@@ -427,7 +432,8 @@ struct Walker {
     // x is the softcapped score in the log2 domain (CAP) or the bare product, which
     // c > 0 takes there: the sign of the scale is in Q, and a scale of 0 becomes
     // tiny so that the -inf of a dead key stays -inf
-    const float to_cap = a.scale * kTwo24 / a.softcap, cap_log2 = a.softcap * kLog2e;  // CAP only
+    // CAP: softcap tanh(y) = softcap (1 - 2 / (1 + e^2y)), within about 2e-7 softcap
+    const float to_cap = 2.0f * kLog2e * kTwo24 * a.scale / a.softcap, cap_log2 = a.softcap * kLog2e;
     const float c_log2 = CAP ? 1.0f : fmaxf(fabsf(a.scale) * (kLog2e * kTwo24), 1e-30f), inv_c = 1.0f / c_log2;
     int edge_k = first * 16 < min_key || bad ? 0 : nt - kStep;  // steps from here on have dead keys
     uint32_t slot = kSlot0, refill = 0;  // byte offsets in the ring
@@ -496,7 +502,7 @@ struct Walker {
           s[3] = n ? fmaf(s1, c[3], s[3]) : s1 * c[3];
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[u][i] = CAP ? cap_log2 * tanhf(s[i] * to_cap) : s[i];
+        for (int i = 0; i < 4; ++i) x[u][i] = CAP ? fmaf(-2.0f * cap_log2, rcp(1.0f + ex2(s[i] * to_cap)), cap_log2) : s[i];
       }
       const uint32_t v_at = wbase + slot + kI4Block + 16 * lane;
       refill = slot;

@@ -44,6 +44,8 @@
 // the last one to arrive.  Short rows, many of them: one CTA each.  Pieces and
 // splits follow from the lengths alone and sums go in the order of the keys, so
 // results do not depend on timing.
+#include <algorithm>
+
 #include <cooperative_groups.h>
 
 #include "int4.cuh"
@@ -61,6 +63,7 @@ constexpr int kBlkRing = 128;                  // block numbers per warp, renewe
 constexpr int kCtasPerSm = 3;                  // resident: 168 registers a thread
 constexpr int kRowCost = 4;                    // a sequence's fixed cost in the list, in blocks
 constexpr int kMinPiece = 8;                   // entries; more than kRowCost, so that no piece is empty
+constexpr uint64_t kListRows = 7;              // x rows from 4 warps' x resident CTAs on: the list
 constexpr uint64_t kShortRow = 128;            // blocks that one CTA walks alone when there are rows enough
 constexpr uint64_t kLoneRow = 32;              // the same, when there are few rows
 constexpr uint64_t kMinSplit = 16;             // blocks
@@ -93,6 +96,7 @@ struct Args {
   int tiles_per_page, tile_shift;  // page_size / 16 and its log2 (-1: not a power of two)
   int num_seqs;
   int split_tiles, max_parts;  // splits: blocks per split, clusters (or single splits) per row
+  int units;                   // or, when not 0: clusters per kv head, shared out by the lengths
   int out_bf16;
   int inputs_stable;
 };
@@ -676,7 +680,7 @@ struct Joined {
 // The last part of a (row, slice of the dims) to finish stitches them, in key order.
 // T threads take every T-th part of four dims of a head each, so that one round
 // of loads reaches all parts (one thread each: 3 of them in turn for 24 parts).
-__device__ __forceinline__ void stitch_parts(const Args& a, size_t row, int rank, int slices, int nparts, int* last) {
+__device__ __forceinline__ void stitch_parts(const Args& a, size_t row, size_t part0, int rank, int slices, int nparts, int* last) {
   __syncthreads();
   if (threadIdx.x == 0) *last = arrive_last(&a.counters[row * slices + rank], nparts);
   __syncthreads();
@@ -690,7 +694,7 @@ __device__ __forceinline__ void stitch_parts(const Args& a, size_t row, int rank
     const int h = at / quads, d = (rank * quads + at % quads) * 4;
     Joined sum;
     sum.add(sub < nparts ? (nparts - sub + T - 1) / T : 0, [&](int p, float2& ml, float4& o) {
-      const size_t from = row * a.max_parts + sub + p * T;
+      const size_t from = part0 + sub + p * T;
       ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + (from * slices + rank) * a.group + h);
       o = __ldcg(reinterpret_cast<const float4*>(a.part_o + (from * a.group + h) * kD + d));
     });
@@ -709,6 +713,61 @@ __device__ __forceinline__ void stitch_parts(const Args& a, size_t row, int rank
   }
 }
 
+// What one cluster (or single CTA) takes of the rows of a kv head.
+struct Share {
+  int b;            // sequence, -1: nothing
+  int unit0, part;  // the sequence's first cluster, and which one of them this is
+  int split_tiles;  // blocks per CTA
+  int len;          // the sequence's, as given
+};
+// Cluster `unit` of a.units: sequences get clusters by their blocks, with the
+// smallest split (of kMinSplit blocks or more) at which they suffice.  Every warp
+// works it out for itself.
+__device__ __forceinline__ Share share_of(const Args& a, int unit, int slices, int lane) {
+  if (a.num_seqs == 1) {
+    const int len = a.seq_lens[0], all = a.units * slices;
+    return Share{0, 0, unit, max((int)kMinSplit, (keys_of(a, len).tiles + all - 1) / all), len};
+  }
+  auto tiles = [&](int i) { return i < a.num_seqs ? keys_of(a, a.seq_lens[i]).tiles : 0; };
+  int total = 0;
+#pragma unroll 1
+  for (int i = lane; i < a.num_seqs; i += 32) total += tiles(i);
+  total = __reduce_add_sync(0xffffffffu, total);  // below 2^31 (plan)
+  unsigned t = max((unsigned)kMinSplit, (unsigned)(total + a.units * slices - 1) / (a.units * slices));
+  auto clusters = [&](int i) -> unsigned {
+    const unsigned n = tiles(i);
+    return i >= a.num_seqs ? 0 : n <= kLoneRow ? 1 : (n + t * slices - 1) / (t * slices);
+  };
+#pragma unroll 1
+  while (true) {  // ends: with t the longest row's blocks, a.units >= num_seqs clusters suffice
+    unsigned n = 0;
+#pragma unroll 1
+    for (int i = lane; i < a.num_seqs; i += 32) n += clusters(i);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (n <= (unsigned)a.units) break;
+    t = max(t + t / 16 + 1, (unsigned)((float)t * (float)n / (float)a.units));
+  }
+  int before = 0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < a.num_seqs; i0 += 32) {
+    const int mine = clusters(i0 + lane);
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const int first = before + upto - mine;
+    const unsigned at = __ballot_sync(0xffffffffu, unit >= first && unit < first + mine);
+    if (at != 0) {
+      const int from = __ffs(at) - 1, unit0 = __shfl_sync(0xffffffffu, first, from);
+      return Share{i0 + from, unit0, unit - unit0, (int)t, a.seq_lens[i0 + from]};
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return Share{-1, 0, 0, (int)t, 0};
+}
+
 // ---- few rows: one CTA per split --------------------------------------------------
 template <bool CAP>
 __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) splits_kernel(const Args a) {
@@ -722,16 +781,23 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) splits_kernel(const A
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int Hkv = a.num_kv_heads, group = a.group;
   const int slices = (int)cg::this_cluster().num_blocks();
-  const int split = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
+  const int split0 = blockIdx.x / slices * slices;  // the cluster's first CTA
+  const Share sh = a.units != 0 ? share_of(a, split0 / slices, slices, lane)
+                                : Share{(int)blockIdx.z, 0, split0 / slices, a.split_tiles, a.seq_lens[blockIdx.z]};
+  if (sh.b < 0) return;
+  const int g = blockIdx.y, b = sh.b, part = sh.part, split_tiles = sh.split_tiles;
+  const int split = part * slices + (blockIdx.x - split0);
+  const size_t row = (size_t)b * Hkv + g;
+  // of the row's first part in the workspace
+  const size_t part0 = a.units != 0 ? (size_t)g * a.units + sh.unit0 : row * a.max_parts;
 
-  const int raw = a.seq_lens[b];
-  const Keys seq = keys_of(a, raw);
-  if (raw != seq.seq_len && split == 0 && g == 0 && threadIdx.x == 0) report(a.status, DOE_DEVICE_ERR_LENGTH);
-  const int nsplits = max(1, (seq.tiles + a.split_tiles - 1) / a.split_tiles);
-  const int part = split / slices, nparts = (nsplits + slices - 1) / slices;
+  const Keys seq = keys_of(a, sh.len);
+  if (sh.len != seq.seq_len && split == 0 && g == 0 && threadIdx.x == 0) report(a.status, DOE_DEVICE_ERR_LENGTH);
+  const int nsplits = a.units != 0 && seq.tiles <= kLoneRow ? 1 : max(1, (seq.tiles + split_tiles - 1) / split_tiles);
+  const int nparts = (nsplits + slices - 1) / slices;
   if (part >= nparts) return;             // the whole cluster; a split past the last joins with nothing
-  if (nsplits == 1 && split != 0) return;  // nothing to join
-  const int tile_begin = split * a.split_tiles, tile_end = min(seq.tiles, tile_begin + a.split_tiles);
+  if (nsplits == 1 && split != part * slices) return;  // nothing to join
+  const int tile_begin = split * split_tiles, tile_end = nsplits == 1 ? seq.tiles : min(seq.tiles, tile_begin + split_tiles);
   const int span = tile_end - tile_begin - warp;
   const Stretch w = {b, g, seq.seq_len, seq.min_key, seq.origin + tile_begin + warp,
                      span > 0 ? (span + kWarps - 1) / kWarps : 0, 0, nsplits == 1};
@@ -756,7 +822,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) splits_kernel(const A
     *reinterpret_cast<float4*>(my_o + (2 * t + j) * kD + d) = v;
   });
   __syncthreads();
-  const size_t row = (size_t)b * Hkv + g, part_row = row * a.max_parts + part;
+  const size_t part_row = part0 + part;
   float* cta_o = reinterpret_cast<float*>(ring);  // [8][128], over the first warp's
   for (int i = threadIdx.x; i < group * (kD / 4); i += kWarps * 32) {
     const int h = i / (kD / 4), d = i % (kD / 4) * 4;
@@ -810,7 +876,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) splits_kernel(const A
     }
     cluster.sync();  // this CTA has read the others' parts
   }
-  if (nparts > 1) stitch_parts(a, row, rank, slices, nparts, &sm_last);
+  if (nparts > 1) stitch_parts(a, row, part0, rank, slices, nparts, &sm_last);
 }
 
 // ---- many rows: pieces of one list, a warp each -------------------------------------
@@ -1052,38 +1118,44 @@ int launch_cap(const Args& a, bool list, dim3 grid, unsigned slices, cudaStream_
 struct Plan {
   bool list;                     // pieces of one list; else splits
   uint64_t split_tiles, slices;  // splits: blocks per split, splits per cluster
-  uint64_t max_parts, grid;      // splits: parts per row; CTAs (per row)
+  uint64_t units;                // splits that follow the lengths: clusters per kv head
+  uint64_t max_parts, grid;      // splits: parts per row; CTAs (per row, or per kv head)
   uint64_t slots;                // parts in the workspace (whatever the window, which its size query lacks)
 };
 
 // `tiles`: the most blocks of a row that can be read (its block-table row, or the
-// window).  Short rows, enough of them to fill the SMs: one CTA each, nothing to
-// join.  Else the list, while a row is cut into about a dozen parts at most, which
-// one warp stitches.  With fewer rows each gets its own splits, as many as CTAs
-// are resident.  A given split_pages asks for splits of that length; they serve
-// more than kMaxListSeqs sequences too.
+// window).
 Plan plan(uint64_t num_seqs, uint64_t kv_heads, uint64_t max_tiles, uint64_t tiles_per_page, uint64_t split_pages,
           uint64_t window) {
   Plan p = {};
   const uint64_t rows = num_seqs * kv_heads, sms = (uint64_t)num_sms(), ctas = sms * kCtasPerSm;
   const uint64_t tiles = window != 0 && window / 16 + 2 < max_tiles ? window / 16 + 2 : max_tiles;
+  const bool counted = num_seqs * (max_tiles + kRowCost) <= 0x1fffffffull;  // the device's sums of blocks
   uint64_t t = split_pages * tiles_per_page;
-  if (t == 0 && num_seqs <= kMaxListSeqs && rows * 14 >= ctas * kWarps && kv_heads <= ctas * kWarps &&
-      num_seqs * (max_tiles + kRowCost) <= 0x1fffffffull) {
-    p.slots = 2 * ctas * kWarps;
-    if (rows < sms || tiles > kShortRow) {
-      p.list = true;
-      p.slices = 1;
-      p.max_parts = 2;
-      p.grid = ctas;
-      return p;
-    }
+  const bool short_rows = t == 0 && rows >= sms && tiles <= kShortRow;
+  if (short_rows) {
     t = tiles;
+  } else if (t == 0 && rows * kListRows < ctas * kWarps && counted) {
+    p.slices = max_tiles > 16 * kMinSplit && rows * 16 < sms * 13 / 5 ? 8 : 1;
+    const uint64_t fill = p.slices > 1 ? sms * 13 / 5 / p.slices : ctas;
+    // no more than the rows can use at all, and one for every row
+    const uint64_t most = max_tiles <= kLoneRow ? 1 : (max_tiles + kMinSplit * p.slices - 1) / (kMinSplit * p.slices);
+    p.units = std::max(num_seqs, std::min(fill / kv_heads, num_seqs * most));
+    p.max_parts = 2;
+    p.grid = p.units * p.slices;
+    p.slots = p.units * kv_heads;
+    return p;
+  } else if (t == 0 && num_seqs <= kMaxListSeqs && kv_heads <= ctas * kWarps && counted) {
+    p.list = true;
+    p.slices = 1;
+    p.max_parts = 2;
+    p.grid = ctas;
+    p.slots = 2 * ctas * kWarps;
+    return p;
   } else if (t == 0) {
-    const uint64_t fill = (sms * 5 / 2 + rows - 1) / rows;
-    p.slots = rows * fill;
-    t = tiles <= (rows >= sms ? kShortRow : kLoneRow) ? tiles : (tiles + fill - 1) / fill;
+    t = rows >= sms ? tiles : (tiles * rows + sms - 1) / sms;
     if (t < kMinSplit) t = kMinSplit;
+    p.slots = rows >= sms ? rows : sms + rows;
   } else {
     p.slots = rows * ((max_tiles + t - 1) / t);
   }
@@ -1173,6 +1245,7 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   a.num_seqs = (int)num_seqs;
   a.split_tiles = (int)pl.split_tiles;
   a.max_parts = (int)pl.max_parts;
+  a.units = (int)pl.units;
   a.out_bf16 = (opts && (opts->flags & DOE_DECODE_OUT_BF16)) ? 1 : 0;
   a.inputs_stable = (opts && (opts->flags & DOE_DECODE_INPUTS_STABLE)) ? 1 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(launch->stream);
@@ -1181,7 +1254,7 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
         cuda_status(cudaMemsetAsync(a.counters, 0, rows * pl.slices * sizeof(unsigned), st), "cudaMemsetAsync(split counters)");
     if (rc != DOE_OK) return rc;
   }
-  const dim3 grid = pl.list ? dim3((unsigned)pl.grid) : dim3((unsigned)pl.grid, Hkv, num_seqs);
+  const dim3 grid = pl.list ? dim3((unsigned)pl.grid) : dim3((unsigned)pl.grid, Hkv, pl.units != 0 ? 1 : num_seqs);
   return a.softcap > 0.0f ? launch_cap<true>(a, pl.list, grid, (unsigned)pl.slices, st)
                           : launch_cap<false>(a, pl.list, grid, (unsigned)pl.slices, st);
 }

@@ -428,3 +428,16 @@ def test_decode_appends_non_finite_rows_as_such():
     k, v = (x.cpu().numpy() for x in ops.paged_read(cache, _t(c.lens - 1), 1, dtype=torch.float32))
     assert np.isnan(k[0, 0, 1, 32:64]).all() and np.isnan(k).sum() == 32
     assert np.isnan(v[1, 0, 0, 64:96]).all() and np.isnan(v).sum() == 32
+
+
+@pytest.mark.parametrize("width", [1, 300])
+@pytest.mark.parametrize("lens", [[4000], [300, 0, 4097, 1], [17] * 20 + [2500], [0] * 40 + [900, 33, 2000]])
+@pytest.mark.parametrize("Hkv", [1, 3])
+def test_decode_few_rows_share_the_splits_by_length(lens, width, Hkv):
+    """Splits follow the lengths, not the block table's width (`width` unused pages a row)."""
+    c = Case(len(lens) + width, lens, Hkv, 4)
+    c.table = np.concatenate([c.table, np.full((len(lens), width), -1, np.int32)], 1)
+    out = _decode(c)
+    c.check(out, 128 ** -0.5)
+    assert np.array_equal(out, _decode(c)), "results depend on timing"
+    c.check(_decode(c, sliding_window=1000), 128 ** -0.5, 1000)

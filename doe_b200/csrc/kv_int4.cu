@@ -4,8 +4,13 @@
 //            quantised into the blocks of int4.cuh
 //   read   : value rows of any cache type (f16, int8, int4) as f16, bf16 or f32
 //
-// Both are copies with a little arithmetic, bound by HBM: 512 bytes of f16 K
-// and V against 144 bytes of blocks per (token, kv head).
+// Copies with a little arithmetic: 512 bytes of f16 K and V against 144 bytes of
+// blocks per (token, kv head).  Writing 32 x 512 tokens of 8 kv heads and reading them
+// back takes 33.7 us for 172 MB (5.1 TB/s, 0.78 of the measured copy rate); the write
+// alone is near 20, bound by issue slots (79 instructions for a token's K or V of a
+// head, half of the cycles) and by how many loads 20 warps an SM keep in flight, the
+// read near 14, bound by HBM writes and the two loads before its own.  32 tokens
+// written and read back take 6.5 us: two launches.
 #include <type_traits>
 
 #include "int4.cuh"
@@ -71,7 +76,8 @@ __device__ __forceinline__ bool find_block(BlockWork& w, const PageMap& map, con
   return true;
 }
 // The block's byte offset in the pool.  False, and reported: it is not mapped.
-__device__ __forceinline__ bool mapped(const BlockWork& w, const PageMap& map, int heads, int32_t* status, size_t& block) {
+__device__ __forceinline__ bool mapped(const BlockWork& w, const PageMap& map, int heads, int32_t* status,
+                                       size_t& block) {
   block = (((size_t)(unsigned)w.entry * heads + w.h) * (map.page_size / 16) + w.tile) * kI4Block;
   if ((uint32_t)w.entry < map.num_pages) return true;
   if ((threadIdx.x & 31) == 0) report(status, DOE_DEVICE_ERR_PAGE);
@@ -407,7 +413,8 @@ static int launch_read(const doe_paged_kv* kv, const PagedReadArgs& a, uint32_t 
   if (kv->kv_dtype == DOE_KV_INT4) {
     const uint64_t warps = (((uint64_t)a.n_tokens + 14) / 16 + 1) * kv->num_kv_heads * 2;
     const dim3 grid((unsigned)((warps + kWarps - 1) / kWarps), num_seqs);
-    return cuda_status(launch_pdl(int4_read_kernel<T>, grid, dim3(kWarps * 32), 0, st, a, (int)warps), "int4_read_kernel");
+    return cuda_status(launch_pdl(int4_read_kernel<T>, grid, dim3(kWarps * 32), 0, st, a, (int)warps),
+                       "int4_read_kernel");
   }
   const dim3 grid(((uint32_t)a.n_tokens + 7) / 8, num_seqs);
   if (kv->kv_dtype == DOE_KV_INT8)

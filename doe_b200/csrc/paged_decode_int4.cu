@@ -38,12 +38,20 @@
 // Work, see plan().  Many long rows (sequence, kv head): the blocks of all
 // sequences are one list cut into even pieces, each for one warp per kv head, so
 // that ragged lengths leave no tail; a row that pieces' ends cut is stitched by the
-// last of its warps to arrive.  Few rows: each is cut into splits of one length,
-// one CTA each; up to 8 of them form a cluster and join in distributed shared
-// memory, each CTA a slice of the dims, and the clusters are stitched per slice by
-// the last one to arrive.  Short rows, many of them: one CTA each.  Pieces and
-// splits follow from the lengths alone and sums go in the order of the keys, so
-// results do not depend on timing.
+// last of its warps to arrive.  Few rows: each is cut into splits, one CTA each,
+// as many as its share of all blocks; with very few, 8 of them form a cluster and
+// join in distributed shared memory, each CTA a slice of the dims, and the clusters
+// are stitched per slice by the last one to arrive.  Short rows, many of them: one
+// CTA each.  Pieces and splits follow from the lengths alone and sums go in the
+// order of the keys, so results do not depend on timing.
+//
+// What bounds it (8 kv heads, 4 query heads each, f32 output): 64 sequences of 1k-8k
+// tokens take 76.9 us for 341 MB (4.4 TB/s, 0.68 of the measured copy rate), 32 of
+// 8k-32k 145 us for 756 MB (5.2 TB/s, 0.80); the same walk without its arithmetic
+// 63 and 122 us.  A block costs a warp about 225 instructions (110 ALU, 65 FMA, 20
+// MMA), so a launch's issue slots are about as scarce as its bytes.  One sequence of
+// 130001 tokens (2 kv heads, 37.5 MB) takes 20 us: a launch, three dependent loads,
+// 11 blocks a warp, and two joins of 3 us each.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -63,10 +71,10 @@ constexpr int kBlkRing = 128;                  // block numbers per warp, renewe
 constexpr int kCtasPerSm = 3;                  // resident: 168 registers a thread
 constexpr int kRowCost = 4;                    // a sequence's fixed cost in the list, in blocks
 constexpr int kMinPiece = 8;                   // entries; more than kRowCost, so that no piece is empty
-constexpr uint64_t kListRows = 7;              // x rows from 4 warps' x resident CTAs on: the list
+constexpr uint64_t kListRows = 7;              // the list serves more rows than a 7th of the resident warps
 constexpr uint64_t kShortRow = 128;            // blocks that one CTA walks alone when there are rows enough
-constexpr uint64_t kLoneRow = 32;              // the same, when there are few rows
-constexpr uint64_t kMinSplit = 16;             // blocks
+constexpr uint64_t kLoneRow = 32;              // the same, when there are few rows (400 tokens: 6.4 us; in splits 7.5)
+constexpr uint64_t kMinSplit = 16;             // blocks (8: 10.4 us for 1 x 4000 tokens, 16: 9.1; 1 x 1024 7.3, 7.8)
 constexpr uint64_t kCounterBytes = 1 << 16;    // of the workspace's head, for 2048 rows' counters
 constexpr uint32_t kMaxListSeqs = 1024;        // sequences whose lengths a CTA adds up
 constexpr int kSlot = 2 * kI4Block;            // K block, V block
@@ -506,7 +514,8 @@ struct Walker {
           s[3] = n ? fmaf(s1, c[3], s[3]) : s1 * c[3];
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[u][i] = CAP ? fmaf(-2.0f * cap_log2, rcp(1.0f + ex2(s[i] * to_cap)), cap_log2) : s[i];
+        for (int i = 0; i < 4; ++i)
+          x[u][i] = CAP ? fmaf(-2.0f * cap_log2, rcp(1.0f + ex2(s[i] * to_cap)), cap_log2) : s[i];
       }
       const uint32_t v_at = wbase + slot + kI4Block + 16 * lane;
       refill = slot;
@@ -680,7 +689,8 @@ struct Joined {
 // The last part of a (row, slice of the dims) to finish stitches them, in key order.
 // T threads take every T-th part of four dims of a head each, so that one round
 // of loads reaches all parts (one thread each: 3 of them in turn for 24 parts).
-__device__ __forceinline__ void stitch_parts(const Args& a, size_t row, size_t part0, int rank, int slices, int nparts, int* last) {
+__device__ __forceinline__ void stitch_parts(const Args& a, size_t row, size_t part0, int rank, int slices, int nparts,
+                                             int* last) {
   __syncthreads();
   if (threadIdx.x == 0) *last = arrive_last(&a.counters[row * slices + rank], nparts);
   __syncthreads();
@@ -797,7 +807,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) splits_kernel(const A
   const int nparts = (nsplits + slices - 1) / slices;
   if (part >= nparts) return;             // the whole cluster; a split past the last joins with nothing
   if (nsplits == 1 && split != part * slices) return;  // nothing to join
-  const int tile_begin = split * split_tiles, tile_end = nsplits == 1 ? seq.tiles : min(seq.tiles, tile_begin + split_tiles);
+  const int tile_begin = split * split_tiles;
+  const int tile_end = nsplits == 1 ? seq.tiles : min(seq.tiles, tile_begin + split_tiles);
   const int span = tile_end - tile_begin - warp;
   const Stretch w = {b, g, seq.seq_len, seq.min_key, seq.origin + tile_begin + warp,
                      span > 0 ? (span + kWarps - 1) / kWarps : 0, 0, nsplits == 1};
@@ -918,9 +929,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) pieces_kernel(const A
     for (int i = b0; i < min(b0 + per, a.num_seqs); ++i) sm_end[i] += before;
     __syncthreads();
   }
-  // An item is a piece of one kv head, the head fastest: the warps of neighbouring
-  // items read neighbouring blocks of the same pages at about the same time
-  // (pieces of one head after another took 118 us where this takes 86).
+  // An item is a piece of one kv head, the head fastest
   const int total = sm_end[a.num_seqs - 1];  // below 2^29 (plan)
   const int most = (int)gridDim.x * kWarps / Hkv;                   // pieces (at least one: plan)
   const int size = max(kMinPiece, (total + most - 1) / most);        // of a piece
@@ -1124,7 +1133,19 @@ struct Plan {
 };
 
 // `tiles`: the most blocks of a row that can be read (its block-table row, or the
-// window).
+// window).  In order (times of this rule against the other one):
+//  - a given split_pages: splits of that length;
+//  - rows for every SM, of kShortRow blocks at most: one CTA each, nothing to join (32
+//    x 8 rows of 1024 tokens 16.7 us, of 2048 27; as a list 23 and 30);
+//  - rows below a seventh of the resident warps: splits by the lengths (24 x 8
+//    rows of 1k-8k 37.7 us, as a list 39.8; 16 x 8 of 1k-16k 43, 47.  From there
+//    on the list: 32 x 8 of 500-16k 71 us, 84 in splits; 32 x 8 of 8k-32k 145, 174).
+//    Their sum is what is resident at once: 3 CTAs per SM, or 384 in clusters of 8, which
+//    not every SM's place can join (1 x 130001 tokens, 2 kv heads: 27 us with 444).
+//    Clusters where a row gets more than 16 splits (that row without: 27 us in
+//    pairs, 20 in eights).  Splits that follow the table's width instead of the
+//    lengths cost 63 us against 19 for 4 x 8192 tokens in tables for 131072;
+//  - else the list, if the device can count its entries.
 Plan plan(uint64_t num_seqs, uint64_t kv_heads, uint64_t max_tiles, uint64_t tiles_per_page, uint64_t split_pages,
           uint64_t window) {
   Plan p = {};

@@ -123,7 +123,7 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     """Batched GQA decode: q [B,H,D] f16, seq_lens [B] int32 -> out [B,H,D] f32.
 
     With new_k/new_v ([B,Hkv,D] f16) the new token is first written at
-    position seq_lens[b] - 1 (quantised for int8 caches).  With freq_cis
+    position seq_lens[b] - 1 (quantised for int8 and int4 caches).  With freq_cis
     ([positions, D/2, 2] f32 RoPE table) the query and the new K row are
     rotated at position seq_lens[b] - 1 first (doe_paged_decode_rope).
     sliding_window > 0 keeps the last sliding_window keys and softcap > 0
@@ -141,6 +141,10 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     if out_dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("out_dtype must be float32 or bfloat16")
     B, H, D = q.shape
+    if cache.kv_dtype == "int4":
+        _check_int4(cache, B, D, (new_k, new_v), (B, cache.num_kv_heads, D))
+        if seq_lens.numel() != B:
+            raise ValueError(f"{B} queries, {seq_lens.numel()} seq_lens")
     out = torch.empty((B, H, D), dtype=out_dtype, device=q.device) if out is None else out
     _need(out, out_dtype, "out")
     flags = abi.DECODE_OUT_BF16 if out_dtype == torch.bfloat16 else 0
@@ -210,7 +214,7 @@ def decode_workspace(cache: PagedKVCache, num_seqs: int, num_heads: int, split_p
 
 
 def paged_append(cache: PagedKVCache, new_k, new_v, positions, status=None, stream=None, freq_cis=None):
-    """Write new_k/new_v [B,T,Hkv,D] f16 at positions[b] + t (quantising int8 caches).
+    """Write new_k/new_v [B,T,Hkv,D] f16 at positions[b] + t (quantising int8 and int4 caches).
 
     With freq_cis ([positions, D/2, 2] f32 RoPE table) each K row is first
     rotated at its position (doe_paged_append_rope)."""
@@ -218,6 +222,10 @@ def paged_append(cache: PagedKVCache, new_k, new_v, positions, status=None, stre
     _need(new_v, torch.float16, "new_v")
     _need(positions, torch.int32, "positions")
     B, T = new_k.shape[:2]
+    if cache.kv_dtype == "int4":
+        _check_int4(cache, B, new_k.shape[-1], (new_k, new_v), (B, T, cache.num_kv_heads, new_k.shape[-1]))
+        if positions.numel() != B:
+            raise ValueError(f"{B} chunks, {positions.numel()} positions")
     kv = cache.struct()
     l = _launch(0, status, stream, new_k.device)
     if freq_cis is None:
@@ -272,6 +280,16 @@ def paged_read(cache: PagedKVCache, positions, n_tokens: int, dtype=torch.float1
     abi.check("doe_paged_read", abi.lib().doe_paged_read(
         C.byref(kv), B, shape[1], positions.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], C.byref(l)))
     return k, v
+
+
+def _check_int4(cache: PagedKVCache, n: int, dim: int, rows, shape) -> None:
+    """n sequences of an int4 cache, dims `dim`, K and V rows (or None) of `shape`."""
+    _rows_of(cache, n)
+    if dim != cache.head_dim:
+        raise ValueError(f"head_dim {dim}, the cache has {cache.head_dim}")
+    for t, name in zip(rows, ("new_k", "new_v")):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float16 or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous f16 {list(shape)}")
 
 
 def _rows_of(cache: PagedKVCache, n: int) -> int:

@@ -441,3 +441,60 @@ def test_decode_few_rows_share_the_splits_by_length(lens, width, Hkv):
     c.check(out, 128 ** -0.5)
     assert np.array_equal(out, _decode(c)), "results depend on timing"
     c.check(_decode(c, sliding_window=1000), 128 ** -0.5, 1000)
+
+
+def test_refusals_of_shapes():
+    cache = PagedKVCache(num_pages=2, page_size=16, num_kv_heads=2, head_dim=128, block_table=np.array([[0, 1]]),
+                         kv_dtype="int4")
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    f16 = lambda *s: torch.zeros(s, dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError):
+        ops.paged_decode(cache, f16(2, 4, 128), i32(1, 1), 0.1)  # two sequences, one table row
+    with pytest.raises(ValueError):
+        ops.paged_decode(cache, f16(1, 4, 128), i32(1, 1), 0.1)
+    with pytest.raises(ValueError):
+        ops.paged_decode(cache, f16(1, 4, 64), i32(1), 0.1)
+    with pytest.raises(ValueError):
+        ops.paged_decode(cache, f16(1, 4, 128), i32(1), 0.1, new_k=f16(1, 1, 128), new_v=f16(1, 2, 128))
+    with pytest.raises(DoeError):
+        ops.paged_decode(cache, f16(1, 3, 128), i32(1), 0.1)  # 3 heads, 2 kv heads
+    with pytest.raises(DoeError):
+        ops.paged_decode(cache, f16(1, 18, 128), i32(1), 0.1)  # 9 heads per kv head
+    with pytest.raises(ValueError):
+        ops.paged_append(cache, f16(1, 3, 2, 128), f16(1, 3, 1, 128), i32(0))
+    with pytest.raises(ValueError):
+        ops.paged_append(cache, f16(1, 3, 2, 128), f16(1, 3, 2, 128), i32(0, 0))
+    with pytest.raises(ValueError):
+        ops.paged_append(cache, f16(2, 3, 2, 128), f16(2, 3, 2, 128), i32(0, 0))
+
+
+def test_backend_dispatch_of_an_int4_cache():
+    """kv_append_paged and attention_paged_decode with kv_dtype 2 give the operators' bytes."""
+    from doe_b200._abi import DOE_KV_INT4
+    from doe_b200.backend import Bind, CudaBackend
+
+    c = Case(41, [10, 200, 33], 2, 4)
+    B, T, Hkv, H = 3, 5, c.Hkv, c.H
+    nk, nv = _rows(c.g, (B, T, Hkv, 128)), _rows(c.g, (B, T, Hkv, 128))
+    starts = c.lens - T
+    cache = c.cache()
+    ops.paged_append(cache, _t(nk), _t(nv), _t(starts))
+    want = ops.paged_decode(cache, _t(c.q), _t(c.lens), 0.1).cpu().numpy()
+    be = CudaBackend(0)
+    try:
+        scale = int(np.float32(0.1).view(np.uint32))
+        uni = lambda *v: np.array(v, np.uint32)
+        for h, a in ((1, uni(B, T, Hkv, 128, 16, c.pages, c.table.shape[1], DOE_KV_INT4)), (2, nk), (3, nv), (4, c.kp),
+                     (5, c.vp), (6, c.table), (7, starts), (8, c.lens), (9, c.q),
+                     (10, uni(B, H, Hkv, 128, 16, c.pages, c.table.shape[1], DOE_KV_INT4, scale, 0))):
+            be.execute_buffer_write_bytes(h, 0, np.ascontiguousarray(a))
+        be.execute_kernel_dispatch("kv_append_paged", [Bind(0, 1, size=32)] + [Bind(i, i + 1) for i in range(1, 7)])
+        be.execute_kernel_dispatch("attention_paged_decode", [
+            Bind(0, 10, size=40), Bind(1, 9), Bind(2, 4), Bind(3, 5), Bind(4, 6), Bind(5, 8),
+            Bind(6, 11, size=B * H * 128 * 4)])
+        out = np.frombuffer(be.capture_buffer(11, 0, B * H * 128 * 4), np.float32).reshape(want.shape)
+        kp = np.frombuffer(be.capture_buffer(4, 0, c.kp.nbytes), np.uint8).reshape(c.kp.shape)
+    finally:
+        be.close()
+    assert np.array_equal(kp, cache.k_pool.cpu().numpy())
+    assert np.array_equal(out, want)

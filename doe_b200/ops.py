@@ -142,9 +142,14 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
         raise ValueError("out_dtype must be float32 or bfloat16")
     B, H, D = q.shape
     if cache.kv_dtype == "int4":
-        _check_int4(cache, B, D, (new_k, new_v), (B, cache.num_kv_heads, D))
-        if seq_lens.numel() != B:
-            raise ValueError(f"{B} queries, {seq_lens.numel()} seq_lens")
+        _rows_of(cache, B)
+        if D != cache.head_dim or seq_lens.numel() != B:
+            raise ValueError(f"q must be [B, H, {cache.head_dim}] and seq_lens [B]")
+        if new_k is not None and new_v is not None:
+            _need(new_k, torch.float16, "new_k")
+            _need(new_v, torch.float16, "new_v")
+            if not new_k.shape == new_v.shape == (B, cache.num_kv_heads, D):
+                raise ValueError(f"new_k and new_v must be [{B}, {cache.num_kv_heads}, {D}]")
     out = torch.empty((B, H, D), dtype=out_dtype, device=q.device) if out is None else out
     _need(out, out_dtype, "out")
     flags = abi.DECODE_OUT_BF16 if out_dtype == torch.bfloat16 else 0
@@ -223,9 +228,9 @@ def paged_append(cache: PagedKVCache, new_k, new_v, positions, status=None, stre
     _need(positions, torch.int32, "positions")
     B, T = new_k.shape[:2]
     if cache.kv_dtype == "int4":
-        _check_int4(cache, B, new_k.shape[-1], (new_k, new_v), (B, T, cache.num_kv_heads, new_k.shape[-1]))
-        if positions.numel() != B:
-            raise ValueError(f"{B} chunks, {positions.numel()} positions")
+        _rows_of(cache, B)
+        if not new_k.shape == new_v.shape == (B, T, cache.num_kv_heads, cache.head_dim) or positions.numel() != B:
+            raise ValueError(f"new_k and new_v must be [B, T, {cache.num_kv_heads}, {cache.head_dim}], positions [B]")
     kv = cache.struct()
     l = _launch(0, status, stream, new_k.device)
     if freq_cis is None:
@@ -268,7 +273,7 @@ def paged_read(cache: PagedKVCache, positions, n_tokens: int, dtype=torch.float1
     shape = (B, int(n_tokens), cache.num_kv_heads, cache.head_dim)
     if out is None:
         k = torch.empty(shape, dtype=dtype, device=positions.device)
-        v = torch.empty(shape, dtype=dtype, device=positions.device)
+        v = torch.empty_like(k)
     else:
         k, v = out
         for t, n in ((k, "out k"), (v, "out v")):
@@ -280,16 +285,6 @@ def paged_read(cache: PagedKVCache, positions, n_tokens: int, dtype=torch.float1
     abi.check("doe_paged_read", abi.lib().doe_paged_read(
         C.byref(kv), B, shape[1], positions.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], C.byref(l)))
     return k, v
-
-
-def _check_int4(cache: PagedKVCache, n: int, dim: int, rows, shape) -> None:
-    """n sequences of an int4 cache, dims `dim`, K and V rows (or None) of `shape`."""
-    _rows_of(cache, n)
-    if dim != cache.head_dim:
-        raise ValueError(f"head_dim {dim}, the cache has {cache.head_dim}")
-    for t, name in zip(rows, ("new_k", "new_v")):
-        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float16 or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous f16 {list(shape)}")
 
 
 def _rows_of(cache: PagedKVCache, n: int) -> int:
@@ -333,10 +328,10 @@ def token_logprobs(logits, tokens=None, top_k: int = 0, status=None, stream=None
         if tokens.numel() != rows:
             raise ValueError(f"{rows} rows of logits, {tokens.numel()} tokens")
     dev = logits.device
-    logprob = torch.empty(rows, dtype=torch.float32, device=dev) if tokens is not None else None
     entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
+    logprob = torch.empty_like(entropy) if tokens is not None else None
     top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    ids = torch.empty_like(top, dtype=torch.int32)
     l = _launch(0, status, stream, dev)
     abi.check("doe_token_logprobs", abi.lib().doe_token_logprobs(
         logits.data_ptr(), _DTYPES[logits.dtype], rows, vocab, max(logits.stride(0), vocab),

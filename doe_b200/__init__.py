@@ -9,6 +9,7 @@ views of its two surfaces:
   doe_b200.kv       -- the KV page pool and the device paged cache
   doe_b200.ort_ep   -- the ORT plugin EP's basic f32 operators (execute(kind, ...))
   doe_b200.decoder  -- a Llama-style decoder step on the library's kernels
+  doe_b200.beam     -- beam search over a decoder with a 4-bit KV cache
   doe_b200.tp       -- peer buffers for its tensor-parallel reduction
 """
 from ._abi import DoeError, lib  # noqa: F401

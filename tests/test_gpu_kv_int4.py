@@ -498,3 +498,34 @@ def test_backend_dispatch_of_an_int4_cache():
         be.close()
     assert np.array_equal(kp, cache.k_pool.cpu().numpy())
     assert np.array_equal(out, want)
+
+
+def test_a_captured_step_replays():
+    """Append, decode, read back, a page copy and the log probabilities in one CUDA graph."""
+    c = Case(51, [40, 3], 2, 4)
+    cache = c.cache()
+    g = np.random.default_rng(52)
+    nk, nv, q = _t(_rows(g, (2, 2, 128))), _t(_rows(g, (2, 2, 128))), _t(c.q)
+    chunk = _t(_rows(g, (2, 3, 2, 128)))
+    lens, zero = _t(c.lens), _t(np.zeros(2, np.int32))
+    logits, tokens = torch.randn((2, 5000), device="cuda"), torch.tensor([4, 9], dtype=torch.int32, device="cuda")
+    spare = next(p for p in range(c.pages) if p not in c.table)
+    pair = np.array([[int(c.table[0, 0]), spare]], np.int32)
+
+    def step(cache):
+        ops.paged_append(cache, chunk, chunk, zero)
+        out = ops.paged_decode(cache, q, lens, 0.1, new_k=nk, new_v=nv)
+        ops.paged_copy_pages(cache, pair)
+        return (out, *ops.paged_read(cache, zero, 3), *ops.token_logprobs(logits, tokens, top_k=3), cache.k_pool.clone())
+
+    want = [x.clone() for x in step(c.cache())]
+    step(cache)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(cache)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

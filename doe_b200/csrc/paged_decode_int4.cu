@@ -1201,7 +1201,8 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   const uint64_t rows = (uint64_t)num_seqs * Hkv;
   const Plan pl = plan(num_seqs ? num_seqs : 1, Hkv, max_tiles, tpp, split_pages, opts ? opts->sliding_window : 0);
   // The counters come first, in a region of one size for all but huge batches, so
-  // that decodes of any shapes can share a workspace whose counters stay zero.  A
+  // that decodes of any shapes can share a workspace whose counters stay zero; a
+  // huge batch's, which others' parts overwrite, are cleared by every launch.  A
   // part has O and, for each of up to 8 slices, (m, l) per head.
   const uint64_t ctr_bytes = (rows * 8 * sizeof(unsigned) + kCounterBytes - 1) / kCounterBytes * kCounterBytes;
   const uint64_t parts = pl.slots * group;
@@ -1270,7 +1271,8 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   a.out_bf16 = (opts && (opts->flags & DOE_DECODE_OUT_BF16)) ? 1 : 0;
   a.inputs_stable = (opts && (opts->flags & DOE_DECODE_INPUTS_STABLE)) ? 1 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(launch->stream);
-  if ((pl.list || pl.max_parts > 1) && !(opts && (opts->flags & DOE_DECODE_COUNTERS_ZEROED))) {
+  const bool zeroed = opts && (opts->flags & DOE_DECODE_COUNTERS_ZEROED) && ctr_bytes == kCounterBytes;
+  if ((pl.list || pl.max_parts > 1) && !zeroed) {
     const int rc =
         cuda_status(cudaMemsetAsync(a.counters, 0, rows * pl.slices * sizeof(unsigned), st), "cudaMemsetAsync(split counters)");
     if (rc != DOE_OK) return rc;

@@ -529,3 +529,18 @@ def test_a_captured_step_replays():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_decodes_of_any_shapes_share_a_stream():
+    """2400 rows in clusters of 8, whose counters outgrow the region that all shapes have in common,
+    between small decodes."""
+    big = Case(61, [1] * 260 + [200] * 40, 8, 1)
+    big.table = np.concatenate([big.table, np.full((300, 30), -1, np.int32)], 1)
+    small = Case(62, [5000, 300], 2, 4)
+    cb, cs = big.cache(), small.cache()
+    first, alone = _decode(big, cb, split_pages=1), _decode(small, cs)
+    big.check(first, 128 ** -0.5)
+    small.check(alone, 128 ** -0.5)
+    for _ in range(2):
+        assert np.array_equal(_decode(small, cs), alone)
+        assert np.array_equal(_decode(big, cb, split_pages=1), first)

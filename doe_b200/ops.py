@@ -132,7 +132,7 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     `ws`: a workspace kept for paged decodes alone, zeroed when created
     (decode_workspace); its split counters then need no clearing per call
     (DOE_DECODE_COUNTERS_ZEROED).  int4 caches keep one per stream by
-    themselves.  inputs_stable: seq_lens, the block table and
+    themselves (a captured graph gets its own).  inputs_stable: seq_lens, the block table and
     the pool rows (other than the appended ones) are final before the call is
     enqueued, so the first copies may start before the preceding kernel ends
     (DOE_DECODE_INPUTS_STABLE)."""
@@ -153,7 +153,9 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     out = torch.empty((B, H, D), dtype=out_dtype, device=q.device) if out is None else out
     _need(out, out_dtype, "out")
     flags = abi.DECODE_OUT_BF16 if out_dtype == torch.bfloat16 else 0
-    if ws is not None or cache.kv_dtype == "int4":
+    # a graph that is being captured holds a workspace of its own, cleared in every replay
+    keep = ws is None and cache.kv_dtype == "int4" and not torch.cuda.is_current_stream_capturing()
+    if ws is not None or keep:
         flags |= abi.DECODE_COUNTERS_ZEROED
     if inputs_stable:
         flags |= abi.DECODE_INPUTS_STABLE
@@ -165,8 +167,11 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
         l = _launch(need, status, stream, q.device)
     else:
         s = _stream_handle(stream, q.device)
-        if ws is None:
+        if keep:
             ws = _kept_workspace(need, q.device, s, stream)
+        elif ws is None:
+            with torch.cuda.stream(stream):
+                ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         elif ws.numel() < need:
             raise ValueError(f"decode workspace of {need} bytes needed, {ws.numel()} given")
         l = abi.Launch(s, ws.data_ptr(), ws.numel(), status.data_ptr() if status is not None else None)
@@ -193,22 +198,19 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     return out
 
 
-_DECODE_WS: dict[tuple[int, int], list[torch.Tensor]] = {}
+_DECODE_WS: dict[tuple[int, int], torch.Tensor] = {}
 
 
 def _kept_workspace(nbytes: int, device, handle: int, stream) -> torch.Tensor:
     """The int4 decodes' own workspace of a stream: its counters stay zero from call to call, whatever
-    the shapes (they come first), so no call clears them.  Outgrown ones are kept, for the CUDA graphs
-    that may hold them; a capture that needs a larger one gets its own."""
-    kept = _DECODE_WS.setdefault((device.index, handle), [])
-    if kept and kept[-1].numel() >= nbytes:
-        return kept[-1]
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    the shapes (they come first), so no call clears them."""
+    kept = _DECODE_WS.get((device.index, handle))
+    if kept is not None and kept.numel() >= nbytes:
+        return kept
     with torch.cuda.stream(stream):  # None: the current stream, which `handle` is then
-        buf = torch.zeros(max(nbytes, 1 << 22, 2 * kept[-1].numel() if kept else 0), dtype=torch.uint8, device=device)
-    kept.append(buf)
-    return buf
+        kept = torch.zeros(max(nbytes, 1 << 22), dtype=torch.uint8, device=device)
+    _DECODE_WS[device.index, handle] = kept
+    return kept
 
 
 def decode_workspace(cache: PagedKVCache, num_seqs: int, num_heads: int, split_pages: int = 0) -> torch.Tensor:

@@ -544,3 +544,25 @@ def test_decodes_of_any_shapes_share_a_stream():
     for _ in range(2):
         assert np.array_equal(_decode(small, cs), alone)
         assert np.array_equal(_decode(big, cb, split_pages=1), first)
+
+
+def test_a_captured_decode_does_not_use_the_streams_workspace():
+    """A graph captured on a stream that has decoded before, replayed beside decodes on that stream."""
+    c = Case(71, [3000, 2500], 2, 4)
+    cache, q, n = c.cache(), _t(c.q), _t(c.lens)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        want = ops.paged_decode(cache, q, n, 0.1).clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = ops.paged_decode(cache, q, n, 0.1)
+    outs = []
+    for _ in range(20):
+        with torch.cuda.stream(other):
+            graph.replay()
+        with torch.cuda.stream(side):
+            outs.append(ops.paged_decode(cache, q, n, 0.1))
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and all(torch.equal(o, want) for o in outs)

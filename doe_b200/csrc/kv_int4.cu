@@ -47,7 +47,9 @@ constexpr int kWarps = 4;
 // One warp per (sequence, 16-token block, kv head, K or V).  Half-warp hw takes the
 // token pairs 2 j + hw, lane l16 the dims [8 l16, 8 l16 + 8): one K word per token
 // and two V words per pair; a group's maximum is four lanes'.  All 16 rows (4 KB)
-// are loaded before any is quantised.
+// are loaded before any is quantised.  (A lane for a whole group of two tokens saves a
+// seventh of the instructions, 32.3 us against 33.7 for 32 x 512 tokens, but has four
+// times the RoPE work in a row: 11.1 against 10.0 for 1 x 8191, 7.3 against 6.5 for 32 x 1.)
 struct BlockWork {
   int b, h, kv;
   long long first;   // the block's first position

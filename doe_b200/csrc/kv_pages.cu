@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kThreads)
   uint4 v[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u)
-    if (i0 + u * kThreads < n) v[u] = ldg_stream(src + i0 + u * kThreads);
+    if (i0 + u * kThreads < n) v[u] = __ldcs(src + i0 + u * kThreads);
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u)
     if (i0 + u * kThreads < n) dst[i0 + u * kThreads] = v[u];

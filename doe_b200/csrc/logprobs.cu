@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         raw[u] = make_uint4(V::kLow, V::kLow, V::kLow, V::kLow);
-        if (inside(at + u * kThreads + tid)) raw[u] = ldg_stream(base + at + u * kThreads + tid);
+        if (inside(at + u * kThreads + tid)) raw[u] = __ldcs(base + at + u * kThreads + tid);
         ring[u * kThreads + tid] = raw[u];
       }
       if (at < whole0 || at + kStep > whole1) edge(at, 0, raw);

@@ -155,7 +155,7 @@ class PagedKVCache:
                         or t.numel() != self.num_pages * num_kv_heads * page_size):
                     raise ValueError("int8 scales must be contiguous CUDA f16 [pages, kv heads, page_size]")
         if not block_table.is_cuda or not block_table.is_contiguous() or block_table.ndim != 2 \
-                or block_table.element_size() != 4:
+                or block_table.dtype.itemsize != 4 or block_table.dtype.is_floating_point:
             raise ValueError("block_table must be a contiguous 2-D CUDA int32 tensor")
         self.num_kv_heads, self.head_dim, self.kv_dtype = num_kv_heads, head_dim, kv_dtype
         self.k_pool, self.v_pool, self.k_scale, self.v_scale = k_pool, v_pool, k_scale, v_scale

@@ -566,3 +566,29 @@ def test_a_captured_decode_does_not_use_the_streams_workspace():
             outs.append(ops.paged_decode(cache, q, n, 0.1))
     torch.cuda.synchronize()
     assert torch.equal(got, want) and all(torch.equal(o, want) for o in outs)
+
+
+def test_pools_and_pages_past_32_bit_offsets():
+    """4.3 GB pools: pages around the 2^31st and 2^32nd byte and the last ones."""
+    g = np.random.default_rng(81)
+    pages, n = 3_740_000, 100
+    cache = PagedKVCache(num_pages=pages, page_size=16, num_kv_heads=1, head_dim=128, block_table=np.zeros((1, 7)),
+                         kv_dtype="int4")
+    assert cache.k_pool.numel() > 2 ** 32
+    edge = [2 ** 31 // 1152, 2 ** 32 // 1152]
+    ids = [edge[0], edge[0] + 1, edge[1], edge[1] + 1, pages - 1, 0, pages - 2]
+    cache.set_block_table(np.array([ids], np.int32))
+    k, v, q = _rows(g, (1, n, 1, 128)), _rows(g, (1, n, 1, 128)), _rows(g, (1, 4, 128))
+    zero, length = _t(np.zeros(1, np.int32)), _t(np.array([n], np.int32))
+    status = ops.status_word()
+    ops.paged_append(cache, _t(k), _t(v), zero, status=status)
+    want = [kv_int4.values(*kv_int4.quantize(x)) for x in (k, v)]
+    for a, w in zip(ops.paged_read(cache, zero, n, dtype=torch.float32, status=status), want):
+        assert np.array_equal(a.cpu().numpy(), w.astype(np.float32))
+    out = ops.paged_decode(cache, _t(q), length, 0.1, status=status)[0].cpu().numpy()
+    ref, a = kv_int4.attend(q[0], want[0][0], want[1][0], 0.1)
+    assert (np.abs(out - ref) <= 2.0 ** -10 * (1 + 2.0 ** -4) * a + 2e-5 * np.abs(want[1]).max()).all()
+    ops.paged_copy_pages(cache, np.array([[i, 100 + j] for j, i in enumerate(ids)], np.int32))
+    cache.set_block_table(np.arange(100, 107, dtype=np.int32)[None])
+    assert np.array_equal(ops.paged_decode(cache, _t(q), length, 0.1, status=status)[0].cpu().numpy(), out)
+    assert int(status.item()) == 0

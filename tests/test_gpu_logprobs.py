@@ -189,3 +189,14 @@ def test_maxima_on_both_sides_of_the_exponents_two_forms(dtype, sign):
     x = torch.from_numpy(x.astype(np.float32)).to(DTYPES[dtype]).cuda()
     assert torch.isfinite(x[0]).all()
     _check(x, [0, 1, 4, 3], 7)
+
+
+def test_rows_past_32_bit_offsets():
+    """A row stride of over 2^32 elements."""
+    stride = 2 ** 32 + 24
+    store = torch.empty(stride + 5000, dtype=torch.float16, device="cuda")
+    x = store.as_strided((2, 5000), (stride, 1))
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    x.copy_(torch.randn((2, 5000), generator=g, device="cuda") * 3)
+    _check(x, [17, 4999], 6)

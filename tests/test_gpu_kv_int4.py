@@ -592,3 +592,16 @@ def test_pools_and_pages_past_32_bit_offsets():
     cache.set_block_table(np.arange(100, 107, dtype=np.int32)[None])
     assert np.array_equal(ops.paged_decode(cache, _t(q), length, 0.1, status=status)[0].cpu().numpy(), out)
     assert int(status.item()) == 0
+
+
+@pytest.mark.parametrize("seqs", [150, 200, 260, 1030])
+def test_decode_many_short_sequences_in_wide_tables(seqs):
+    """More rows than SMs, tables of over 2048 tokens: splits by length, the list, and past the list's sequences."""
+    g = np.random.default_rng(seqs)
+    lens = g.integers(0, 6, seqs)
+    lens[seqs // 2] = 700
+    c = Case(seqs, lens, 1, 4, 64)
+    c.table = np.concatenate([c.table, np.full((seqs, 40), -1, np.int32)], 1)
+    out = _decode(c)
+    c.check(out, 128 ** -0.5)
+    assert np.array_equal(out, _decode(c)), "results depend on timing"

@@ -48,8 +48,11 @@
 // What bounds it (8 kv heads, 4 query heads each, f32 output): 64 sequences of 1k-8k
 // tokens take 76.9 us for 341 MB (4.4 TB/s, 0.68 of the measured copy rate), 32 of
 // 8k-32k 145 us for 756 MB (5.2 TB/s, 0.80); the same walk without its arithmetic
-// 63 and 122 us.  A block costs a warp about 225 instructions (110 ALU, 65 FMA, 20
-// MMA), so a launch's issue slots are about as scarce as its bytes.  One sequence of
+// 63 and 122 us.  Over the batch sizes that is a line, 0.38 ns a block (6.1 TB/s) and
+// 20 us for a launch: its start (5 us until the first blocks arrive), the warps' uneven
+// ends (14 us from the first third of them to the last, which weighting their pieces
+// does not shorten) and the last stitch (8).  A block costs a warp about 225
+// instructions (110 ALU, 65 FMA, 20 MMA), half of the issue slots.  One sequence of
 // 130001 tokens (2 kv heads, 37.5 MB) takes 20 us: a launch, three dependent loads,
 // 11 blocks a warp, and two joins of 3 us each.
 #include <algorithm>
@@ -648,10 +651,10 @@ __device__ __forceinline__ void store_out(const Args& a, size_t row, int d, floa
 // Counts one part of a row in; true for the last of n.  The caller's threads have
 // met at a barrier after their writes and meet at one before they read the parts.
 __device__ __forceinline__ bool arrive_last(unsigned* counter, int n) {
-  asm volatile("fence.acq_rel.gpu;\n" ::: "memory");
-  const bool last = atomicAdd(counter, 1u) == (unsigned)(n - 1);
+  unsigned old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;\n" : "=r"(old) : "l"(counter) : "memory");
+  const bool last = old == (unsigned)(n - 1);
   if (last) *counter = 0u;  // ready for the next launch
-  asm volatile("fence.acq_rel.gpu;\n" ::: "memory");
   return last;
 }
 

@@ -31,7 +31,9 @@
 // Between cuts the warps run on without a barrier (one per step cost 40 of 155 us
 // at 1024 rows of 128256 bf16 logits), and a thread puts its own elements into the
 // buffer (a scan over the warp for their places cost 19 of 96 us).  A row that fills the buffer all the same
-// (rising ones) is gone over again with a cut whenever it is full.  Where fewer
+// (rising ones, or a mask that leaves a group nothing) is gone over again with a cut
+// whenever it is full; which of a step's elements fit is a matter of timing, so within
+// the step the bound is the k-th one's value and index.  Where fewer
 // than k elements lie above the first bound (rows that a mask or ties leave with
 // few values) the first ones that equal it are looked for in another pass.
 //
@@ -365,6 +367,29 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
     }
     return lost;
   };
+  // The same for elements whose key is above `kth`, of the step in slot 0.
+  auto push_keys = [&](uint32_t at, unsigned long long kth) {
+    constexpr uint32_t M = kUnroll * N;
+    auto key_at = [&](uint32_t e) {
+      const uint32_t u = e / N, i = e % N;
+      const float v = V::one(reinterpret_cast<const T*>(&ring[u * kThreads + tid]) + i);
+      return key_of(v, (at + u * kThreads + tid) * N + i - shift);
+    };
+    uint32_t n = 0;
+#pragma unroll 1
+    for (uint32_t e = 0; e < M; ++e) n += key_at(e) > kth;
+    if (n == 0) return false;
+    uint32_t pos = atomicAdd(&sh.count, n);
+    const bool lost = pos + n > kCap;
+#pragma unroll 1
+    for (uint32_t e = 0; e < M; ++e) {
+      const unsigned long long key = key_at(e);
+      if (key <= kth) continue;
+      if (pos < kCap) sh.buf[pos] = lost ? 0ull : key;
+      ++pos;
+    }
+    return lost;
+  };
   // An edge vector, element by element: those outside the row are -inf.
   auto edge = [&](uint32_t at, uint32_t slot, uint4 (&raw)[kUnroll]) {
 #pragma unroll
@@ -490,14 +515,18 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Args a, uin
       tmax = fmaxf(tmax, vmax);
       if (at == v0) bound = group_bound(sh, tmax, k);
       bool todo = true;
+      unsigned long long kth = 0;
       for (int round = 0;; ++round) {
-        todo = todo && vmax > bound && push(raw, at, 0, bound);
+        todo = todo && (kth == 0 ? vmax > bound && push(raw, at, 0, bound) : vmax >= bound && push_keys(at, kth));
         if (!__syncthreads_or(todo)) break;
         if (round == 0) {  // a new bound
           bound = fmaxf(bound, group_bound(sh, tmax, k));
           filter(sh, bound);
-        } else {  // full again: the best k so far are the bound
+        } else {
+          // full again: the best k so far are the bound, for the rest of this step by value and
+          // index, as elements left out may come before kept ones that they equal
           cut(sh, kCap, k, bound);
+          kth = sh.sel[k - 1];
         }
       }
     }

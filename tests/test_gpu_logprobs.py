@@ -200,3 +200,36 @@ def test_rows_past_32_bit_offsets():
     g.manual_seed(1)
     x.copy_(torch.randn((2, 5000), generator=g, device="cuda") * 3)
     _check(x, [17, 4999], 6)
+
+
+def _stable_ids(x, k):
+    return torch.sort(x.float(), dim=-1, descending=True, stable=True).indices[:, :k].int()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", ["plateau", "short", "holes"])
+def test_ties_behind_masked_stretches(dtype, case):
+    """A forbidden stretch leaves a group of threads without a maximum, so every allowed element is a
+    candidate and more of them are met than the buffer holds; which ones fit is a matter of timing."""
+    g = np.random.default_rng(11)
+    if case == "plateau":      # one value, the first allowed tokens far from the first thread's
+        x = np.zeros((4, 4096), np.float32)
+        x[:, :1536] = x[:, 2048:2112] = -np.inf
+        x[1, 1600:] = 1.0
+        x[2, 1536:1700] = -1.0
+        x[3, 1560::7] = 2.0
+        rows = [x]
+    elif case == "short":      # fewer groups hold an element than alternatives are asked for
+        rows = [g.integers(0, n, (8, V)).astype(np.float32) for V in (1025, 1056, 1100, 1537, 2000) for n in (2, 40)]
+    else:                      # a hole at the start of every split
+        x = g.integers(0, 3, (2, 131072)).astype(np.float32)
+        for s in range(0, 131072, 4096):
+            x[:, s:s + 64] = -np.inf
+        x[1] = np.where(np.isinf(x[1]), x[1], 0.5)
+        rows = [x]
+    for x in rows:
+        x = torch.from_numpy(x).to(DTYPES[dtype]).cuda()
+        for k in (20, 32):
+            want = _stable_ids(x, k)
+            got = [ops.token_logprobs(x, top_k=k).top_ids for _ in range(50)]
+            assert all(torch.equal(i, want) for i in got)

@@ -56,6 +56,7 @@
 // 130001 tokens (2 kv heads, 37.5 MB) takes 20 us: a launch, three dependent loads,
 // 11 blocks a warp, and two joins of 3 us each.
 #include <algorithm>
+#include <cmath>
 
 #include <cooperative_groups.h>
 
@@ -121,6 +122,14 @@ __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+// tanh within 2^-20 of its size: its Taylor series to y^7 (the next term is 3e-7 of it at 1/4)
+// and, from 1/4 on, 1 - 2 / (1 + e^2y), which cancels for small y.
+__device__ __forceinline__ float tanh_of(float y) {
+  const float t = y * y;
+  const float series = y * fmaf(t, fmaf(t, fmaf(t, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+  const float closed = fmaf(-2.0f, rcp(1.0f + ex2(y * (2.0f * kLog2e))), 1.0f);
+  return fabsf(y) < 0.25f ? series : closed;
 }
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // A block's 16-byte copies of one lane (two of K codes, two of V codes, one of
@@ -447,8 +456,7 @@ struct Walker {
     // x is the softcapped score in the log2 domain (CAP) or the bare product, which
     // c > 0 takes there: the sign of the scale is in Q, and a scale of 0 becomes
     // tiny so that the -inf of a dead key stays -inf
-    // CAP: softcap tanh(y) = softcap (1 - 2 / (1 + e^2y)), within about 2e-7 softcap
-    const float to_cap = 2.0f * kLog2e * kTwo24 * a.scale / a.softcap, cap_log2 = a.softcap * kLog2e;
+    const float to_cap = fminf(fmaxf(kTwo24 * a.scale / a.softcap, -3e38f), 3e38f), cap_log2 = a.softcap * kLog2e;
     const float c_log2 = CAP ? 1.0f : fmaxf(fabsf(a.scale) * (kLog2e * kTwo24), 1e-30f), inv_c = 1.0f / c_log2;
     int edge_k = first * 16 < min_key || bad ? 0 : nt - kStep;  // steps from here on have dead keys
     uint32_t slot = kSlot0, refill = 0;  // byte offsets in the ring
@@ -518,7 +526,7 @@ struct Walker {
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          x[u][i] = CAP ? fmaf(-2.0f * cap_log2, rcp(1.0f + ex2(s[i] * to_cap)), cap_log2) : s[i];
+          x[u][i] = CAP ? cap_log2 * tanh_of(s[i] * to_cap) : s[i];
       }
       const uint32_t v_at = wbase + slot + kI4Block + 16 * lane;
       refill = slot;
@@ -1255,7 +1263,9 @@ int launch_paged_decode_int4(const doe_paged_kv* kv, uint32_t num_seqs, uint32_t
   a.freq_cis = opts ? opts->freq_cis : nullptr;
   a.rope_positions = opts ? (int)opts->rope_positions : 0;
   a.window = opts ? (int)(opts->sliding_window > 0x7fffffffu ? 0x7fffffffu : opts->sliding_window) : 0;
-  a.softcap = opts ? opts->attn_softcap : 0.0f;
+  // A score is at most 128 * 65504^2 |scale| < 2^39 |scale|, and tanh(y) is y within 2^-25 below y =
+  // 2^-12: a cap from 2^51 |scale| on changes nothing.
+  a.softcap = opts && opts->attn_softcap < 0x1p51f * std::fabs(scale) ? opts->attn_softcap : 0.0f;
   a.scale = scale;
   a.num_heads = (int)num_heads;
   a.num_kv_heads = (int)Hkv;

@@ -605,3 +605,27 @@ def test_decode_many_short_sequences_in_wide_tables(seqs):
     out = _decode(c)
     c.check(out, 128 ** -0.5)
     assert np.array_equal(out, _decode(c)), "results depend on timing"
+
+
+@pytest.mark.parametrize("softcap", [1e3, 1e5, 1e8, 1e20, 3e38])
+@pytest.mark.parametrize("scale", [0.35, -0.35])
+def test_decode_large_softcaps(softcap, scale):
+    """Caps far above the scores, down to where the cap changes nothing.  Scores reach |s| < 24, and the
+    capped one is within 2^-20 of its own size, so each p is within 2^-19 |s| more than without a cap:
+    24 2^-19 on numerator and denominator add 10^-4 A to the bound."""
+    c = Case(16, [1, 33, 257], 1, 4)
+    out = _decode(c, softcap=softcap, scale=scale)
+    for b in range(3):
+        kk, vv = c.values(b)
+        assert np.abs(np.einsum("hd,td->ht", c.q[b].astype(np.float64), kk[:, 0])).max() * abs(scale) < 24
+        ref, a = kv_int4.attend(c.q[b], kk, vv, scale, 0, softcap)
+        bound = (2.0 ** -10 * (1 + 2.0 ** -4) + 1e-4) * a + 2e-5 * np.abs(vv).max()
+        assert (np.abs(out[b] - ref) <= bound).all()
+
+
+@pytest.mark.parametrize("softcap", [0.01, 1.0, 15.0, 100.0])
+def test_decode_softcap_on_both_sides_of_its_two_forms(softcap):
+    """Scores from a thousandth of the cap to many times it; the flat softmax shows small errors."""
+    c = Case(17, [400], 2, 4)
+    for scale in (1e-4 * softcap, 0.02 * softcap, 2.0 * softcap):
+        c.check(_decode(c, softcap=softcap, scale=scale), scale, 0, softcap)

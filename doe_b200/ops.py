@@ -131,7 +131,10 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     out_dtype torch.bfloat16 writes a bf16 output (DOE_DECODE_OUT_BF16).
     `ws`: a workspace kept for paged decodes alone, zeroed when created
     (decode_workspace); its split counters then need no clearing per call
-    (DOE_DECODE_COUNTERS_ZEROED).  int4 caches keep one per stream by
+    (DOE_DECODE_COUNTERS_ZEROED).  One tensor serves int4 caches, of any shapes,
+    or f16 and int8 ones (a call of another shape or type than the last one
+    clears them), and never both; what a graph was captured with serves no other
+    shape.  int4 caches keep one per stream by
     themselves (a captured graph gets its own).  inputs_stable: seq_lens, the block table and
     the pool rows (other than the appended ones) are final before the call is
     enqueued, so the first copies may start before the preceding kernel ends
@@ -155,14 +158,22 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     flags = abi.DECODE_OUT_BF16 if out_dtype == torch.bfloat16 else 0
     # a graph that is being captured holds a workspace of its own, cleared in every replay
     keep = ws is None and cache.kv_dtype == "int4" and not torch.cuda.is_current_stream_capturing()
-    if ws is not None or keep:
-        flags |= abi.DECODE_COUNTERS_ZEROED
     if inputs_stable:
         flags |= abi.DECODE_INPUTS_STABLE
     kv = cache.struct()
     lib = abi.lib()
     need = _decode_need(B, H, split_pages, cache.kv_dtype, cache.num_pages, cache.page_size, cache.num_kv_heads,
                         cache.head_dim, cache.max_pages_per_seq, q.device.index)
+    given = ws
+    if given is not None:
+        if given.numel() < need:
+            raise ValueError(f"decode workspace of {need} bytes needed, {given.numel()} given")
+        layout = "int4" if cache.kv_dtype == "int4" else (B * cache.num_kv_heads, need)
+        last = getattr(given, "_decode_layout", layout)
+        if (last == "int4") != (layout == "int4"):
+            raise ValueError("a decode workspace serves int4 caches or f16 and int8 ones, not both")
+    if keep or (given is not None and last == layout):
+        flags |= abi.DECODE_COUNTERS_ZEROED
     if ws is None and cache.kv_dtype != "int4":
         l = _launch(need, status, stream, q.device)
     else:
@@ -172,8 +183,6 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
         elif ws is None:
             with torch.cuda.stream(stream):
                 ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        elif ws.numel() < need:
-            raise ValueError(f"decode workspace of {need} bytes needed, {ws.numel()} given")
         l = abi.Launch(s, ws.data_ptr(), ws.numel(), status.data_ptr() if status is not None else None)
     nk = new_k.data_ptr() if new_k is not None else None
     nv = new_v.data_ptr() if new_v is not None else None
@@ -195,6 +204,8 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
         abi.check("doe_paged_decode_rope", lib.doe_paged_decode_rope(
             C.byref(kv), B, H, q.data_ptr(), seq_lens.data_ptr(), nk, nv, float(scale), out.data_ptr(),
             split_pages, freq_cis.data_ptr(), freq_cis.shape[0], C.byref(l)))
+    if given is not None:
+        given._decode_layout = layout
     return out
 
 
@@ -214,7 +225,7 @@ def _kept_workspace(nbytes: int, device, handle: int, stream) -> torch.Tensor:
 
 
 def decode_workspace(cache: PagedKVCache, num_seqs: int, num_heads: int, split_pages: int = 0) -> torch.Tensor:
-    """A zeroed workspace for paged decodes alone (pass as paged_decode(ws=...))."""
+    """A zeroed workspace for paged decodes of this kind of cache alone (pass as paged_decode(ws=...))."""
     kv = cache.struct()
     need = int(abi.lib().doe_paged_decode_workspace_bytes(C.byref(kv), num_seqs, num_heads, split_pages))
     return torch.zeros(max(need, 256), dtype=torch.uint8, device=cache.k_pool.device)

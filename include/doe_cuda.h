@@ -370,7 +370,14 @@ int doe_paged_decode_rope(const doe_paged_kv* kv, uint32_t num_seqs,
  *                              serves paged decodes only, the first of them
  *                              on zeroed memory; every decode that sets no
  *                              DOE_DEVICE_ERR_TIMEOUT leaves them zero), so
- *                              the per-call clear is skipped;
+ *                              the per-call clear is skipped.  The counters
+ *                              of int4 pools come first in the workspace:
+ *                              it serves any of their decodes and no other
+ *                              pool's.  Those of f16 and int8 pools come after
+ *                              partial sums: it serves decodes of one kv_dtype,
+ *                              num_seqs, heads, page and table size and
+ *                              split_pages (without the flag a decode clears
+ *                              its counters and takes any workspace);
  *                              DOE_DECODE_INPUTS_STABLE: seq_lens, the block
  *                              table and every pool row other than the rows
  *                              this call appends hold their final values

@@ -629,3 +629,59 @@ def test_decode_softcap_on_both_sides_of_its_two_forms(softcap):
     c = Case(17, [400], 2, 4)
     for scale in (1e-4 * softcap, 0.02 * softcap, 2.0 * softcap):
         c.check(_decode(c, softcap=softcap, scale=scale), scale, 0, softcap)
+
+
+def _f16_cache(seed, B, n, width):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    pages = B * width
+    cache = PagedKVCache(num_pages=pages, page_size=16, num_kv_heads=2, head_dim=128,
+                         block_table=np.arange(pages, dtype=np.int32).reshape(B, width))
+    for p in (cache.k_pool, cache.v_pool):
+        p.copy_(torch.randn(p.shape, generator=g, device="cuda"))
+    return cache, torch.randn((B, 8, 128), generator=g, device="cuda").half(), torch.full((B,), n, dtype=torch.int32,
+                                                                                          device="cuda")
+
+
+def test_a_kept_workspace_serves_one_kind_of_cache():
+    """int4 decodes keep their counters where the f16 and int8 decodes put partial sums: one workspace
+    for both is refused, whichever came first."""
+    c = Case(91, [3000, 2500], 2, 4)
+    cache = c.cache()
+    old, q, n = _f16_cache(1, 2, 3000, 188)
+    size = max(ops.decode_workspace(x, 2, 8).numel() for x in (cache, old))
+    for first in ("int4", "f16"):
+        ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+        four = lambda: _decode(c, cache, ws=ws)
+        half = lambda: ops.paged_decode(old, q, n, 0.1, ws=ws)
+        a, b = (four, half) if first == "int4" else (half, four)
+        a()
+        with pytest.raises(ValueError):
+            b()
+        a()
+    c.check(_decode(c, cache, ws=torch.zeros(size, dtype=torch.uint8, device="cuda")), 128 ** -0.5)
+
+
+def test_f16_decodes_of_several_shapes_on_one_workspace():
+    """Their counters lie behind partial sums whose size follows the shape: another shape clears them."""
+    shapes = [_f16_cache(2, 4, 3000, 188), _f16_cache(3, 1, 5000, 313), _f16_cache(4, 9, 700, 44)]
+    want = [ops.paged_decode(cache, q, n, 0.1).clone() for cache, q, n in shapes]
+    ws = torch.zeros(max(ops.decode_workspace(cache, q.shape[0], 8).numel() for cache, q, n in shapes), dtype=torch.uint8,
+                     device="cuda")
+    for _ in range(2):
+        for (cache, q, n), w in zip(shapes, want):
+            for _ in range(2):
+                out = torch.full_like(w, 7.0)
+                ops.paged_decode(cache, q, n, 0.1, ws=ws, out=out)
+                assert torch.equal(out, w)
+
+
+def test_int4_decodes_of_several_shapes_on_one_workspace():
+    cases = [Case(92, [3000, 2500], 2, 4), Case(93, [5000], 1, 8), Case(94, [700] * 9, 2, 2)]
+    caches = [c.cache() for c in cases]
+    want = [_decode(c, k) for c, k in zip(cases, caches)]
+    ws = torch.zeros(max(ops.decode_workspace(k, len(c.lens), c.H).numel() for c, k in zip(cases, caches)),
+                     dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        for c, k, w in zip(cases, caches, want):
+            assert np.array_equal(_decode(c, k, ws=ws), w)

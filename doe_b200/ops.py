@@ -157,7 +157,7 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     _need(out, out_dtype, "out")
     flags = abi.DECODE_OUT_BF16 if out_dtype == torch.bfloat16 else 0
     # a graph that is being captured holds a workspace of its own, cleared in every replay
-    keep = ws is None and cache.kv_dtype == "int4" and not torch.cuda.is_current_stream_capturing()
+    keep = ws is None and cache.kv_dtype == "int4" and not _capturing(stream)
     if inputs_stable:
         flags |= abi.DECODE_INPUTS_STABLE
     kv = cache.struct()
@@ -207,6 +207,14 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     if given is not None:
         given._decode_layout = layout
     return out
+
+
+def _capturing(stream) -> bool:
+    """Whether `stream`, or the current one, is being captured into a graph."""
+    if stream is None:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
 
 
 _DECODE_WS: dict[tuple[int, int], torch.Tensor] = {}

@@ -685,3 +685,32 @@ def test_int4_decodes_of_several_shapes_on_one_workspace():
     for _ in range(2):
         for c, k, w in zip(cases, caches, want):
             assert np.array_equal(_decode(c, k, ws=ws), w)
+
+
+def test_a_decode_captured_on_a_given_stream_has_its_own_workspace(monkeypatch):
+    """stream= names a stream that is being captured while the current one is not."""
+    c = Case(72, [3000, 2500], 2, 4)
+    cache, q, n = c.cache(), _t(c.q), _t(c.lens)
+    main, side, idle = (torch.cuda.Stream() for _ in range(3))
+    torch.cuda.synchronize()
+    want = ops.paged_decode(cache, q, n, 0.1, stream=side)
+    got = torch.empty_like(want)
+    torch.cuda.synchronize()
+
+    def kept(*_):
+        raise AssertionError("the stream's workspace went into the graph")
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        side.wait_stream(main)
+        with monkeypatch.context() as m:
+            m.setattr(ops, "_kept_workspace", kept)
+            with torch.cuda.stream(idle):
+                ops.paged_decode(cache, q, n, 0.1, out=got, stream=side)
+        main.wait_stream(side)
+    for _ in range(3):
+        got.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

@@ -134,7 +134,7 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     (DOE_DECODE_COUNTERS_ZEROED).  One tensor serves int4 caches, of any shapes,
     or f16 and int8 ones (a call of another shape or type than the last one
     clears them), and never both; what a graph was captured with serves no other
-    shape.  int4 caches keep one per stream by
+    shape.  int4 caches keep one per stream of torch's by
     themselves (a captured graph gets its own).  inputs_stable: seq_lens, the block table and
     the pool rows (other than the appended ones) are final before the call is
     enqueued, so the first copies may start before the preceding kernel ends
@@ -156,15 +156,16 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     out = torch.empty((B, H, D), dtype=out_dtype, device=q.device) if out is None else out
     _need(out, out_dtype, "out")
     flags = abi.DECODE_OUT_BF16 if out_dtype == torch.bfloat16 else 0
-    # a graph that is being captured holds a workspace of its own, cleared in every replay
-    keep = ws is None and cache.kv_dtype == "int4" and not _capturing(stream)
     if inputs_stable:
         flags |= abi.DECODE_INPUTS_STABLE
     kv = cache.struct()
     lib = abi.lib()
     need = _decode_need(B, H, split_pages, cache.kv_dtype, cache.num_pages, cache.page_size, cache.num_kv_heads,
                         cache.head_dim, cache.max_pages_per_seq, q.device.index)
-    given = ws
+    given, kept = ws, None
+    # a graph that is being captured holds a workspace of its own, cleared in every replay
+    if ws is None and cache.kv_dtype == "int4" and not _capturing(stream):
+        kept = ws = _kept_workspace(need, q.device, _stream_handle(stream, q.device), stream)
     if given is not None:
         if given.numel() < need:
             raise ValueError(f"decode workspace of {need} bytes needed, {given.numel()} given")
@@ -172,18 +173,16 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
         last = getattr(given, "_decode_layout", layout)
         if (last == "int4") != (layout == "int4"):
             raise ValueError("a decode workspace serves int4 caches or f16 and int8 ones, not both")
-    if keep or (given is not None and last == layout):
+    if kept is not None or (given is not None and last == layout):
         flags |= abi.DECODE_COUNTERS_ZEROED
     if ws is None and cache.kv_dtype != "int4":
         l = _launch(need, status, stream, q.device)
     else:
-        s = _stream_handle(stream, q.device)
-        if keep:
-            ws = _kept_workspace(need, q.device, s, stream)
-        elif ws is None:
+        if ws is None:
             with torch.cuda.stream(stream):
                 ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        l = abi.Launch(s, ws.data_ptr(), ws.numel(), status.data_ptr() if status is not None else None)
+        l = abi.Launch(_stream_handle(stream, q.device), ws.data_ptr(), ws.numel(),
+                       status.data_ptr() if status is not None else None)
     nk = new_k.data_ptr() if new_k is not None else None
     nv = new_v.data_ptr() if new_v is not None else None
     if sliding_window or softcap or flags:
@@ -220,13 +219,17 @@ def _capturing(stream) -> bool:
 _DECODE_WS: dict[tuple[int, int], torch.Tensor] = {}
 
 
-def _kept_workspace(nbytes: int, device, handle: int, stream) -> torch.Tensor:
+def _kept_workspace(nbytes: int, device, handle: int, stream) -> torch.Tensor | None:
     """The int4 decodes' own workspace of a stream: its counters stay zero from call to call, whatever
-    the shapes (they come first), so no call clears them."""
+    the shapes (they come first), so no call clears them.  It lasts as long as the process, as torch's
+    own streams do, of which there are a few dozen.  None for a stream that torch did not make: it can
+    be destroyed with work pending, and another stream get its handle."""
     kept = _DECODE_WS.get((device.index, handle))
     if kept is not None and kept.numel() >= nbytes:
         return kept
     with torch.cuda.stream(stream):  # None: the current stream, which `handle` is then
+        if handle and torch.cuda.current_stream(device).stream_id == handle:  # the id of a foreign stream
+            return None
         kept = torch.zeros(max(nbytes, 1 << 22), dtype=torch.uint8, device=device)
     _DECODE_WS[device.index, handle] = kept
     return kept

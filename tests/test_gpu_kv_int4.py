@@ -9,6 +9,8 @@ bf16 outputs are rounded once more (2^-8 |ref|).
 """
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -714,3 +716,29 @@ def test_a_decode_captured_on_a_given_stream_has_its_own_workspace(monkeypatch):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+def test_a_stream_of_the_callers_own_has_no_kept_workspace():
+    """A stream that torch did not make can be destroyed, and its handle be another stream's then."""
+    c = Case(73, [3000, 2500], 2, 4)
+    cache, q, n = c.cache(), _t(c.q), _t(c.lens)
+    want = ops.paged_decode(cache, q, n, 0.1)
+    made = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    before = set(ops._DECODE_WS)
+    handle = ctypes.c_void_p()
+    assert torch.cuda.cudart().cudaStreamCreate(ctypes.addressof(handle)) == 0
+    try:
+        s = torch.cuda.ExternalStream(handle.value)
+        outs = [ops.paged_decode(cache, q, n, 0.1, stream=s)]
+        with torch.cuda.stream(s):
+            outs.append(ops.paged_decode(cache, q, n, 0.1))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+        assert set(ops._DECODE_WS) == before
+        ops._DECODE_WS.pop((0, made.cuda_stream), None)
+        out = ops.paged_decode(cache, q, n, 0.1, stream=made)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and (0, made.cuda_stream) in ops._DECODE_WS
+    finally:
+        assert torch.cuda.cudart().cudaStreamDestroy(handle.value) == 0

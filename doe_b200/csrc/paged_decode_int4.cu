@@ -24,10 +24,13 @@
 // f32; P and s p are rounded to f16 (2^-11 relative at most, the f16 and int8
 // kernels' choice).
 //
-// The running reference of a head, m, is its score maximum plus the exponent
-// of the V scales seen, so that s p stays within f16's range and out of its
-// subnormals whatever the magnitude of V.  It is lazy: it moves only when a
-// score exceeds it by 2^8 or a V scale exceeds the exponent.
+// The running reference of a head, m, is its score maximum plus the exponent e of
+// the largest V scale seen, where that is within [-3, 1]; larger and smaller scales are
+// first multiplied by the power of two that takes e there, which comes off at the end.
+// So p and s p stay within f16's range, and a key down to 2^-17 of the largest one's
+// weight out of its subnormals, whatever the magnitude of V (scales below 2^-18 lose
+// that range by as much).  The reference is lazy: it moves only when a score exceeds it
+// by 2^8 or a V scale exceeds the exponent.
 //
 // Loads: a warp walks its blocks kStep at a time out of a ring of its own in
 // shared memory, filled with cp.async: a block is 1024 + 128 contiguous bytes
@@ -286,6 +289,7 @@ struct Sums {
   float m[2], l[2];   // reference and sum of p (of this lane's tokens)
   float acc[8][4];    // O^T: m-block 2 n + j, rows (lo, lo + 16 hi) of dims 32 n + 4 r + 2 j + {0, 1}
   float off[4];       // rows 2 n: 8 sum s p of group n
+  float unit;         // of acc and off
 };
 
 // A warp's ring of blocks and the walk over a stretch.
@@ -434,8 +438,10 @@ struct Walker {
     float (&off)[4] = sums.off;
     m_ref[0] = m_ref[1] = kNone;
     l_run[0] = l_run[1] = 0.0f;
-    int v_exp = -3;                // every V scale seen is at most 2^v_exp (or infinite)
-    uint32_t v_lim = 0x30003000u;  // 2^v_exp as an f16 pair
+    int v_exp = -18;               // every V scale seen is at most 2^v_exp (or infinite)
+    uint32_t v_lim = 0x00400040u;  // 2^v_exp as an f16 pair
+    uint32_t lift = 0x78007800u;   // 2^(middle(v_exp) - v_exp), what V scales are multiplied by, likewise
+    auto middle = [](int e) { return min(max(e, -3), 1); };
     float m_lim[2] = {kNone, kNone};  // x of a score 2^8 over its maximum
     off[0] = off[1] = off[2] = off[3] = 0.0f;
 #pragma unroll
@@ -570,18 +576,20 @@ struct Walker {
         const float vm = warp_max(fmaxf(vf.x, vf.y));
         int e = v_exp;
         if (vm > f2(v_lim).x) e = min(15, (int)((__float_as_uint(vm) >> 23) & 255) - 126);
+        const int mid = middle(e), drop = (mid - e) - (middle(v_exp) - v_exp);  // of the lift's exponent
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], o));
-          // reference = score maximum + exponent of the V scales - 4: p <= 2^15
+          // reference = score maximum + exponent of the lifted V scales - 4: p <= 2^15
           // and s p <= 2^12 while a score may still outgrow the maximum by 2^8
-          const float base = m_ref[j] - (float)(v_exp - 4);
-          const float top = fmaxf(base, mx[j] * c_log2), m_new = top + (float)(e - 4);
-          const float corr = ex2(m_ref[j] - m_new);
+          const float base = m_ref[j] - (float)(middle(v_exp) - 4);
+          const float top = fmaxf(base, mx[j] * c_log2), m_new = top + (float)(mid - 4);
+          float corr = ex2(m_ref[j] - m_new);
           m_ref[j] = m_new;
           m_lim[j] = (top + 8.0f) * inv_c;
           l_run[j] *= corr;
+          corr *= __uint_as_float((uint32_t)(127 + drop) << 23);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             acc[i][j] *= corr;
@@ -590,7 +598,19 @@ struct Walker {
           off[j] *= corr;
         }
         v_exp = e;
-        v_lim = (uint32_t)(e + 15) * 0x04000400u;
+        v_lim = e >= -14 ? (uint32_t)(e + 15) * 0x04000400u : 0x00010001u << (e + 24);
+        lift = (uint32_t)(mid - e + 15) * 0x04000400u;
+      }
+      if (lift != 0x3c003c00u) {
+#pragma unroll
+        for (int u = 0; u < kStep; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            vs[u][h].x = hmul2(vs[u][h].x, lift);
+            vs[u][h].y = hmul2(vs[u][h].y, lift);
+            vs[u][h].z = hmul2(vs[u][h].z, lift);
+            vs[u][h].w = hmul2(vs[u][h].w, lift);
+          }
       }
 
 #pragma unroll
@@ -620,6 +640,7 @@ struct Walker {
     }
     copy_wait<0>();
     __syncwarp();
+    sums.unit = kTwo24 * __uint_as_float((uint32_t)(127 + v_exp - middle(v_exp)) << 23);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -638,7 +659,7 @@ struct Walker {
         const float lo0 = s.acc[2 * n][j], lo1 = s.acc[2 * n + 1][j];
         const float hi0 = (s.acc[2 * n][2 + j] - lo0) * 0.0625f, hi1 = (s.acc[2 * n + 1][2 + j] - lo1) * 0.0625f;
         put(j, 32 * n + 4 * r,
-            make_float4((lo0 - o8) * kTwo24, (hi0 - o8) * kTwo24, (lo1 - o8) * kTwo24, (hi1 - o8) * kTwo24));
+            make_float4((lo0 - o8) * s.unit, (hi0 - o8) * s.unit, (lo1 - o8) * s.unit, (hi1 - o8) * s.unit));
       }
   }
 };

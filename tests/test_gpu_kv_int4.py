@@ -742,3 +742,28 @@ def test_a_stream_of_the_callers_own_has_no_kept_workspace():
         assert torch.equal(out, want) and (0, made.cuda_stream) in ops._DECODE_WS
     finally:
         assert torch.cuda.cudart().cudaStreamDestroy(handle.value) == 0
+
+
+@pytest.mark.parametrize("vstd", [1e-6, 1e-5, 1e-4, 1e-2, 1.0, 30.0, 1000.0, 9000.0])
+def test_decode_long_tails_at_every_magnitude_of_v(vstd):
+    """Each warp walks one key of 2^14.4 times the weight of its other 15000, which carry 0.4 of the sum.
+    s p is held in f16 over 17 powers of two below the largest key's, so a tail key's is rounded to 2^-11
+    of itself; p is too (2^-10 of the sum together, as V has one sign), and V is what the cache holds."""
+    n = 60000
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    pages = n // 16
+    cache = PagedKVCache(num_pages=pages, page_size=16, num_kv_heads=1, head_dim=128,
+                         block_table=np.arange(pages, dtype=np.int32)[None], kv_dtype="int4")
+    q = torch.ones((1, 4, 128), device="cuda").half()
+    k = torch.zeros((1, n, 1, 128), device="cuda").half()
+    k[0, [0, 16, 32, 48]] = 1.0  # one block of each of a CTA's four warps
+    v = (torch.randn((1, n, 1, 128), generator=g, device="cuda").abs() * vstd).clamp(max=65504.0).half()
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.paged_append(cache, k, v, zero)
+    scale = 14.4 * np.log(2) / 128
+    out = ops.paged_decode(cache, q, torch.full((1,), n, dtype=torch.int32, device="cuda"), scale, split_pages=pages)
+    kk, vv = (x[0, :, 0].double() for x in ops.paged_read(cache, zero, n, dtype=torch.float32))
+    p = torch.softmax((q[0].double() @ kk.T) * scale, -1)
+    ref = p @ vv
+    assert bool(((out[0].double() - ref).abs() <= 2.0 ** -9 * ref).all()), float(((out[0] - ref).abs() / ref).max())

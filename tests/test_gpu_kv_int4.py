@@ -767,3 +767,78 @@ def test_decode_long_tails_at_every_magnitude_of_v(vstd):
     p = torch.softmax((q[0].double() @ kk.T) * scale, -1)
     ref = p @ vv
     assert bool(((out[0].double() - ref).abs() <= 2.0 ** -9 * ref).all()), float(((out[0] - ref).abs() / ref).max())
+
+
+def _ragged(n, *more):
+    return [(7 * i * i) % 41 for i in range(n)] + list(more)
+
+
+# Each way a launch is cut up: lengths, kv heads, heads per kv head, unused pages per table row, window
+PLANS = {
+    "splits by length": (_ragged(9, 1, 2, 15, 16, 17, 31, 32, 33, 65, 300, 700), 2, 4, 0, 37),
+    "clusters by length": ([1, 2600, 17, 0, 300], 1, 5, 200, 2100),        # table of more than 256 blocks, few rows
+    "pieces of one list": (_ragged(130, 2300, 150, 2049), 2, 4, 0, 2100),   # more than a 7th of the warps' rows
+    "pieces, one head": (_ragged(256, 700, 2300), 1, 3, 0, 2250),
+    "a CTA a row": (_ragged(40, 300, 1, 129), 4, 2, 0, 100),                # tables of at most 128 blocks
+    "past the list": (_ragged(1028, 700, 40), 1, 1, 140, 2100),              # more than 1024 sequences
+}
+
+
+@pytest.mark.parametrize("rope,stable,windowed,softcap,bf16", [
+    (False, False, False, 0.0, False), (True, True, False, 0.0, True), (True, False, True, 0.0, False),
+    (False, True, True, 20.0, True)])
+@pytest.mark.parametrize("plan", PLANS)
+def test_decode_appends_in_every_plan(plan, rope, stable, windowed, softcap, bf16):
+    lens, Hkv, group, wide, window = PLANS[plan]
+    window = window if windowed else 0
+    c = Case(len(lens), lens, Hkv, group)
+    c.table = np.concatenate([c.table, np.full((len(lens), wide), -1, np.int32)], 1)
+    B = len(lens)
+    nk, nv = _rows(c.g, (B, Hkv, 128)), _rows(c.g, (B, Hkv, 128), 3.0)
+    last = c.lens.astype(np.int64) - 1
+    cis = rope_table(int(last.max()) + 1, 128, 10000.0)
+    rk, q = (kv_int4.rotate(nk, last, cis), kv_int4.rotate(c.q, last, cis)) if rope else (nk, c.q)
+    cache = c.cache()
+    out = _decode(c, cache, new_k=_t(nk), new_v=_t(nv), freq_cis=_t(cis) if rope else None, inputs_stable=stable,
+                  sliding_window=window, softcap=softcap, out_dtype=torch.bfloat16 if bf16 else torch.float32)
+    k, v = c.k.copy(), c.v.copy()
+    for b in range(B):
+        k[b, last[b]], v[b, last[b]] = rk[b], nv[b]  # of an empty sequence: a row that nobody reads
+    c.check(out, 128 ** -0.5, window, softcap, q=q, k=k, v=v, bf16=bf16)
+    kv_int4.append(c.kp, c.vp, c.table, 16, rk[:, None], nv[:, None], last)
+    assert np.array_equal(cache.k_pool.cpu().numpy(), c.kp), "the append wrote other K bytes"
+    assert np.array_equal(cache.v_pool.cpu().numpy(), c.vp), "the append wrote other V bytes"
+
+
+@pytest.mark.parametrize("plan", PLANS)
+def test_decode_reports_bad_pages_and_lengths_in_every_plan(plan):
+    """One sequence has pages outside the pool (their keys are left out), two have lengths outside the
+    table; the others are not touched."""
+    lens, Hkv, group, wide, _ = PLANS[plan]
+    c = Case(len(lens), lens, Hkv, group)
+    c.table = np.concatenate([c.table, np.full((len(lens), wide), -1, np.int32)], 1)
+    b = int(np.argmax(c.lens))
+    pages = -(-int(c.lens[b]) // 16)
+    bad = np.arange(pages)[1::3]
+    c.table[b, bad[::2]], c.table[b, bad[1::2]] = c.pages, -7
+    short = [i for i in range(len(lens)) if 0 < lens[i] < 20][:2]
+    given = c.lens.copy()
+    given[short[0]], given[short[1]] = -3, 10 ** 6  # nothing; the row up to its end, which is unmapped
+    status = ops.status_word()
+    out = ops.paged_decode(c.cache(), _t(c.q), _t(given), 128 ** -0.5, status=status).cpu().numpy()
+    assert int(status.item()) == DOE_DEVICE_ERR_PAGE | DOE_DEVICE_ERR_LENGTH
+    assert not out[short[0]].any()
+    keep = np.ones(int(c.lens[b]), bool)
+    for p in bad:
+        keep[16 * p:16 * p + 16] = False
+    for i in range(len(lens)):
+        if i == short[0]:
+            continue
+        kk, vv = c.values(i)
+        if i == short[1]:  # the last page's unwritten rows are attended too: anything
+            continue
+        if i == b:
+            kk, vv = kk[keep], vv[keep]
+        ref, a = kv_int4.attend(c.q[i], kk, vv, 128 ** -0.5)
+        bound = 2.0 ** -10 * (1 + 2.0 ** -4) * a + 2e-5 * (np.abs(vv).max() if len(vv) else 0.0)
+        assert (np.abs(out[i] - ref) <= bound).all(), i

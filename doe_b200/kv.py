@@ -99,6 +99,11 @@ class KvPool:
 KV_DTYPES = {"f16": abi.DOE_KV_F16, "int8": abi.DOE_KV_INT8, "int4": abi.DOE_KV_INT4}
 
 
+def _other_float(t) -> bool:
+    """Of a floating type whose bytes the kernels would read as something else (integers may hold raw bytes)."""
+    return t.dtype.is_floating_point and str(t.dtype) != "torch.float16"
+
+
 class PagedKVCache:
     """Device pools + block table for the paged kernels (torch tensors on one GPU)."""
 
@@ -146,17 +151,21 @@ class PagedKVCache:
         if row <= 0 or k_pool.numel() % row or k_pool.numel() != v_pool.numel():
             raise ValueError("k_pool and v_pool must hold the same whole number of pages")
         for p in (k_pool, v_pool):
-            if not p.is_cuda or not p.is_contiguous() or p.element_size() != itemsize:
-                raise ValueError(f"pools must be contiguous CUDA tensors of {itemsize}-byte elements")
+            if not p.is_cuda or not p.is_contiguous() or p.element_size() != itemsize or _other_float(p):
+                raise ValueError(f"pools must be contiguous CUDA tensors of {kv_dtype} ({itemsize}-byte) elements")
         self.num_pages, self.page_size = k_pool.numel() // row, page_size
         if kv_dtype == "int8":
             for t in (k_scale, v_scale):
-                if (not t.is_cuda or not t.is_contiguous() or t.element_size() != 2
+                if (not t.is_cuda or not t.is_contiguous() or t.element_size() != 2 or _other_float(t)
                         or t.numel() != self.num_pages * num_kv_heads * page_size):
                     raise ValueError("int8 scales must be contiguous CUDA f16 [pages, kv heads, page_size]")
         if not block_table.is_cuda or not block_table.is_contiguous() or block_table.ndim != 2 \
                 or block_table.dtype.itemsize != 4 or block_table.dtype.is_floating_point:
             raise ValueError("block_table must be a contiguous 2-D CUDA int32 tensor")
+        dev = k_pool.get_device()
+        if not dev == v_pool.get_device() == block_table.get_device() or (
+                kv_dtype == "int8" and not dev == k_scale.get_device() == v_scale.get_device()):
+            raise ValueError("pools, scales and block_table must be on one device")
         self.num_kv_heads, self.head_dim, self.kv_dtype = num_kv_heads, head_dim, kv_dtype
         self.k_pool, self.v_pool, self.k_scale, self.v_scale = k_pool, v_pool, k_scale, v_scale
         self.block_table, self.max_pages_per_seq = block_table, block_table.shape[1]

@@ -842,3 +842,22 @@ def test_decode_reports_bad_pages_and_lengths_in_every_plan(plan):
         ref, a = kv_int4.attend(c.q[i], kk, vv, 128 ** -0.5)
         bound = 2.0 ** -10 * (1 + 2.0 ** -4) * a + 2e-5 * (np.abs(vv).max() if len(vv) else 0.0)
         assert (np.abs(out[i] - ref) <= bound).all(), i
+
+
+@pytest.mark.parametrize("kv_dtype,good,bad", [("f16", torch.float16, torch.bfloat16), ("int8", torch.int8, torch.float8_e4m3fn),
+                                               ("int4", torch.uint8, torch.float8_e5m2)])
+def test_pools_of_another_floating_type_are_refused(kv_dtype, good, bad):
+    """Their elements have the size of the right ones, and would be read as those."""
+    n = 1152 if kv_dtype == "int4" else 16 * 128
+    pool = lambda dt: torch.zeros(n, dtype=dt, device="cuda")
+    scale = lambda dt: torch.zeros(16, dtype=dt, device="cuda") if kv_dtype == "int8" else None
+    make = lambda k, v, s: PagedKVCache.from_pools(k, v, page_size=16, num_kv_heads=1, head_dim=128, kv_dtype=kv_dtype,
+                                                   block_table=_t(np.zeros((1, 1), np.int32)), k_scale=s, v_scale=s)
+    assert make(pool(good), pool(good), scale(torch.float16)).num_pages == 1
+    with pytest.raises(ValueError):
+        make(pool(bad), pool(good), scale(torch.float16))
+    with pytest.raises(ValueError):
+        make(pool(good), pool(bad), scale(torch.float16))
+    if kv_dtype == "int8":
+        with pytest.raises(ValueError):
+            make(pool(good), pool(good), scale(torch.bfloat16))

@@ -162,10 +162,12 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
     lib = abi.lib()
     need = _decode_need(B, H, split_pages, cache.kv_dtype, cache.num_pages, cache.page_size, cache.num_kv_heads,
                         cache.head_dim, cache.max_pages_per_seq, q.device.index)
+    shared = ws is None and cache.kv_dtype != "int4"  # the workspace of all operators
+    s = None if shared else _stream_handle(stream, q.device)
     given, kept = ws, None
     # a graph that is being captured holds a workspace of its own, cleared in every replay
-    if ws is None and cache.kv_dtype == "int4" and not _capturing(stream):
-        kept = ws = _kept_workspace(need, q.device, _stream_handle(stream, q.device), stream)
+    if ws is None and not shared and not _capturing(stream):
+        kept = ws = _kept_workspace(need, q.device, s, stream)
     if given is not None:
         if given.numel() < need:
             raise ValueError(f"decode workspace of {need} bytes needed, {given.numel()} given")
@@ -175,14 +177,13 @@ def paged_decode(cache: PagedKVCache, q, seq_lens, scale: float, new_k=None, new
             raise ValueError("a decode workspace serves int4 caches or f16 and int8 ones, not both")
     if kept is not None or (given is not None and last == layout):
         flags |= abi.DECODE_COUNTERS_ZEROED
-    if ws is None and cache.kv_dtype != "int4":
+    if shared:
         l = _launch(need, status, stream, q.device)
     else:
         if ws is None:
             with torch.cuda.stream(stream):
                 ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        l = abi.Launch(_stream_handle(stream, q.device), ws.data_ptr(), ws.numel(),
-                       status.data_ptr() if status is not None else None)
+        l = abi.Launch(s, ws.data_ptr(), ws.numel(), status.data_ptr() if status is not None else None)
     nk = new_k.data_ptr() if new_k is not None else None
     nv = new_v.data_ptr() if new_v is not None else None
     if sliding_window or softcap or flags:

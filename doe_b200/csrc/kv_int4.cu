@@ -6,7 +6,7 @@
 //
 // Copies with a little arithmetic: 512 bytes of f16 K and V against 144 bytes of
 // blocks per (token, kv head).  Writing 32 x 512 tokens of 8 kv heads and reading them
-// back takes 33.7 us for 172 MB (5.1 TB/s, 0.78 of the measured copy rate); the write
+// back takes 33.4 us for 172 MB (5.1 TB/s, 0.79 of the measured copy rate); the write
 // alone is near 20, bound by issue slots (79 instructions for a token's K or V of a
 // head, half of the cycles) and by how many loads 20 warps an SM keep in flight, the
 // read near 14, bound by HBM writes and the two loads before its own.  32 tokens
@@ -367,7 +367,9 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const PagedReadA
 }
 
 // f16 and int8 rows: one warp per (sequence, token), lanes over Hkv * D in
-// runs of 8.
+// runs of 8.  Bound by HBM writes and, for int8, by a scale load per run: 32 x 512 tokens
+// of 8 kv heads as f16 take 26.8 us from f16 pools (134 MB, 0.77 of the measured copy
+// rate), 25.8 from int8 (101 MB, 0.60).
 template <typename T, bool INT8>
 __global__ void __launch_bounds__(256) paged_read_kernel(const PagedReadArgs a) {
   const int tok = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, b = blockIdx.y;

@@ -49,7 +49,7 @@
 // order of the keys, so results do not depend on timing.
 //
 // What bounds it (8 kv heads, 4 query heads each, f32 output): 64 sequences of 1k-8k
-// tokens take 76.9 us for 341 MB (4.4 TB/s, 0.68 of the measured copy rate), 32 of
+// tokens take 76.8 us for 341 MB (4.4 TB/s, 0.68 of the measured copy rate), 32 of
 // 8k-32k 145 us for 756 MB (5.2 TB/s, 0.80); the same walk without its arithmetic
 // 63 and 122 us.  Over the batch sizes that is a line, 0.38 ns a block (6.1 TB/s) and
 // 20 us for a launch: its start (5 us until the first blocks arrive), the warps' uneven
@@ -475,8 +475,8 @@ struct Walker {
           bad |= __any_sync(0xffffffffu, i < nt && ahead == kDead);
         }
         // the -8 comes off the sums now and then: the tensor core truncates what it adds
-        // to, and sums of codes from 1 on grow as sums of values do not (0.0018 of
-        // O at 20000 tokens without this)
+        // to, and sums of codes from 1 on grow as sums of values do not (0.0020 of
+        // O at 20000 tokens without this, 0.0004 with it)
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
